@@ -623,6 +623,50 @@ int w3d_raster_blend_backward(const float *splats, int P, int H, int W, int tile
 int w3d_raster_preprocess_backward(const W3dRasterIn *in, const int32_t *radii, const void *geom_buffer,
                                    W3dRasterGradOut *gout, w3d_stream_t stream);
 
+/* ---- layers of a feature head (no counterpart in the reference): rows of any width -> the rows the match takes.
+ * Row-major, contiguous; any row count (0 is a no-op), any width, any element alignment of the pointers; aligned tensors (16 B, widths that are multiples of 16 B) run fastest.
+ * dtype: W3D_DTYPE_F32 / BF16 / F16 for rows, weights, residual and outputs alike; weight_dtype / bias_dtype (norm weight, biases): dtype or W3D_DTYPE_F32.
+ * All sums are f32, outputs are rounded once.  Results do not depend on the launch (no atomics).  Workspaces: 16-byte aligned, contents irrelevant before and after, one per call in flight.
+ *
+ * Root-mean-square norm: s = x + residual (residual NULL: s = x); rstd = 1 / sqrt(mean(s^2) + eps); y = s * rstd * weight (weight NULL: 1).
+ *   w3d_rms_norm_fwd: y [R,d]; s [R,d] (optional, only with a residual; the sum, rounded); rstd f32 [R] (optional, for the backward pass).
+ *   w3d_rms_norm_fp8: the same y as e4m3 bytes q [R,d] + E8M0 exponents [R] (the format and the scale rule of w3d_quantize_rows_fp8), s optional as above.
+ *   w3d_rms_norm_bwd: from s (x without a residual), rstd, dy and ds (gradient that reaches s itself, optional): dx [R,d] (also the residual's gradient) and / or dweight [d]
+ *     (of weight_dtype; needs the workspace). */
+int w3d_rms_norm_fwd(const void *x, const void *residual, const void *weight, int weight_dtype, int64_t R, int d, int dtype, float eps, void *y, void *s, float *rstd,
+                     w3d_stream_t stream);
+int w3d_rms_norm_fp8(const void *x, const void *residual, const void *weight, int weight_dtype, int64_t R, int d, int dtype, float eps, void *q, int32_t *scale_e8m0, void *s,
+                     w3d_stream_t stream);
+size_t w3d_rms_norm_bwd_workspace_bytes(int64_t R, int d);
+int w3d_rms_norm_bwd(const void *s, const void *weight, int weight_dtype, const float *rstd, const void *dy, const void *ds, int64_t R, int d, int dtype, void *dx, void *dweight,
+                     void *workspace, size_t workspace_bytes, w3d_stream_t stream);
+/* Linear layer: y = act(x W^T + bias) + residual;  x [R,K], w [N,K], bias [N] or NULL, residual [R,N] or NULL, y [R,N].
+ * Gated linear layer: y = act(x Wg^T + bg) * (x Wu^T + bu), one launch for both products.
+ * act: W3D_ACT_*; gelu is z * Phi(z).  Rows of x, w and y shorter than 8 MB (W3D_ERR_UNSUPPORTED otherwise).
+ * The _fp8 forms take e4m3 rows with one E8M0 exponent (1..254) each for x AND the weights, and write bf16 or f16 (residual and biases of out_dtype, biases also f32).
+ * The _bwd forms need the forward's inputs (they form z again) and dy [R,N]: dx [R,K], dw [N,K], dbias [N] (of bias_dtype), each optional; the residual's gradient is dy itself.
+ * workspace: w3d_linear_workspace_bytes (dtype W3D_DTYPE_FP8_E4M3 for the _fp8 forms) / w3d_linear_bwd_workspace_bytes. */
+#define W3D_ACT_NONE 0
+#define W3D_ACT_RELU 1
+#define W3D_ACT_GELU 2
+#define W3D_ACT_SILU 3
+#define W3D_ACT_SIGMOID 4
+size_t w3d_linear_workspace_bytes(int64_t R, int64_t K, int64_t N, int dtype, int gated);
+size_t w3d_linear_bwd_workspace_bytes(int64_t R, int64_t K, int64_t N, int dtype, int act, int gated);
+int w3d_linear_fwd(const void *x, const void *w, const void *bias, int bias_dtype, const void *residual, int64_t R, int64_t K, int64_t N, int dtype, int act, void *y,
+                   void *workspace, size_t workspace_bytes, w3d_stream_t stream);
+int w3d_linear_fp8_fwd(const void *x, const int32_t *x_scale, const void *w, const int32_t *w_scale, const void *bias, int bias_dtype, const void *residual, int64_t R, int64_t K,
+                       int64_t N, int out_dtype, int act, void *y, void *workspace, size_t workspace_bytes, w3d_stream_t stream);
+int w3d_linear_bwd(const void *x, const void *w, const void *bias, int bias_dtype, const void *dy, int64_t R, int64_t K, int64_t N, int dtype, int act, void *dx, void *dw,
+                   void *dbias, void *workspace, size_t workspace_bytes, w3d_stream_t stream);
+int w3d_gated_linear_fwd(const void *x, const void *w_gate, const void *w_up, const void *b_gate, const void *b_up, int bias_dtype, int64_t R, int64_t K, int64_t N, int dtype,
+                         int act, void *y, void *workspace, size_t workspace_bytes, w3d_stream_t stream);
+int w3d_gated_linear_fp8_fwd(const void *x, const int32_t *x_scale, const void *w_gate, const int32_t *gate_scale, const void *w_up, const int32_t *up_scale, const void *b_gate,
+                             const void *b_up, int bias_dtype, int64_t R, int64_t K, int64_t N, int out_dtype, int act, void *y, void *workspace, size_t workspace_bytes,
+                             w3d_stream_t stream);
+int w3d_gated_linear_bwd(const void *x, const void *w_gate, const void *w_up, const void *b_gate, const void *b_up, int bias_dtype, const void *dy, int64_t R, int64_t K, int64_t N,
+                         int dtype, int act, void *dx, void *dw_gate, void *dw_up, void *db_gate, void *db_up, void *workspace, size_t workspace_bytes, w3d_stream_t stream);
+
 /* GaussianRasterizer.markVisible (RAST/diff_gaussian_rasterization/__init__.py:192-201) */
 int w3d_mark_visible(const float *means3D, const float *viewmatrix, const float *projmatrix, int P,
                      uint8_t *present, w3d_stream_t stream);

@@ -20,14 +20,19 @@ FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wno-unused-re
          "-I/opt/rocm/include", "-DROCPRIM_NO_DEPRECATED_WARNINGS"]
 
 
+# no packed f32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on this hardware
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 # per-file additions.  knn_mfma.hip: scores are compared with fmaxf trees; without "no NaNs" every fmaxf input gets a canonicalising
 # v_max_f32 x, x (15 instead of 9 VALU per 32x32 block in the selection pretest).  Infinities stay honoured (they are the sentinels).
-EXTRA_FLAGS = {"knn_mfma.hip": ["-fno-honor-nans"]}
+EXTRA_FLAGS = {"knn_mfma.hip": ["-fno-honor-nans"], "rms_norm.hip": NO_PACKED_F32, "columns.hip": NO_PACKED_F32, "linear.hip": NO_PACKED_F32}
 
 
 # knn_mfma.hip is compiled into a main object (entry points, dispatch) and one leaf object per (operand format, feature width): the leaves hold the kernel
 # instantiations of one shape each and compile in parallel (a single translation unit took six minutes)
 KNN_LEAVES = [(f, d) for f in (0, 1) for d in (64, 128, 256)] + [(2, 128), (2, 256)]
+# linear.hip: the entry points and one leaf per operand type (f32, bf16, f16, fp8) with its tile kernels
+LINEAR_LEAVES = (0, 1, 2, 3)
 
 
 def sources():
@@ -44,6 +49,9 @@ def units():
         if base == "knn_mfma.hip":
             for f, d in KNN_LEAVES:
                 out.append((src, os.path.join(OBJ, f"knn_mfma_f{f}_d{d}.o"), extra + [f"-DW3D_KNN_FMT={f}", f"-DW3D_KNN_D={d}"]))
+        if base == "linear.hip":
+            for dt in LINEAR_LEAVES:
+                out.append((src, os.path.join(OBJ, f"linear_t{dt}.o"), extra + [f"-DW3D_LIN_DT={dt}"]))
     return out
 
 

@@ -1,0 +1,490 @@
+// Linear and gated linear layers on feature rows: z = x W^T + b;  y = act(z) + residual  /  y = act(x Wg^T + bg) * (x Wu^T + bu), and their gradients.
+//
+// Three kernels do the products (gemm_tile.h has the tile):
+//   * few rows (<= SKINNY_ROWS): the weights are read once, straight into MFMA fragments, by as many waves as there are; the rows are the other operand
+//   * tiles of 128 x 128 through LDS
+//   * when the tiles are few for 256 CUs the contraction is cut into slices; partial tiles are added in slice order, and the epilogue applied, by a second launch
+//
+// Backward keeps nothing of the forward pass but its inputs: z is formed again and turned into dz in the epilogue, where the column sums for the bias
+// gradient are taken too — storing z in 16 bits would put its rounding into every gradient, storing it in 32 costs more traffic than forming it again
+// (R x N x 12 bytes written and read, against 2 R N K operations).  dz is rounded once to the operands' type (it is an operand of two products); sums are f32.
+//
+// One translation unit per operand type (W3D_LIN_DT: the tiles), one for the entry points.
+#include "gemm_tile.h"
+
+int w3d_fold_columns(const float *part, int parts, int64_t ld, int64_t n, void *out, int out_dtype, hipStream_t st);      // columns.hip
+int w3d_column_strips(int64_t R, int64_t n);
+int w3d_column_sums(const void *x, int64_t R, int64_t n, int dtype, float *part, int64_t ld, hipStream_t st);
+
+namespace {
+enum { PROD_LINEAR = 0, PROD_GATED = 1, PROD_LINEAR_BWD = 2, PROD_GATED_BWD = 3, PROD_DX = 4, PROD_DW = 5 };
+constexpr int SKINNY_ROWS = 64;
+}  // namespace
+
+// launches of one operand type's kernels
+int w3d_lin_tiles_f32(const GemmArgs &a, int prod, bool aligned, int z, hipStream_t st);
+int w3d_lin_tiles_bf16(const GemmArgs &a, int prod, bool aligned, int z, hipStream_t st);
+int w3d_lin_tiles_f16(const GemmArgs &a, int prod, bool aligned, int z, hipStream_t st);
+int w3d_lin_tiles_fp8(const GemmArgs &a, int prod, bool aligned, int z, hipStream_t st);
+int w3d_lin_skinny_f32(const GemmArgs &a, int prod, hipStream_t st);
+int w3d_lin_skinny_bf16(const GemmArgs &a, int prod, hipStream_t st);
+int w3d_lin_skinny_f16(const GemmArgs &a, int prod, hipStream_t st);
+int w3d_lin_skinny_fp8(const GemmArgs &a, int prod, hipStream_t st);
+
+#ifdef W3D_LIN_DT
+namespace {
+
+template <int LX, int LW, int EPI, int BM, int BN, int WM, int WN, bool ALIGNED>
+int launch_tiles(const GemmArgs &a, int z, hipStream_t st) {
+    typedef Gemm<W3D_LIN_DT, LX, LW, EPI, BM, BN, WM, WN, ALIGNED> G;
+    auto kernel = gemm_kernel<W3D_LIN_DT, LX, LW, EPI, BM, BN, WM, WN, ALIGNED>;
+    if (G::LDS_BYTES > 65536) W3D_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS_BYTES));
+    const int64_t blocks = (int64_t)a.tiles_m * a.tiles_n * a.slices;
+    if (blocks < 1 || blocks > 0x7fffffff) return W3D_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, 1, z), dim3(G::NT), G::LDS_BYTES, st, a);
+    W3D_CHECK_LAUNCH();
+    return W3D_OK;
+}
+template <int LX, int LW, int EPI>
+int launch_shape(const GemmArgs &a, bool aligned, int z, hipStream_t st) {
+    if (!aligned) return launch_tiles<LX, LW, EPI, 128, 128, 2, 2, false>(a, z, st);
+    return launch_tiles<LX, LW, EPI, 128, 128, 2, 2, true>(a, z, st);
+}
+int launch_prod(const GemmArgs &a, int prod, bool aligned, int z, hipStream_t st) {
+    switch (prod) {
+        case PROD_LINEAR: return launch_shape<K_ROWS, K_ROWS, EPI_LINEAR>(a, aligned, z, st);
+        case PROD_GATED: return launch_shape<K_ROWS, K_ROWS, EPI_GATED>(a, aligned, z, st);
+        default: break;
+    }
+    if constexpr (W3D_LIN_DT != W3D_DTYPE_FP8_E4M3) {
+        switch (prod) {
+            case PROD_LINEAR_BWD: return launch_shape<K_ROWS, K_ROWS, EPI_LINEAR_BWD>(a, aligned, z, st);
+            case PROD_GATED_BWD: return launch_shape<K_ROWS, K_ROWS, EPI_GATED_BWD>(a, aligned, z, st);
+            case PROD_DX: return launch_shape<K_ROWS, M_ROWS, EPI_STORE>(a, aligned, z, st);
+            case PROD_DW: return launch_shape<M_ROWS, M_ROWS, EPI_STORE>(a, aligned, z, st);
+            default: break;
+        }
+    }
+    return W3D_ERR_UNSUPPORTED;
+}
+
+// ---- few rows.  Bound by the weights: every one is read once.  A block owns 16 columns (of each half of a gated layer); its waves share the contraction in turns of STEP_RUN steps of 64
+// bytes, a lane loading 16 bytes of one weight row per step, so that a row's 256 consecutive bytes are in flight together; rows of any alignment are read in place.  The waves' partial
+// sums meet in LDS.
+template <int EPI, int RF>
+__global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
+    constexpr int DT = W3D_LIN_DT, EB = Elem<DT>::B, WAVES = 8, KPSTEP = 64 / EB, STEP_RUN = 4;
+    constexpr bool GATED = EPI == EPI_GATED;
+    constexpr int PARTS = GATED ? 2 : 1;
+    __shared__ f32x4 sums[WAVES][PARTS * RF][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * 16;
+    const int64_t n = n0 + (lane & 15) < a.N ? n0 + (lane & 15) : a.N - 1;                    // (rows past the end: the last one again, never stored)
+    const uint8_t *wr[PARTS];
+    wr[0] = a.w + n * a.ldw;
+    if (GATED) wr[PARTS - 1] = a.w2 + n * a.ldw;
+    const uint8_t *xr[RF];
+#pragma unroll
+    for (int i = 0; i < RF; ++i) {
+        const int64_t m = 16 * i + (lane & 15);
+        xr[i] = a.x + (m < a.M ? m : a.M - 1) * a.ldx;
+    }
+    f32x4 acc[PARTS][RF];
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+        for (int i = 0; i < RF; ++i) acc[p][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto load = [&](const uint8_t *row, int64_t k) -> i32x4 {                                 // 16 bytes from contraction index k, zeros behind the end
+        i32x4 v = {0, 0, 0, 0};
+        const int64_t left = a.K - k;
+        if (left >= 16 / EB) { __builtin_memcpy(&v, row + k * EB, 16); return v; }
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 16 / EB; ++e)
+            if (e < left) {
+                uint32_t b = 0;
+                __builtin_memcpy(&b, row + (k + e) * EB, EB);
+                w[e * EB / 4] |= b << (8 * ((e * EB) & 3));
+            }
+        __builtin_memcpy(&v, w, 16);
+        return v;
+    };
+    const int64_t steps = (a.K + KPSTEP - 1) / KPSTEP;
+    for (int64_t s0 = (int64_t)wave * STEP_RUN; s0 < steps; s0 += WAVES * STEP_RUN) {
+        i32x4 wf[PARTS][STEP_RUN], xf[RF][STEP_RUN];
+#pragma unroll
+        for (int s = 0; s < STEP_RUN; ++s) {
+            const int64_t k = (s0 + s) * KPSTEP + q * (16 / EB);                              // (steps past the end load zeros)
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) wf[p][s] = load(wr[p], k);
+#pragma unroll
+            for (int i = 0; i < RF; ++i) xf[i][s] = load(xr[i], k);
+        }
+#pragma unroll
+        for (int s = 0; s < STEP_RUN; s += 2)
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                for (int i = 0; i < RF; ++i) {
+                    const i32x4 w2[2] = {wf[p][s], wf[p][s + 1]}, x2[2] = {xf[i][s], xf[i][s + 1]};
+                    acc[p][i] = mfma_step<DT>(w2, x2, 0, acc[p][i]);
+                    acc[p][i] = mfma_step<DT>(w2, x2, 1, acc[p][i]);
+                }
+    }
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+        for (int i = 0; i < RF; ++i) sums[wave][p * RF + i][lane] = acc[p][i];
+    __syncthreads();
+    // fragment i is summed and finished by wave i: lane = row 16 i + (lane & 15), columns n0 + 4 q .. + 3
+    if (wave >= RF) return;
+    const int64_t m = 16 * wave + (lane & 15);
+    float v[4], u[4] = {};
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+        f32x4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) t += sums[w][p * RF + wave][lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) (p ? u : v)[e] = t[e];
+    }
+    if (m >= a.M) return;
+    auto out = [&](auto ot) {
+        constexpr int OT = decltype(ot)::value, OB = Elem<OT>::B;
+        const int64_t c = n0 + 4 * q;
+        with_act(a.act, [&](auto act_c) {
+            constexpr int ACT = decltype(act_c)::value;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (c + e >= a.N) break;
+                if (DT == W3D_DTYPE_FP8_E4M3) {
+                    v[e] = __builtin_ldexpf(v[e], a.xs[m] + a.ws[c + e] - 254);
+                    if (GATED) u[e] = __builtin_ldexpf(u[e], a.xs[m] + a.ws2[c + e] - 254);
+                }
+                float y = act_fwd<ACT>(v[e] + bias_at<OT>(a.bias, a.bias_f32, c + e, a.N));
+                if (GATED) y *= u[e] + bias_at<OT>(a.bias2, a.bias_f32, c + e, a.N);
+                else if (a.res) y += load1<OT>(a.res + (m * a.N + c + e) * OB);
+                store1<OT>(a.out + m * a.ld_out + (c + e) * OB, y);
+            }
+        });
+    };
+    if constexpr (DT != W3D_DTYPE_FP8_E4M3) out(std::integral_constant<int, DT>());
+    else if (a.out_dt == W3D_DTYPE_BF16) out(std::integral_constant<int, W3D_DTYPE_BF16>());
+    else out(std::integral_constant<int, W3D_DTYPE_F16>());
+}
+template <int EPI>
+int launch_skinny(const GemmArgs &a, hipStream_t st) {
+    const int64_t blocks = (a.N + 15) / 16;
+    if (blocks > 0x7fffffff) return W3D_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)blocks), block(512);
+    if (a.M <= 16) hipLaunchKernelGGL((skinny_kernel<EPI, 1>), grid, block, 0, st, a);
+    else if (a.M <= 32) hipLaunchKernelGGL((skinny_kernel<EPI, 2>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((skinny_kernel<EPI, 4>), grid, block, 0, st, a);
+    W3D_CHECK_LAUNCH();
+    return W3D_OK;
+}
+}  // namespace
+
+#if W3D_LIN_DT == 0
+#define W3D_LIN_NAME(f) f##_f32
+#elif W3D_LIN_DT == 1
+#define W3D_LIN_NAME(f) f##_bf16
+#elif W3D_LIN_DT == 2
+#define W3D_LIN_NAME(f) f##_f16
+#else
+#define W3D_LIN_NAME(f) f##_fp8
+#endif
+int W3D_LIN_NAME(w3d_lin_tiles)(const GemmArgs &a, int prod, bool aligned, int z, hipStream_t st) { return launch_prod(a, prod, aligned, z, st); }
+int W3D_LIN_NAME(w3d_lin_skinny)(const GemmArgs &a, int prod, hipStream_t st) {
+    return prod == PROD_GATED ? launch_skinny<EPI_GATED>(a, st) : launch_skinny<EPI_LINEAR>(a, st);
+}
+
+#else  // ---------------------------------------------------------------- entry points
+
+namespace {
+
+// Partial sums of a sliced product: part[slice][m][ld] -> the epilogue of the product, one lane per column, a strip of rows per block (column sums of dz per strip)
+constexpr int JOIN_ROWS = 32;
+template <int OT, int EPI>
+__global__ __launch_bounds__(256) void join_slices_kernel(GemmArgs a, int z_first) {
+    constexpr int OB = Elem<OT>::B;
+    constexpr bool GATED = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
+    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x, r0 = (int64_t)blockIdx.y * JOIN_ROWS;
+    const int64_t r1 = min(a.M, r0 + JOIN_ROWS);
+    const int64_t pad = EPI == EPI_LINEAR_BWD ? a.ld_out / OB : EPI == EPI_GATED_BWD ? a.half_out / OB : a.N;
+    if (n >= pad) return;
+    const bool in = n < a.N;
+    const float b0 = bias_at<OT>(a.bias, a.bias_f32, n, a.N), b1 = GATED ? bias_at<OT>(a.bias2, a.bias_f32, n, a.N) : 0.f;
+    const int s0 = a.ws && in ? a.ws[n] - 254 : 0, s1 = GATED && a.ws2 && in ? a.ws2[n] - 254 : 0;
+    const int64_t z = blockIdx.z + z_first;
+    with_act(a.act, [&](auto act_c) {
+        constexpr int ACT = decltype(act_c)::value;
+        float c0 = 0.f, c1 = 0.f;
+        for (int64_t m = r0; m < r1; ++m) {
+            float v = 0.f, u = 0.f;
+            if (in)
+                for (int s = 0; s < a.slices; ++s) {
+                    const float *p = a.part + ((z * a.slices + s) * a.M + m) * a.part_ld + n;
+                    v += p[0];
+                    if (GATED) u += p[a.part_ld / 2];
+                }
+            if (a.xs) { v = __builtin_ldexpf(v, a.xs[m] + s0); if (GATED) u = __builtin_ldexpf(u, a.xs[m] + s1); }
+            v += b0; u += b1;
+            uint8_t *o = (EPI == EPI_STORE && z ? a.out2 : a.out) + m * a.ld_out + n * OB;
+            if (EPI == EPI_STORE) store1<OT>(o, v);
+            else if (EPI == EPI_LINEAR) {
+                v = act_fwd<ACT>(v);
+                if (a.res) v += load1<OT>(a.res + (m * a.N + n) * OB);
+                store1<OT>(o, v);
+            } else if (EPI == EPI_GATED) store1<OT>(o, act_fwd<ACT>(v) * u);
+            else {
+                float act, der;
+                act_both<ACT>(v, act, der);
+                const float dy = in ? load1<OT>(a.dy + (m * a.N + n) * OB) : 0.f;
+                if (EPI == EPI_LINEAR_BWD) v = in ? dy * der : 0.f;
+                else { v = in ? dy * (u * der) : 0.f; u = in ? dy * act : 0.f; store1<OT>(o + a.half_out, u); c1 += u; }
+                store1<OT>(o, v);
+                c0 += v;
+            }
+        }
+        if ((EPI == EPI_LINEAR_BWD || EPI == EPI_GATED_BWD) && a.colsum && in) {
+            float *o = a.colsum + (int64_t)blockIdx.y * a.colsum_ld + n;
+            o[0] = c0;
+            if (GATED) o[a.colsum_ld / 2] = c1;
+        }
+    });
+}
+template <int OT>
+int join_as(const GemmArgs &a, int prod, int z, hipStream_t st) {
+    const int64_t cols = prod == PROD_LINEAR_BWD ? a.ld_out / Elem<OT>::B : prod == PROD_GATED_BWD ? a.half_out / Elem<OT>::B : a.N;
+    // (grid.y is limited to 65 535: longer matrices in turns of whole strips)
+    const int64_t strips = (a.M + JOIN_ROWS - 1) / JOIN_ROWS;
+    if (strips > 65535) return W3D_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)((cols + 255) / 256), (unsigned)strips, z), block(256);
+    switch (prod) {
+        case PROD_LINEAR: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_LINEAR>), grid, block, 0, st, a, 0); break;
+        case PROD_GATED: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_GATED>), grid, block, 0, st, a, 0); break;
+        case PROD_LINEAR_BWD: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_LINEAR_BWD>), grid, block, 0, st, a, 0); break;
+        case PROD_GATED_BWD: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_GATED_BWD>), grid, block, 0, st, a, 0); break;
+        default: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_STORE>), grid, block, 0, st, a, 0); break;
+    }
+    W3D_CHECK_LAUNCH();
+    return W3D_OK;
+}
+
+int eb_of(int dtype) { return dtype == W3D_DTYPE_F32 ? 4 : dtype == W3D_DTYPE_FP8_E4M3 ? 1 : 2; }
+bool float_dtype(int t) { return t == W3D_DTYPE_F32 || t == W3D_DTYPE_BF16 || t == W3D_DTYPE_F16; }
+int64_t ceil_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+bool aligned16(const void *p, int64_t ld) { return !(((uintptr_t)p) & 15) && ld % 16 == 0; }
+
+// How a product is cut.  When the tiles are fewer than the CUs, the contraction is cut until the blocks are about two per CU, each slice at least four slabs long (a slice costs a round
+// trip of its f32 tile).
+struct Cut { int slices; int64_t tiles_m, tiles_n; };
+Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool gated, int batch) {
+    const int bn = gated ? 64 : 128;
+    Cut c;
+    c.tiles_m = (M + 127) / 128; c.tiles_n = (N + bn - 1) / bn;
+    const int64_t tiles = c.tiles_m * c.tiles_n * batch, slabs = (K * eb_of(dtype) + SLAB - 1) / SLAB;
+    int64_t s = 1;
+    if (tiles < 256) s = 512 / tiles;
+    if (s > slabs / 4) s = slabs / 4;
+    if (s > 32) s = 32;
+    c.slices = (int)(s < 1 ? 1 : s);
+    return c;
+}
+size_t part_bytes(const Cut &c, int64_t M, int64_t N, bool gated, int batch) {
+    return c.slices > 1 ? (size_t)batch * c.slices * M * ceil_to(N, 16) * (gated ? 2 : 1) * 4 : 0;
+}
+
+int run_product(GemmArgs &a, int prod, int dtype, const Cut &c, bool aligned, int z, hipStream_t st) {
+    a.slices = c.slices;
+    if (c.tiles_m > 0x7fffffff || c.tiles_n > 0x7fffffff) return W3D_ERR_UNSUPPORTED;
+    a.tiles_m = (int)c.tiles_m; a.tiles_n = (int)c.tiles_n;
+    a.part_ld = ceil_to(a.N, 16) * (prod == PROD_GATED || prod == PROD_GATED_BWD ? 2 : 1);
+    int rc;
+    switch (dtype) {
+        case W3D_DTYPE_F32: rc = w3d_lin_tiles_f32(a, prod, aligned, z, st); break;
+        case W3D_DTYPE_BF16: rc = w3d_lin_tiles_bf16(a, prod, aligned, z, st); break;
+        case W3D_DTYPE_F16: rc = w3d_lin_tiles_f16(a, prod, aligned, z, st); break;
+        default: rc = w3d_lin_tiles_fp8(a, prod, aligned, z, st); break;
+    }
+    if (rc != W3D_OK || c.slices == 1) return rc;
+    switch (a.out_dt) {
+        case W3D_DTYPE_F32: return join_as<W3D_DTYPE_F32>(a, prod, z, st);
+        case W3D_DTYPE_BF16: return join_as<W3D_DTYPE_BF16>(a, prod, z, st);
+        default: return join_as<W3D_DTYPE_F16>(a, prod, z, st);
+    }
+}
+
+// 32-bit offsets inside a tile: rows of less than 8 MB
+static bool row_ok(int64_t ld) { return ld < (8 << 20); }
+
+int forward(const void *x, const int32_t *xs, const void *w, const int32_t *ws, const void *w2, const int32_t *ws2, const void *bias, const void *bias2, int bias_dtype,
+            const void *residual, int64_t R, int64_t K, int64_t N, int dtype, int out_dtype, int act, bool gated, void *y, void *workspace, size_t workspace_bytes, hipStream_t st) {
+    if (R < 0 || K < 1 || N < 1 || act < 0 || act > ACT_SIGMOID || !float_dtype(out_dtype)) return W3D_ERR_ARG;
+    if ((bias || bias2) && bias_dtype != out_dtype && bias_dtype != W3D_DTYPE_F32) return W3D_ERR_ARG;
+    if (R == 0) return W3D_OK;
+    if (!x || !w || !y || (gated && !w2)) return W3D_ERR_ARG;
+    const int64_t ld = K * eb_of(dtype);
+    if (!row_ok(ld) || !row_ok(N * eb_of(out_dtype))) return W3D_ERR_UNSUPPORTED;
+    GemmArgs a = {};
+    a.x = (const uint8_t *)x; a.w = (const uint8_t *)w; a.w2 = (const uint8_t *)w2;
+    a.ldx = a.ldw = ld; a.M = R; a.N = N; a.K = K;
+    a.bias = (const uint8_t *)bias; a.bias2 = (const uint8_t *)bias2; a.bias_f32 = bias_dtype == W3D_DTYPE_F32 && out_dtype != W3D_DTYPE_F32;
+    a.res = (const uint8_t *)residual; a.xs = xs; a.ws = ws; a.ws2 = ws2;
+    a.out = (uint8_t *)y; a.ld_out = N * eb_of(out_dtype); a.act = act; a.out_dt = out_dtype;
+    a.vec_io = aligned16(y, a.ld_out) && aligned16(residual, 0);
+    const int prod = gated ? PROD_GATED : PROD_LINEAR;
+    if (R <= SKINNY_ROWS) {
+        switch (dtype) {
+            case W3D_DTYPE_F32: return w3d_lin_skinny_f32(a, prod, st);
+            case W3D_DTYPE_BF16: return w3d_lin_skinny_bf16(a, prod, st);
+            case W3D_DTYPE_F16: return w3d_lin_skinny_f16(a, prod, st);
+            default: return w3d_lin_skinny_fp8(a, prod, st);
+        }
+    }
+    const bool aligned = aligned16(x, ld) && aligned16(w, ld) && aligned16(w2, ld);
+    const Cut c = cut_of(R, N, K, dtype, gated, 1);
+    if (c.slices > 1 && (!workspace || (((uintptr_t)workspace) & 15) || workspace_bytes < part_bytes(c, R, N, gated, 1))) return W3D_ERR_WORKSPACE;
+    a.part = (float *)workspace;
+    return run_product(a, prod, dtype, c, aligned, 1, st);
+}
+
+size_t forward_bytes(int64_t R, int64_t K, int64_t N, int dtype, bool gated) {
+    if (R <= SKINNY_ROWS || K < 1 || N < 1) return 0;
+    return part_bytes(cut_of(R, N, K, dtype, gated, 1), R, N, gated, 1);
+}
+
+// ---- backward.  Workspace: dz | column sums | partial tiles (of one product at a time)
+struct Bwd {
+    int64_t pad, ld_dz;          // columns of one half of dz, bytes of a row of dz
+    int64_t dz_bytes, strips, colsum_ld, colsum_bytes, part;
+};
+int64_t max64(int64_t a, int64_t b) { return a > b ? a : b; }
+Bwd bwd_plan(int64_t R, int64_t K, int64_t N, int dtype, bool gated, bool no_act) {
+    Bwd b;
+    const int eb = eb_of(dtype), parts = gated ? 2 : 1;
+    b.pad = ceil_to(N, gated ? 64 : 16 / eb);
+    b.ld_dz = b.pad * parts * eb;
+    b.dz_bytes = no_act ? 0 : ceil_to(R * b.ld_dz, 256);
+    b.colsum_ld = ceil_to(N, 16) * parts;
+    b.part = 0;
+    const Cut z = cut_of(R, N, K, dtype, gated, 1), dx = cut_of(R, K, gated ? 2 * b.pad : N, dtype, false, 1), dw = cut_of(N, K, R, dtype, false, parts);
+    b.strips = no_act ? w3d_column_strips(R, N) : z.slices > 1 ? (R + JOIN_ROWS - 1) / JOIN_ROWS : z.tiles_m * 2;
+    if (!no_act) b.part = (int64_t)part_bytes(z, R, N, gated, 1);
+    b.part = max64(b.part, max64((int64_t)part_bytes(dx, R, K, false, 1), (int64_t)part_bytes(dw, N, K, false, parts)));
+    b.colsum_bytes = ceil_to(b.strips * b.colsum_ld * 4, 256);
+    return b;
+}
+
+int backward(const void *x, const void *w, const void *w2, const void *bias, const void *bias2, int bias_dtype, const void *dy, int64_t R, int64_t K, int64_t N, int dtype, int act,
+             bool gated, void *dx, void *dw, void *dw2, void *db, void *db2, void *workspace, size_t workspace_bytes, hipStream_t st) {
+    if (R < 0 || K < 1 || N < 1 || act < 0 || act > ACT_SIGMOID || !float_dtype(dtype)) return W3D_ERR_ARG;
+    if ((bias || bias2 || db || db2) && bias_dtype != dtype && bias_dtype != W3D_DTYPE_F32) return W3D_ERR_ARG;
+    if (!dx && !dw && !dw2 && !db && !db2) return W3D_ERR_ARG;
+    const int eb = eb_of(dtype), parts = gated ? 2 : 1;
+    if (!row_ok(K * eb) || !row_ok((N + 64) * eb * parts)) return W3D_ERR_UNSUPPORTED;
+    if (R > 0 && (!x || !w || !dy || (gated && !w2))) return W3D_ERR_ARG;
+    const bool no_act = !gated && act == ACT_NONE;
+    const Bwd b = bwd_plan(R, K, N, dtype, gated, no_act);
+    uint8_t *ws = (uint8_t *)workspace;
+    if (R > 0) {
+        if (b.dz_bytes + b.colsum_bytes + b.part > 0 && (!ws || (((uintptr_t)ws) & 15) || workspace_bytes < (size_t)(b.dz_bytes + b.colsum_bytes + b.part))) return W3D_ERR_WORKSPACE;
+    }
+    float *colsum = (float *)(ws + b.dz_bytes), *part = (float *)(ws + b.dz_bytes + b.colsum_bytes);
+    const uint8_t *dz = (const uint8_t *)dy;
+    int64_t ld_dz = N * eb, strips = 0;
+    if (R > 0 && !no_act) {
+        GemmArgs a = {};
+        a.x = (const uint8_t *)x; a.w = (const uint8_t *)w; a.w2 = (const uint8_t *)w2;
+        a.ldx = a.ldw = K * eb; a.M = R; a.N = N; a.K = K;
+        a.bias = (const uint8_t *)bias; a.bias2 = (const uint8_t *)bias2; a.bias_f32 = bias_dtype == W3D_DTYPE_F32 && dtype != W3D_DTYPE_F32;
+        a.dy = (const uint8_t *)dy; a.out = ws; a.ld_out = b.ld_dz; a.half_out = b.pad * eb; a.act = act; a.out_dt = dtype;
+        a.vec_io = aligned16(dy, N * eb);
+        a.colsum = db || db2 ? colsum : nullptr; a.colsum_ld = b.colsum_ld; a.part = part;
+        const bool al = aligned16(x, K * eb) && aligned16(w, K * eb) && aligned16(w2, K * eb);
+        const Cut c = cut_of(R, N, K, dtype, gated, 1);
+        const int rc = run_product(a, gated ? PROD_GATED_BWD : PROD_LINEAR_BWD, dtype, c, al, 1, st);
+        if (rc != W3D_OK) return rc;
+        strips = b.strips;
+        dz = ws; ld_dz = b.ld_dz;
+    } else if (R > 0 && db) {
+        const int rc = w3d_column_sums(dy, R, N, dtype, colsum, b.colsum_ld, st);
+        if (rc != W3D_OK) return rc;
+        strips = b.strips;
+    }
+    if (db) { const int rc = w3d_fold_columns(colsum, (int)strips, b.colsum_ld, N, db, bias_dtype, st); if (rc != W3D_OK) return rc; }
+    if (db2) { const int rc = w3d_fold_columns(colsum + b.colsum_ld / 2, (int)strips, b.colsum_ld, N, db2, bias_dtype, st); if (rc != W3D_OK) return rc; }
+    if (dx && R > 0) {
+        GemmArgs a = {};
+        a.x = dz; a.ldx = ld_dz; a.w = (const uint8_t *)w; a.w2 = (const uint8_t *)w2; a.ldw = K * eb;
+        a.M = R; a.N = K; a.K = gated ? 2 * b.pad : N; a.k_split = gated ? b.pad : 0; a.w_rows = N;
+        a.out = (uint8_t *)dx; a.ld_out = K * eb; a.out_dt = dtype; a.part = part;
+        a.vec_io = aligned16(dx, K * eb);
+        const bool al = aligned16(dz, ld_dz) && aligned16(w, K * eb) && aligned16(w2, K * eb);
+        const int rc = run_product(a, PROD_DX, dtype, cut_of(R, K, a.K, dtype, false, 1), al, 1, st);
+        if (rc != W3D_OK) return rc;
+    }
+    // weight gradients: the two halves of a gated layer are one launch (blockIdx.z) when both are wanted
+    const bool both = dw && dw2;
+    for (int h = 0; h < 2; ++h) {
+        void *o = h ? dw2 : dw;
+        if (!o || (both && h)) continue;
+        if (R == 0) {
+            const int z = w3d_fold_columns(nullptr, 0, 0, N * K, o, dtype, st);
+            if (z != W3D_OK) return z;
+            if (both) { const int z2 = w3d_fold_columns(nullptr, 0, 0, N * K, dw2, dtype, st); if (z2 != W3D_OK) return z2; }
+            continue;
+        }
+        GemmArgs a = {};
+        a.x = dz + (h ? b.pad * eb : 0); a.ldx = ld_dz; a.w = (const uint8_t *)x; a.ldw = K * eb;
+        a.M = N; a.N = K; a.K = R; a.w_rows = R; a.z_x = b.pad * eb;
+        a.out = (uint8_t *)o; a.out2 = (uint8_t *)dw2; a.ld_out = K * eb; a.out_dt = dtype; a.part = part;
+        a.vec_io = aligned16(o, K * eb) && aligned16(both ? dw2 : nullptr, 0);
+        const bool al = aligned16(a.x, ld_dz) && aligned16(x, K * eb);
+        const int rc = run_product(a, PROD_DW, dtype, cut_of(N, K, R, dtype, false, parts), al, both ? 2 : 1, st);
+        if (rc != W3D_OK) return rc;
+    }
+    return W3D_OK;
+}
+}  // namespace
+
+extern "C" size_t w3d_linear_workspace_bytes(int64_t R, int64_t K, int64_t N, int dtype, int gated) { return R < 1 ? 0 : forward_bytes(R, K, N, dtype, gated != 0); }
+extern "C" size_t w3d_linear_bwd_workspace_bytes(int64_t R, int64_t K, int64_t N, int dtype, int act, int gated) {
+    if (R < 1 || K < 1 || N < 1) return 0;
+    const Bwd b = bwd_plan(R, K, N, dtype, gated != 0, !gated && act == ACT_NONE);
+    return (size_t)(b.dz_bytes + b.colsum_bytes + b.part);
+}
+extern "C" int w3d_linear_fwd(const void *x, const void *w, const void *bias, int bias_dtype, const void *residual, int64_t R, int64_t K, int64_t N, int dtype, int act, void *y,
+                              void *workspace, size_t workspace_bytes, w3d_stream_t stream) {
+    if (!float_dtype(dtype)) return W3D_ERR_ARG;
+    return forward(x, nullptr, w, nullptr, nullptr, nullptr, bias, nullptr, bias_dtype, residual, R, K, N, dtype, dtype, act, false, y, workspace, workspace_bytes, w3d_s(stream));
+}
+extern "C" int w3d_linear_fp8_fwd(const void *x, const int32_t *x_scale, const void *w, const int32_t *w_scale, const void *bias, int bias_dtype, const void *residual, int64_t R,
+                                  int64_t K, int64_t N, int out_dtype, int act, void *y, void *workspace, size_t workspace_bytes, w3d_stream_t stream) {
+    if ((out_dtype != W3D_DTYPE_BF16 && out_dtype != W3D_DTYPE_F16) || (R > 0 && (!x_scale || !w_scale))) return W3D_ERR_ARG;
+    return forward(x, x_scale, w, w_scale, nullptr, nullptr, bias, nullptr, bias_dtype, residual, R, K, N, W3D_DTYPE_FP8_E4M3, out_dtype, act, false, y, workspace, workspace_bytes,
+                   w3d_s(stream));
+}
+extern "C" int w3d_gated_linear_fwd(const void *x, const void *w_gate, const void *w_up, const void *b_gate, const void *b_up, int bias_dtype, int64_t R, int64_t K, int64_t N, int dtype,
+                                    int act, void *y, void *workspace, size_t workspace_bytes, w3d_stream_t stream) {
+    if (!float_dtype(dtype)) return W3D_ERR_ARG;
+    return forward(x, nullptr, w_gate, nullptr, w_up, nullptr, b_gate, b_up, bias_dtype, nullptr, R, K, N, dtype, dtype, act, true, y, workspace, workspace_bytes, w3d_s(stream));
+}
+extern "C" int w3d_gated_linear_fp8_fwd(const void *x, const int32_t *x_scale, const void *w_gate, const int32_t *gate_scale, const void *w_up, const int32_t *up_scale,
+                                        const void *b_gate, const void *b_up, int bias_dtype, int64_t R, int64_t K, int64_t N, int out_dtype, int act, void *y, void *workspace,
+                                        size_t workspace_bytes, w3d_stream_t stream) {
+    if ((out_dtype != W3D_DTYPE_BF16 && out_dtype != W3D_DTYPE_F16) || (R > 0 && (!x_scale || !gate_scale || !up_scale))) return W3D_ERR_ARG;
+    return forward(x, x_scale, w_gate, gate_scale, w_up, up_scale, b_gate, b_up, bias_dtype, nullptr, R, K, N, W3D_DTYPE_FP8_E4M3, out_dtype, act, true, y, workspace, workspace_bytes,
+                   w3d_s(stream));
+}
+extern "C" int w3d_linear_bwd(const void *x, const void *w, const void *bias, int bias_dtype, const void *dy, int64_t R, int64_t K, int64_t N, int dtype, int act, void *dx, void *dw,
+                              void *dbias, void *workspace, size_t workspace_bytes, w3d_stream_t stream) {
+    return backward(x, w, nullptr, bias, nullptr, bias_dtype, dy, R, K, N, dtype, act, false, dx, dw, nullptr, dbias, nullptr, workspace, workspace_bytes, w3d_s(stream));
+}
+extern "C" int w3d_gated_linear_bwd(const void *x, const void *w_gate, const void *w_up, const void *b_gate, const void *b_up, int bias_dtype, const void *dy, int64_t R, int64_t K,
+                                    int64_t N, int dtype, int act, void *dx, void *dw_gate, void *dw_up, void *db_gate, void *db_up, void *workspace, size_t workspace_bytes,
+                                    w3d_stream_t stream) {
+    return backward(x, w_gate, w_up, b_gate, b_up, bias_dtype, dy, R, K, N, dtype, act, true, dx, dw_gate, dw_up, db_gate, db_up, workspace, workspace_bytes, w3d_s(stream));
+}
+#endif

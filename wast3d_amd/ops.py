@@ -10,12 +10,13 @@ Two layers:
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import torch
 
 from . import _lib
-from ._lib import BF16, F16, F32, FP8, W3dError, check, lib, ptr, require_cuda, stream_ptr
+from ._lib import BF16, F16, F32, FP8, W3dError, check, clear_stale_hip_error, lib, ptr, require_cuda, stream_ptr
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -1392,3 +1393,333 @@ def content_loss(features_gt, features_pred):
     for gt, pred in zip(features_gt, features_pred):
         total = total + l2_loss(pred, gt.detach())
     return total
+
+
+# ------------------------------------------------------------------------------------------------
+# Layers of a feature head: rows of any width (descriptors, network taps) -> the rows the match takes.  rms_norm, linear and gated_linear are differentiable; their _fp8 forms
+# work on e4m3 rows with one E8M0 exponent each, the format of quantize_rows_fp8 / raw_knn_match_fp8.  Workspaces are torch allocations of the call's own stream (graph-capturable).
+# ------------------------------------------------------------------------------------------------
+_ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "silu": 3, "sigmoid": 4}
+
+
+def _head_act(activation) -> int:
+    try:
+        return _ACTIVATIONS[activation]
+    except (KeyError, TypeError):
+        raise W3dError(f"unknown activation {activation!r} (None, 'relu', 'gelu', 'silu' or 'sigmoid')") from None
+
+
+def _head_check(what: str, x, width: int, dtype, **others):
+    """Shapes, types and devices of one call: others = name -> (tensor or None, shape, may it be f32 next to 16-bit rows)."""
+    if x.dim() < 1 or x.shape[-1] != width or width < 1:
+        raise W3dError(f"{what}: rows of width {width} expected, got a tensor of shape {tuple(x.shape)}")
+    for name, (t, shape, wide) in others.items():
+        if t is None:
+            continue
+        if tuple(t.shape) != tuple(shape):
+            raise W3dError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+        if t.dtype != dtype and not (wide and t.dtype == torch.float32):
+            raise W3dError(f"{what}: {name} is {t.dtype}, expected {dtype}" + (" or torch.float32" if wide else ""))
+        if t.device != x.device:
+            raise W3dError(f"{what}: {name} is on {t.device}, the rows are on {x.device}")
+
+
+def _head_eps(eps) -> float:
+    eps = float(eps)
+    if not 0.0 <= eps < float("inf"):
+        raise W3dError(f"eps = {eps}: a finite value >= 0 expected")
+    return eps
+
+
+def _on_device_of(t: torch.Tensor):
+    """The launches go to the current stream of the tensors' own device."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _scratch(nbytes: int, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def raw_rms_norm(x, weight, residual, eps: float, y, s=None, rstd=None):
+    """y (and s = x + residual, and rstd f32 [R]) of contiguous rows x [R,d]."""
+    R, d = x.shape
+    check(lib().w3d_rms_norm_fwd(ptr(x), ptr(residual), ptr(weight), _dtype_code(weight) if weight is not None else 0, R, d, _dtype_code(x), eps, ptr(y), ptr(s), ptr(rstd), stream_ptr()),
+          "w3d_rms_norm_fwd")
+
+
+def raw_rms_norm_bwd(s, weight, rstd, dy, ds, dx=None, dweight=None):
+    """dx [R,d] and / or dweight [d] of contiguous rows (s: what the norm was taken of)."""
+    R, d = s.shape
+    ws = _scratch(lib().w3d_rms_norm_bwd_workspace_bytes(R, d) if dweight is not None else 0, s.device)
+    wdt = _dtype_code(weight) if weight is not None else 0
+    check(lib().w3d_rms_norm_bwd(ptr(s), ptr(weight), wdt, ptr(rstd), ptr(dy), ptr(ds), R, d, _dtype_code(s), ptr(dx), ptr(dweight), ptr(ws), ws.numel() if ws is not None else 0,
+                                 stream_ptr()), "w3d_rms_norm_bwd")
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        xc = x.contiguous()
+        wc = weight.contiguous() if weight is not None else None
+        d = xc.shape[-1]
+        rows = xc.view(-1, d)
+        y = torch.empty_like(xc)
+        s = torch.empty_like(xc) if residual is not None else None
+        rstd = torch.empty(rows.shape[0], dtype=torch.float32, device=x.device)
+        with _on_device_of(x):
+            raw_rms_norm(rows, wc, residual.contiguous().view(-1, d) if residual is not None else None, eps, y, s, rstd)
+        ctx.save_for_backward(s if s is not None else xc, wc, rstd)
+        ctx.set_materialize_grads(False)
+        return y if s is None else (y, s)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy, gs=None):
+        s, w, rstd = ctx.saved_tensors
+        want_x, want_w, want_r, _ = ctx.needs_input_grad
+        d = s.shape[-1]
+        dw = None
+        if gy is None:                                             # only s was used: its gradient passes through
+            dx = gs
+            if want_w:
+                dw = torch.zeros_like(w)
+        else:
+            dx = torch.empty_like(s) if want_x or want_r else None
+            dw = torch.empty_like(w) if want_w else None
+            if s.numel() == 0:
+                dw = dw.zero_() if dw is not None else None
+            else:
+                with _on_device_of(s):
+                    clear_stale_hip_error()
+                    raw_rms_norm_bwd(s.view(-1, d), w, rstd, gy.contiguous(), gs.contiguous() if gs is not None else None, dx, dw)
+        return dx if want_x else None, dw, dx if want_r else None, None
+
+
+def rms_norm(x, weight=None, residual=None, eps: float = 1e-6):
+    """y = s / sqrt(mean(s^2) + eps) * weight over the last dimension of s = x + residual.  x [..., d] f32 / bf16 / f16, residual like x, weight [d] of x's type or f32.
+    Returns y, or (y, s) with a residual (s rounded to x's type: what the next block adds to).  The norm is taken of the unrounded sum; sums are f32.
+    Differentiable in x, weight and residual."""
+    require_cuda(x, weight, residual)
+    d = x.shape[-1] if x.dim() else 0
+    _dtype_code(x)
+    _head_check("rms_norm", x, d, x.dtype, weight=(weight, (d,), True), residual=(residual, x.shape, False))
+    eps = _head_eps(eps)
+    if _wants_grad(x, weight, residual):
+        return _RmsNorm.apply(x, weight, residual, eps)
+    xc = x.contiguous()
+    y = torch.empty_like(xc)
+    s = torch.empty_like(xc) if residual is not None else None
+    with _on_device_of(x):
+        raw_rms_norm(xc.view(-1, d), weight.contiguous() if weight is not None else None, residual.contiguous() if residual is not None else None, eps, y, s)
+    return y if s is None else (y, s)
+
+
+def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-6):
+    """rms_norm with its rows in 8 bits: (q uint8 [R,d] = OCP e4m3 bytes, scale int32 [R] = E8M0 exponents) as of quantize_rows_fp8, and s [R,d] behind them with a residual.
+    x [R,d].  The rows are quantised from the f32 values, by quantize_rows_fp8's rule; they go straight into raw_knn_match_fp8 (d = 128, 256) or the _fp8 layers.  No gradient."""
+    require_cuda(x, weight, residual)
+    if x.dim() != 2:
+        raise W3dError(f"rms_norm_fp8: rows [R,d] expected, got a tensor of shape {tuple(x.shape)}")
+    if _wants_grad(x, weight, residual):
+        raise W3dError("rms_norm_fp8 has no gradient: call it under torch.no_grad() or on detached tensors")
+    R, d = x.shape
+    _dtype_code(x)
+    _head_check("rms_norm_fp8", x, d, x.dtype, weight=(weight, (d,), True), residual=(residual, x.shape, False))
+    eps = _head_eps(eps)
+    xc = x.contiguous()
+    q = torch.empty(R, d, dtype=torch.uint8, device=x.device)
+    scale = torch.empty(R, dtype=torch.int32, device=x.device)
+    s = torch.empty_like(xc) if residual is not None else None
+    wc = weight.contiguous() if weight is not None else None
+    rc = residual.contiguous() if residual is not None else None
+    with _on_device_of(x):
+        check(lib().w3d_rms_norm_fp8(ptr(xc), ptr(rc), ptr(wc), _dtype_code(wc) if wc is not None else 0, R, d, _dtype_code(xc), eps, ptr(q), ptr(scale), ptr(s), stream_ptr()),
+              "w3d_rms_norm_fp8")
+    return (q, scale) if s is None else (q, scale, s)
+
+
+def raw_linear(x, w, bias, residual, act: int, y):
+    """y [R,N] = act(x [R,K] w [N,K]^T + bias) + residual, contiguous."""
+    (R, K), N, dt = x.shape, w.shape[0], _dtype_code(x)
+    ws = _scratch(lib().w3d_linear_workspace_bytes(R, K, N, dt, 0), x.device)
+    check(lib().w3d_linear_fwd(ptr(x), ptr(w), ptr(bias), _dtype_code(bias) if bias is not None else 0, ptr(residual), R, K, N, dt, act, ptr(y), ptr(ws),
+                               ws.numel() if ws is not None else 0, stream_ptr()), "w3d_linear_fwd")
+
+
+def raw_gated_linear(x, wg, wu, bg, bu, act: int, y):
+    """y [R,N] = act(x wg^T + bg) * (x wu^T + bu), contiguous."""
+    (R, K), N, dt = x.shape, wg.shape[0], _dtype_code(x)
+    b = bg if bg is not None else bu
+    ws = _scratch(lib().w3d_linear_workspace_bytes(R, K, N, dt, 1), x.device)
+    check(lib().w3d_gated_linear_fwd(ptr(x), ptr(wg), ptr(wu), ptr(bg), ptr(bu), _dtype_code(b) if b is not None else 0, R, K, N, dt, act, ptr(y), ptr(ws),
+                                     ws.numel() if ws is not None else 0, stream_ptr()), "w3d_gated_linear_fwd")
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, residual, act):
+        xc, wc = x.contiguous(), w.contiguous()
+        bc = bias.contiguous() if bias is not None else None
+        y = torch.empty(*x.shape[:-1], w.shape[0], dtype=x.dtype, device=x.device)
+        with _on_device_of(x):
+            raw_linear(xc.view(-1, xc.shape[-1]), wc, bc, residual.contiguous() if residual is not None else None, act, y)
+        ctx.save_for_backward(xc, wc, bc)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x, w, bias = ctx.saved_tensors
+        want_x, want_w, want_b, want_r, _ = ctx.needs_input_grad
+        gyc = gy.contiguous()
+        K, N = x.shape[-1], w.shape[0]
+        dx = torch.empty_like(x) if want_x else None
+        dw = torch.empty_like(w) if want_w else None
+        db = torch.empty_like(bias) if want_b else None
+        R = x.numel() // K
+        if R == 0:
+            dw, db = (t.zero_() if t is not None else None for t in (dw, db))
+        elif want_x or want_w or want_b:
+            dt = _dtype_code(x)
+            with _on_device_of(x):
+                clear_stale_hip_error()
+                ws = _scratch(lib().w3d_linear_bwd_workspace_bytes(R, K, N, dt, ctx.act, 0), x.device)
+                check(lib().w3d_linear_bwd(ptr(x), ptr(w), ptr(bias), _dtype_code(bias) if bias is not None else 0, ptr(gyc), R, K, N, dt, ctx.act, ptr(dx), ptr(dw), ptr(db), ptr(ws),
+                                           ws.numel() if ws is not None else 0, stream_ptr()), "w3d_linear_bwd")
+        return dx, dw, db, gy if want_r else None, None
+
+
+def linear(x, weight, bias=None, activation=None, residual=None):
+    """y = act(x weight^T + bias) + residual in one launch.  x [..., K] f32 / bf16 / f16, weight [N,K] and residual [..., N] of x's type, bias [N] of x's type or f32;
+    activation None, 'relu', 'gelu' (z Phi(z)), 'silu' or 'sigmoid'.  Sums in f32, one rounding at the end.  Differentiable in everything; nothing but the inputs is kept for it."""
+    require_cuda(x, weight, bias, residual)
+    _dtype_code(x)
+    act = _head_act(activation)
+    if weight.dim() != 2 or weight.shape[0] < 1:
+        raise W3dError(f"linear: weight [N,K] expected, got shape {tuple(weight.shape)}")
+    N, K = weight.shape
+    _head_check("linear", x, K, x.dtype, weight=(weight, (N, K), False), bias=(bias, (N,), True), residual=(residual, (*x.shape[:-1], N), False))
+    if _wants_grad(x, weight, bias, residual):
+        return _Linear.apply(x, weight, bias, residual, act)
+    y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
+    with _on_device_of(x):
+        raw_linear(x.contiguous().view(-1, K), weight.contiguous(), bias.contiguous() if bias is not None else None, residual.contiguous() if residual is not None else None, act, y)
+    return y
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, wg, wu, bg, bu, act):
+        xc, wgc, wuc = x.contiguous(), wg.contiguous(), wu.contiguous()
+        bgc, buc = (b.contiguous() if b is not None else None for b in (bg, bu))
+        y = torch.empty(*x.shape[:-1], wg.shape[0], dtype=x.dtype, device=x.device)
+        with _on_device_of(x):
+            raw_gated_linear(xc.view(-1, xc.shape[-1]), wgc, wuc, bgc, buc, act, y)
+        ctx.save_for_backward(xc, wgc, wuc, bgc, buc)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x, wg, wu, bg, bu = ctx.saved_tensors
+        want = ctx.needs_input_grad
+        K, N = x.shape[-1], wg.shape[0]
+        grads = [torch.empty_like(t) if need else None for t, need in zip((x, wg, wu, bg, bu), want)]
+        R = x.numel() // K
+        if R == 0:
+            grads = [t.zero_() if t is not None else None for t in grads]
+        else:
+            gyc, dt, b = gy.contiguous(), _dtype_code(x), bg if bg is not None else bu
+            with _on_device_of(x):
+                clear_stale_hip_error()
+                ws = _scratch(lib().w3d_linear_bwd_workspace_bytes(R, K, N, dt, ctx.act, 1), x.device)
+                check(lib().w3d_gated_linear_bwd(ptr(x), ptr(wg), ptr(wu), ptr(bg), ptr(bu), _dtype_code(b) if b is not None else 0, ptr(gyc), R, K, N, dt, ctx.act,
+                                                 *(ptr(t) for t in grads), ptr(ws), ws.numel() if ws is not None else 0, stream_ptr()), "w3d_gated_linear_bwd")
+        return (*grads, None)
+
+
+def _gated_check(what, x, wg, wu, bg, bu, dtype, bias_dtype):
+    if wg.dim() != 2 or wg.shape[0] < 1:
+        raise W3dError(f"{what}: w_gate [N,K] expected, got shape {tuple(wg.shape)}")
+    N, K = wg.shape
+    _head_check(what, x, K, dtype, w_gate=(wg, (N, K), False), w_up=(wu, (N, K), False))
+    _head_check(what, x, K, bias_dtype, b_gate=(bg, (N,), True), b_up=(bu, (N,), True))
+    if bg is not None and bu is not None and bg.dtype != bu.dtype:
+        raise W3dError(f"{what}: b_gate is {bg.dtype}, b_up is {bu.dtype}")
+    return N, K
+
+
+def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
+    """y = act(x w_gate^T + b_gate) * (x w_up^T + b_up): both products, the activation and the product in one launch.  x [..., K] f32 / bf16 / f16, weights [N,K] of x's type, biases
+    [N] of x's type or f32 (both alike); activation as in linear.  Sums in f32, one rounding at the end.  Differentiable in everything; nothing but the inputs is kept for it."""
+    require_cuda(x, w_gate, w_up, b_gate, b_up)
+    _dtype_code(x)
+    act = _head_act(activation)
+    N, K = _gated_check("gated_linear", x, w_gate, w_up, b_gate, b_up, x.dtype, x.dtype)
+    if _wants_grad(x, w_gate, w_up, b_gate, b_up):
+        return _GatedLinear.apply(x, w_gate, w_up, b_gate, b_up, act)
+    y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
+    with _on_device_of(x):
+        raw_gated_linear(x.contiguous().view(-1, K), w_gate.contiguous(), w_up.contiguous(), *(b.contiguous() if b is not None else None for b in (b_gate, b_up)), act, y)
+    return y
+
+
+def _fp8_rows(what, name, q, scale, device):
+    if q.dtype != torch.uint8 or q.dim() != 2 or scale.dtype != torch.int32 or tuple(scale.shape) != (q.shape[0],) or q.device != device or scale.device != device:
+        raise W3dError(f"{what}: {name} expected as e4m3 bytes uint8 [rows,K] + E8M0 exponents int32 [rows] on {device}, got {q.dtype} {tuple(q.shape)} on {q.device} and "
+                       f"{scale.dtype} {tuple(scale.shape)} on {scale.device}")
+
+
+def _fp8_out(what, out_dtype, *tensors):
+    if out_dtype not in (torch.bfloat16, torch.float16):
+        raise W3dError(f"{what}: out_dtype {out_dtype} (torch.bfloat16 or torch.float16)")
+    if _wants_grad(*tensors):
+        raise W3dError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+
+
+def linear_fp8(q, scale, weight_q, weight_scale, bias=None, activation=None, residual=None, out_dtype=torch.bfloat16):
+    """linear on 8-bit rows: q [R,K], weight_q [N,K] e4m3 bytes with one E8M0 exponent a row (quantize_rows_fp8, rms_norm_fp8), products on the fp8 matrix cores, the exponents applied to
+    the f32 sums.  y [R,N] of out_dtype (bf16 / f16), residual [R,N] of out_dtype, bias [N] of out_dtype or f32.  No gradient."""
+    require_cuda(q, scale, weight_q, weight_scale, bias, residual)
+    act = _head_act(activation)
+    for name, a, b in (("q, scale", q, scale), ("weight_q, weight_scale", weight_q, weight_scale)):
+        _fp8_rows("linear_fp8", name, a, b, q.device)
+    _fp8_out("linear_fp8", out_dtype, bias, residual)
+    (R, K), N = q.shape, weight_q.shape[0]
+    if weight_q.shape[1] != K or K < 1 or N < 1:
+        raise W3dError(f"linear_fp8: rows {tuple(q.shape)} against weights {tuple(weight_q.shape)}")
+    _head_check("linear_fp8", q, K, out_dtype, bias=(bias, (N,), True), residual=(residual, (R, N), False))
+    y = torch.empty(R, N, dtype=out_dtype, device=q.device)
+    qc, sc, wc, wsc = (t.contiguous() for t in (q, scale, weight_q, weight_scale))
+    bc, rc = (t.contiguous() if t is not None else None for t in (bias, residual))
+    with _on_device_of(q):
+        ws = _scratch(lib().w3d_linear_workspace_bytes(R, K, N, FP8, 0), q.device)
+        check(lib().w3d_linear_fp8_fwd(ptr(qc), ptr(sc), ptr(wc), ptr(wsc), ptr(bc), _dtype_code(bc) if bc is not None else 0, ptr(rc), R, K, N, _dtype_code(y), act, ptr(y), ptr(ws),
+                                       ws.numel() if ws is not None else 0, stream_ptr()), "w3d_linear_fp8_fwd")
+    return y
+
+
+def gated_linear_fp8(q, scale, gate_q, gate_scale, up_q, up_scale, b_gate=None, b_up=None, activation="silu", out_dtype=torch.bfloat16):
+    """gated_linear on 8-bit rows and weights (see linear_fp8).  y [R,N] of out_dtype.  No gradient."""
+    require_cuda(q, scale, gate_q, gate_scale, up_q, up_scale, b_gate, b_up)
+    act = _head_act(activation)
+    for name, a, b in (("q, scale", q, scale), ("gate_q, gate_scale", gate_q, gate_scale), ("up_q, up_scale", up_q, up_scale)):
+        _fp8_rows("gated_linear_fp8", name, a, b, q.device)
+    _fp8_out("gated_linear_fp8", out_dtype, b_gate, b_up)
+    N, K = _gated_check("gated_linear_fp8", q, gate_q, up_q, b_gate, b_up, torch.uint8, out_dtype)
+    R = q.shape[0]
+    y = torch.empty(R, N, dtype=out_dtype, device=q.device)
+    qc, sc, gc, gsc, uc, usc = (t.contiguous() for t in (q, scale, gate_q, gate_scale, up_q, up_scale))
+    bgc, buc = (t.contiguous() if t is not None else None for t in (b_gate, b_up))
+    b = bgc if bgc is not None else buc
+    with _on_device_of(q):
+        ws = _scratch(lib().w3d_linear_workspace_bytes(R, K, N, FP8, 1), q.device)
+        check(lib().w3d_gated_linear_fp8_fwd(ptr(qc), ptr(sc), ptr(gc), ptr(gsc), ptr(uc), ptr(usc), ptr(bgc), ptr(buc), _dtype_code(b) if b is not None else 0, R, K, N,
+                                             _dtype_code(y), act, ptr(y), ptr(ws), ws.numel() if ws is not None else 0, stream_ptr()), "w3d_gated_linear_fp8_fwd")
+    return y
