@@ -631,14 +631,14 @@ int w3d_raster_preprocess_backward(const W3dRasterIn *in, const int32_t *radii, 
  * Root-mean-square norm: s = x + residual (residual NULL: s = x); rstd = 1 / sqrt(mean(s^2) + eps); y = s * rstd * weight (weight NULL: 1).
  *   w3d_rms_norm_fwd: y [R,d]; s [R,d] (optional, only with a residual; the sum, rounded); rstd f32 [R] (optional, for the backward pass).
  *   w3d_rms_norm_fp8: the same y as e4m3 bytes q [R,d] + E8M0 exponents [R] (the format and the scale rule of w3d_quantize_rows_fp8), s optional as above.
- *   w3d_rms_norm_bwd: from s (x without a residual), rstd, dy and ds (gradient that reaches s itself, optional): dx [R,d] (also the residual's gradient) and / or dweight [d]
+ *   w3d_rms_norm_bwd: from the forward's inputs, rstd, dy and ds (gradient that reaches s itself, optional): dx [R,d] (also the residual's gradient) and / or dweight [d]
  *     (of weight_dtype; needs the workspace). */
 int w3d_rms_norm_fwd(const void *x, const void *residual, const void *weight, int weight_dtype, int64_t R, int d, int dtype, float eps, void *y, void *s, float *rstd,
                      w3d_stream_t stream);
 int w3d_rms_norm_fp8(const void *x, const void *residual, const void *weight, int weight_dtype, int64_t R, int d, int dtype, float eps, void *q, int32_t *scale_e8m0, void *s,
                      w3d_stream_t stream);
 size_t w3d_rms_norm_bwd_workspace_bytes(int64_t R, int d);
-int w3d_rms_norm_bwd(const void *s, const void *weight, int weight_dtype, const float *rstd, const void *dy, const void *ds, int64_t R, int d, int dtype, void *dx, void *dweight,
+int w3d_rms_norm_bwd(const void *x, const void *residual, const void *weight, int weight_dtype, const float *rstd, const void *dy, const void *ds, int64_t R, int d, int dtype, void *dx, void *dweight,
                      void *workspace, size_t workspace_bytes, w3d_stream_t stream);
 /* Linear layer: y = act(x W^T + bias) + residual;  x [R,K], w [N,K], bias [N] or NULL, residual [R,N] or NULL, y [R,N].
  * Gated linear layer: y = act(x Wg^T + bg) * (x Wu^T + bu), one launch for both products.

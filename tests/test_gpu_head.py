@@ -73,6 +73,8 @@ def deriv_error(z, ez, name):
 # sizes: one element, odd everything, the boundaries of fragments (16), few-row form (64 / 65), tiles (128 / 256), sliced contractions, several tiles each way
 SIZES = [(1, 1, 1), (1, 4096, 17), (3, 7, 5), (16, 64, 64), (17, 130, 33), (33, 40, 256), (64, 256, 48), (65, 128, 128), (100, 1000, 3), (129, 72, 200), (257, 515, 131), (300, 2048, 96),
          (1000, 64, 1024), (700, 999, 515), (4100, 136, 264)]
+# 16-bit (and 8-bit) rows in numbers that take the 256 x 256 tile: whole tiles, odd edges everywhere, a contraction tail, sliced contractions
+LARGE = [(4096, 512, 2048), (9001, 264, 1304), (16400, 72, 1032), (1030, 2056, 1016), (5000, 1032, 520)]
 
 
 def linear_case(R, K, N, dt, act, bias, res, seed=0, bias_dt=None):
@@ -99,10 +101,36 @@ def test_linear_forward(R, K, N, dt):
         check_linear(x, w, b, r, act, ops.linear(x, w, b, activation=act, residual=r))
 
 
+@pytest.mark.parametrize("R,K,N", LARGE)
+def test_large_forward(R, K, N):
+    for i, (dt, act) in enumerate(((BF16, "gelu"), (F16, None))):
+        x, w, b, r = linear_case(R, K, N, dt, act, bias=i == 0, res=i == 1)
+        check_linear(x, w, b, r, act, ops.linear(x, w, b, activation=act, residual=r))
+        c = gated_case(R, K, N, dt, bias=i == 1)
+        check_gated(*c, "silu", ops.gated_linear(*c, activation="silu"))
+
+
+@pytest.mark.parametrize("R,K,N", LARGE)
+def test_large_gradients(R, K, N):
+    linear_gradients(R, K, N, BF16, [(2, "gelu")])
+    linear_gradients(R, K, N, F16, [(0, None), (1, "relu")])
+    gated_gradients(R, K, N, BF16, [(1, "silu")])
+    gated_gradients(R, K, N, F16, [(0, "gelu")])
+
+
+@pytest.mark.parametrize("R,K,N", LARGE)
+def test_large_fp8(R, K, N):
+    fp8_layers(R, K, N, BF16, [(0, None), (1, "gelu"), (2, "silu")])
+
+
 @pytest.mark.parametrize("dt", [BF16, F16, F32])
 @pytest.mark.parametrize("R,K,N", SIZES)
 def test_linear_gradients(R, K, N, dt):
-    for i, act in enumerate(ACTS):
+    linear_gradients(R, K, N, dt, list(enumerate(ACTS)))
+
+
+def linear_gradients(R, K, N, dt, acts):
+    for i, act in acts:
         x, w, b, r = linear_case(R, K, N, dt, act, bias=i != 1, res=i % 2 == 1, bias_dt=F32 if i == 3 else None, seed=10)
         leaves = [t.requires_grad_(True) for t in (x, w, b, r) if t is not None]
         y = ops.linear(x, w, b, activation=act, residual=r)
@@ -152,7 +180,11 @@ def test_gated_forward(R, K, N, dt):
 @pytest.mark.parametrize("dt", [BF16, F16, F32])
 @pytest.mark.parametrize("R,K,N", SIZES)
 def test_gated_gradients(R, K, N, dt):
-    for i, act in enumerate(ACTS):
+    gated_gradients(R, K, N, dt, list(enumerate(ACTS)))
+
+
+def gated_gradients(R, K, N, dt, acts):
+    for i, act in acts:
         c = gated_case(R, K, N, dt, bias=i % 2 == 1, seed=30)
         leaves = [t.requires_grad_(True) for t in c if t is not None]
         y = ops.gated_linear(*c, activation=act)
@@ -185,12 +217,16 @@ def dequant(q, e):
 @pytest.mark.parametrize("out", [BF16, F16])
 @pytest.mark.parametrize("R,K,N", SIZES)
 def test_fp8_layers(R, K, N, out):
+    fp8_layers(R, K, N, out, list(enumerate(ACTS)))
+
+
+def fp8_layers(R, K, N, out, acts):
     kp = -(-K // 4) * 4                                                                        # quantize_rows_fp8 takes multiples of 4; the layers any width
     rows = lambda n, seed, scale=1.0: (rnd(n, kp, seed=seed, scale=scale) * torch.exp2(rnd(n, 1, seed=seed + 1) * 3)).contiguous()  # noqa: E731
     q, wq, uq = (ops.quantize_rows_fp8(t) for t in (rows(R, 50), rows(N, 51, 1 / math.sqrt(K)), rows(N, 52, 1 / math.sqrt(K))))
     (q, e), (wq, we), (uq, ue) = ((a[:, :K].contiguous(), b) for a, b in (q, wq, uq))
     x, w, u = dequant(q, e), dequant(wq, we), dequant(uq, ue)
-    for i, act in enumerate(ACTS):
+    for i, act in acts:
         b = rnd(N, seed=53, dtype=F32 if i == 1 else out) if i % 2 else None
         r = rnd(R, N, seed=54, dtype=out) if i % 3 == 0 else None
         y = ops.linear_fp8(q, e, wq, we, b, activation=act, residual=r, out_dtype=out)
@@ -252,7 +288,7 @@ def test_rms_norm(R, d, dt):
         g = dy.double() * w64
         dot = (g * unit).mean(1, keepdim=True)
         dx = rs * (g - unit * dot) + (ds.double() if res else 0.0)
-        ex = u + ef                                                                            # relative error of x^ from the rounded s
+        ex = ef + 2 * W                                                                        # relative error of x^ (s is formed again, in f32)
         edot = (g * unit).abs().mean(1, keepdim=True) * (ex + (d + 8) * W)
         tol = rs * (unit.abs() * edot + ex * (unit * dot).abs() + (ef + 4 * W) * (g.abs() + (unit * dot).abs()))
         within(grads[0], dx, tol + u * (dx.abs() + tol) + tiny(dt), "dx")

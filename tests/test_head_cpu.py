@@ -32,10 +32,10 @@ def test_rms_norm_arguments(L):
     assert f(None, None, None, 0, 0, 8, 0, 1e-6, None, None, None, None) == 0                   # no rows
     assert L.w3d_rms_norm_fp8(P, None, None, 0, 4, 8, 0, 1e-6, P, None, None, None) == ARG
     b = L.w3d_rms_norm_bwd
-    assert b(P, P, 0, P, P, None, 4, 8, 0, None, None, P, 4096, None) == ARG                    # nothing wanted
-    assert b(P, P, 0, P, None, None, 4, 8, 0, P, P, P, 4096, None) == ARG
-    assert b(P, P, 0, P, P, None, 4, 8, 0, P, P, P, 16, None) == WS
-    assert b(P, P, 0, P, P, None, 4, 8, 0, P, P, None, 0, None) == WS
+    assert b(P, None, P, 0, P, P, None, 4, 8, 0, None, None, P, 4096, None) == ARG                    # nothing wanted
+    assert b(P, None, P, 0, P, None, None, 4, 8, 0, P, P, P, 4096, None) == ARG
+    assert b(P, None, P, 0, P, P, None, 4, 8, 0, P, P, P, 16, None) == WS
+    assert b(P, None, P, 0, P, P, None, 4, 8, 0, P, P, None, 0, None) == WS
     assert L.w3d_rms_norm_bwd_workspace_bytes(0, 8) == 0 and L.w3d_rms_norm_bwd_workspace_bytes(4, 8) >= 32
 
 

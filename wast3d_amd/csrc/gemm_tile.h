@@ -9,8 +9,7 @@
 // Slabs.  The contraction advances in slabs of 128 bytes of k (32 f32, 64 16-bit, 128 fp8 elements).  A K_ROWS slab is [rows][128 B], an M_ROWS slab [k of the slab][rows x element];
 // 16-byte chunks are permuted inside a row (XOR with bits of the row) so that the fragment reads of 8 (16) neighbouring lanes touch all LDS banks.
 //
-// Matrix instructions.  W is the A operand and X the B operand: a lane then holds, for ONE row m, runs of consecutive n of the output.  Which row of W sits in which row of the operand is
-// free, and is chosen so that a lane's runs join to 8 or 16 elements (K_ROWS; the M_ROWS read fixes it to 4).
+// Matrix instructions.  W is the A operand and X the B operand: a lane then holds, for ONE row m, groups of four consecutive n of the output.
 //
 // Sums are f32 in the accumulators, over the whole contraction or over one slice of it (slices > 1: partial tiles go to a workspace and are added in slice order by a second launch).
 #pragma once
@@ -50,6 +49,7 @@ enum { EPI_LINEAR = 0, EPI_GATED = 1, EPI_LINEAR_BWD = 2, EPI_GATED_BWD = 3, EPI
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -126,6 +126,18 @@ __device__ __forceinline__ void load_run(const uint8_t *p, int64_t n, bool vec, 
 #pragma unroll
     for (int i = 0; i < CNT; ++i) v[i] = i < n ? load1<DT>(p + i * EB) : 0.f;
 }
+template <int DT>
+__device__ __forceinline__ void unpack8(const i32x4 (&r)[Elem<DT>::B / 2], float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (DT == W3D_DTYPE_F32) v[i] = __int_as_float(r[i / 4 * (Elem<DT>::B / 4)][i % 4]);
+        else {
+            const uint32_t w = (uint32_t)r[0][i / 2];
+            if (DT == W3D_DTYPE_BF16) v[i] = (i & 1) ? __uint_as_float(w & 0xffff0000u) : __uint_as_float(w << 16);
+            else v[i] = f16_to_f32((uint16_t)(w >> (16 * (i & 1))));
+        }
+    }
+}
 template <int DT, int CNT>
 __device__ __forceinline__ void store_run(uint8_t *p, int64_t n, bool vec, const float (&v)[CNT]) {
     constexpr int EB = Elem<DT>::B;
@@ -157,16 +169,16 @@ __device__ __forceinline__ float bias_at(const uint8_t *b, int bias_f32, int64_t
 }
 
 // ---- one side's slabs: global -> LDS.  ROWS rows of the output tile, NT threads.
-template <int LAY, int ROWS, int EB, int NT, int HASH_BIT>
+template <int LAY, int ROWS, int EB, int NT>
 struct Stage {
     static constexpr int BYTES = ROWS * SLAB, PIECES = BYTES / 16 / NT, KPS = SLAB / EB;      // KPS: contraction elements per slab
     static constexpr int CPR = LAY == K_ROWS ? SLAB / 16 : ROWS * EB / 16;                     // chunks per LDS row
     static_assert(BYTES % (16 * NT) == 0, "whole pieces");
 
-    // permutation of the 16-byte chunks of an LDS row.  K_ROWS: neighbouring operand rows r = 0..7 sit in tile rows (r & 3) + (4 * group stride) * (r >> 2): HASH_BIT is log2 of
-    // that stride (2 where operand rows are tile rows).  M_ROWS, 16 bits: four consecutive k share a transposing read of 16 lanes; f32: k and k + 4 share the 64-lane read's halves.
+    // permutation of the 16-byte chunks of an LDS row.  K_ROWS: 8 lanes read the same chunk of 8 neighbouring rows.  M_ROWS, 16 bits: four consecutive k share a transposing read of 16
+    // lanes; f32: k and k + 4 share a read's halves.
     static __device__ __forceinline__ int swizzle(int row) {
-        if (LAY == K_ROWS) return (row & 3) | (((row >> HASH_BIT) & 1) << 2);
+        if (LAY == K_ROWS) return row & 7;
         return EB == 4 ? ((row >> 2) & 1) << 2 : (row & 3) << 1;
     }
     static __device__ __forceinline__ void place(int tid, int i, int &row, int &chunk) {      // storage row inside the slab and source chunk of piece i
@@ -195,27 +207,226 @@ __device__ __forceinline__ f32x4 mfma_step(const i32x4 (&w)[2], const i32x4 (&x)
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 127, 0, 127);
 }
 
+// ---- what becomes of a wave's accumulators.  MS: rows of the matrix instruction (16 or 32): a lane holds groups of four consecutive n of one row m.  They go through a patch of LDS that the
+// wave has to itself, 64 rows at a time and in f32, and come back as runs of 8 n: 8 (gated: 4) lanes hold a row's 64 (32) columns, so that every load and store of the epilogue is whole
+// 128-byte (64-byte) pieces of a row.  (Straight from the accumulators a store writes 16-byte pieces of 16 rows: 14 us per 256 x 256 tile instead of 8.)
+// What the epilogue reads (residual, dy) is loaded AHEAD passes early: a pass is a fraction of the memory's latency.
+template <int DT, int EPI, int BM, int BN, int WM, int WN, int MS>
+struct Out {
+    static constexpr int EB = Elem<DT>::B;
+    static constexpr bool GATED = EPI == EPI_GATED || EPI == EPI_GATED_BWD, BWD = EPI == EPI_LINEAR_BWD || EPI == EPI_GATED_BWD;
+    static constexpr int PARTS = GATED ? 2 : 1, BNP = BN / PARTS;                              // a gated tile is BN / 2 columns of each half: rows [0, BN/2) of the W slab gate, the rest up
+    static constexpr int FM = BM / WM / MS, FN = BN / WN / MS, FP = FN / PARTS;
+    static constexpr int COLS = BN / WN, PCOLS = COLS / PARTS, LPR = PCOLS / 8, RPP = 64 / LPR;      // lanes per row, rows per pass
+    static constexpr int ROWS = 64, CHUNKS = BM / WM / ROWS, PASSES = ROWS / RPP, AHEAD = 4;
+    static constexpr int PATCH = ROWS * COLS * 4;
+    static_assert(COLS == 64 && BM / WM % ROWS == 0 && AHEAD <= PASSES, "a patch row is 16 chunks; whole chunks of rows");
+    typedef typename std::conditional<MS == 32, f32x16, f32x4>::type acc_t;
+    typedef acc_t Acc[FM][FN];
+
+    static __device__ __forceinline__ int w_row(int wn, int f, int lane) { return (f / FP) * BNP + wn * PCOLS + MS * (f % FP) + (lane & (MS - 1)); }     // tile row of the lane's operand row
+    static __device__ __forceinline__ int x_row(int wm, int f, int lane) { return wm * (BM / WM) + MS * f + (lane & (MS - 1)); }
+
+    // chunks of 16 bytes are permuted by XOR with the row: lanes that write (read) neighbouring rows touch different banks
+    static __device__ __forceinline__ void put(const Acc &acc, int i, int lane, uint8_t *patch) {
+        const int row = MS * (i % (ROWS / MS)) + (lane & (MS - 1));
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int b = 0; b < MS * MS / 256; ++b) {
+                const int chunk = MS == 32 ? 8 * j + 2 * b + (lane >> 5) : 4 * j + (lane >> 4);
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * b + e];
+                *reinterpret_cast<f32x4 *>(patch + row * (COLS * 4) + ((chunk ^ (row & 15)) << 4)) = v;
+            }
+    }
+    static __device__ __forceinline__ void get(const uint8_t *patch, int row, int part, int lane, float (&v)[8]) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int chunk = part * (PCOLS / 4) + 2 * (lane % LPR) + c;
+            const f32x4 t = *reinterpret_cast<const f32x4 *>(patch + row * (COLS * 4) + ((chunk ^ (row & 15)) << 4));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * c + e] = t[e];
+        }
+    }
+    // f(row m, row in the patch, 8 elements of src) for every row this lane finishes.  src: [M][N] of type OT or NULL; n: the lane's first column
+    template <int OT, typename F>
+    static __device__ __forceinline__ void each_row(const GemmArgs &a, const Acc &acc, const uint8_t *src, int64_t m0, int64_t n, int wm, int lane, uint8_t *patch, F f) {
+        constexpr int OB = Elem<OT>::B, RAW = OB * 8 / 16;
+        const int64_t mw = m0 + wm * (BM / WM) + lane / LPR;
+        const bool fast = src && a.vec_io && n + 8 <= a.N;
+        i32x4 ring[AHEAD][RAW];
+        const uint8_t *at = src + (mw * a.N + n) * OB;
+        const int64_t step = RPP * a.N * OB;
+        int64_t next = mw;
+        auto fetch = [&](i32x4 (&r)[RAW]) {
+            if (fast && next < a.M)
+#pragma unroll
+                for (int k = 0; k < RAW; ++k) r[k] = reinterpret_cast<const i32x4 *>(at)[k];
+            at += step;
+            next += RPP;
+        };
+        if (src)
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) fetch(ring[k]);
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+#pragma unroll
+            for (int i = 0; i < ROWS / MS; ++i) put(acc, c * (ROWS / MS) + i, lane, patch);
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+            for (int p = 0; p < PASSES; ++p) {
+                const int64_t m = mw + c * ROWS + p * RPP;
+                float t[8] = {};
+                if (src) {
+                    if (fast) unpack8<OT>(ring[0], t);
+                    else if (m < a.M) load_run<OT, 8>(src + (m * a.N + n) * OB, a.N - n, false, t);
+#pragma unroll
+                    for (int k = 0; k + 1 < AHEAD; ++k)
+#pragma unroll
+                        for (int q = 0; q < RAW; ++q) ring[k][q] = ring[k + 1][q];
+                    fetch(ring[AHEAD - 1]);
+                }
+                f(m, p * RPP + lane / LPR, t);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+
+    static __device__ __forceinline__ void epilogue(const GemmArgs &a, const Acc &acc, int64_t m0, int64_t n0, int slice, int tm, int wm, int wn, int lane, bool z1, uint8_t *patch) {
+        const int64_t n = n0 + wn * PCOLS + 8 * (lane % LPR);
+        if (a.slices > 1) {
+            const int64_t z = (int64_t)(z1 ? a.slices : 0) + slice;
+            each_row<W3D_DTYPE_F32>(a, acc, nullptr, m0, n, wm, lane, patch, [&](int64_t m, int row, float (&)[8]) {
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    float v[8];
+                    get(patch, row, p, lane, v);
+                    if (m < a.M) store_run<W3D_DTYPE_F32, 8>((uint8_t *)(a.part + (z * a.M + m) * a.part_ld + p * (a.part_ld / 2) + n), a.N - n, true, v);
+                }
+            });
+            return;
+        }
+        // (fp8 rows: the output is bf16 or f16)
+        if constexpr (DT == W3D_DTYPE_FP8_E4M3) {
+            if (a.out_dt == W3D_DTYPE_BF16) finish<W3D_DTYPE_BF16>(a, acc, m0, n, tm, wm, lane, z1, patch);
+            else finish<W3D_DTYPE_F16>(a, acc, m0, n, tm, wm, lane, z1, patch);
+        } else finish<DT>(a, acc, m0, n, tm, wm, lane, z1, patch);
+    }
+
+    template <int OT>
+    static __device__ __forceinline__ void finish(const GemmArgs &a, const Acc &acc, int64_t m0, int64_t n, int tm, int wm, int lane, bool z1, uint8_t *patch) {
+        constexpr int OB = Elem<OT>::B;
+        const bool vec = a.vec_io != 0;
+        if constexpr (EPI == EPI_STORE) {
+            uint8_t *out = z1 ? a.out2 : a.out;
+            each_row<OT>(a, acc, nullptr, m0, n, wm, lane, patch, [&](int64_t m, int row, float (&)[8]) {
+                float v[8];
+                get(patch, row, 0, lane, v);
+                if (m < a.M) store_run<OT, 8>(out + m * a.ld_out + n * OB, a.N - n, vec, v);
+            });
+            return;
+        }
+        float b0[8], b1[8], c0[8], c1[8];
+        int s0[8], s1[8];                                // fp8: the sums are scaled by 2^(row exponent of x + row exponent of w), exactly
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            b0[e] = bias_at<OT>(a.bias, a.bias_f32, n + e, a.N);
+            b1[e] = GATED ? bias_at<OT>(a.bias2, a.bias_f32, n + e, a.N) : 0.f;
+            c0[e] = c1[e] = 0.f;
+            s0[e] = s1[e] = 0;
+            if (DT == W3D_DTYPE_FP8_E4M3 && n + e < a.N) { s0[e] = a.ws[n + e] - 254; if (GATED) s1[e] = a.ws2[n + e] - 254; }
+        }
+        each_row<OT>(a, acc, BWD ? a.dy : a.res, m0, n, wm, lane, patch, [&](int64_t m, int row, float (&t)[8]) {
+            const bool live = m < a.M;
+            float v[8], u[8];
+            get(patch, row, 0, lane, v);
+            if (GATED) get(patch, row, 1, lane, u);
+            if (DT == W3D_DTYPE_FP8_E4M3) {
+                const int xs = live ? a.xs[m] : 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { v[e] = __builtin_ldexpf(v[e], xs + s0[e]); if (GATED) u[e] = __builtin_ldexpf(u[e], xs + s1[e]); }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { v[e] += b0[e]; if (GATED) u[e] += b1[e]; }
+            with_act(a.act, [&](auto act_c) {
+                constexpr int ACT = decltype(act_c)::value;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (!BWD) {
+                        v[e] = act_fwd<ACT>(v[e]);
+                        if (EPI == EPI_GATED) v[e] *= u[e];
+                    } else {
+                        float act, der;
+                        act_both<ACT>(v[e], act, der);
+                        if (EPI == EPI_LINEAR_BWD) v[e] = t[e] * der;
+                        else { v[e] = t[e] * (u[e] * der); u[e] = t[e] * act; }
+                    }
+                }
+            });
+            if (!BWD) {
+                if (EPI == EPI_LINEAR && a.res)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] += t[e];
+                if (live) store_run<OT, 8>(a.out + m * a.ld_out + n * OB, a.N - n, vec, v);
+            } else {
+                // dz; zeros in the padding columns (dy is read as zero there and z is finite: W has no such rows, the bias no such elements), which are part of the contraction of dx.
+                // Column sums in f32 before the rounding.
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { c0[e] += live ? v[e] : 0.f; if (GATED) c1[e] += live ? u[e] : 0.f; }
+                const int64_t pad = (EPI == EPI_GATED_BWD ? a.half_out : a.ld_out) / OB - n;      // columns of the padded row from here: a multiple of 8 (16 bits) or 4
+                uint8_t *o = a.out + m * a.ld_out + n * OB;
+                if (live && pad > 0) {
+                    store_run<OT, 8>(o, pad, true, v);
+                    if (EPI == EPI_GATED_BWD) store_run<OT, 8>(o + a.half_out, pad, true, u);
+                }
+            }
+        });
+        if (BWD && a.colsum) {
+            // lanes l, l + LPR, ... hold the same columns
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int o = LPR; o < 64; o *= 2) {
+                    c0[e] += __shfl_xor(c0[e], o, 64);
+                    if (GATED) c1[e] += __shfl_xor(c1[e], o, 64);
+                }
+            if (lane < LPR) {
+                float *o = a.colsum + ((int64_t)tm * WM + wm) * a.colsum_ld + n;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (n + e < a.N) { o[e] = c0[e]; if (GATED) o[a.colsum_ld / 2 + e] = c1[e]; }
+            }
+        }
+    }
+};
+
+// tile of a block: consecutive blocks go round the 8 XCDs, so block b works on place (b % 8) * (tiles / 8) + b / 8 of an order in which neighbours share operand rows (each XCD's L2 then
+// serves a compact patch of C); the order runs down groups of 8 tile rows
+__device__ __forceinline__ void tile_of_block(const GemmArgs &a, int &slice, int &tm, int &tn) {
+    const int tiles = a.tiles_m * a.tiles_n, total = tiles * a.slices;
+    const int q = total / 8, r = total % 8, xcd = blockIdx.x % 8, at = blockIdx.x / 8;
+    int id = xcd * q + min(xcd, r) + at;
+    slice = id / tiles;
+    id -= slice * tiles;
+    const int span = 8 * a.tiles_n, g = id / span, first = g * 8, rows = min(8, a.tiles_m - first), in = id - g * span;
+    tm = first + in % rows;
+    tn = in / rows;
+}
+
 template <int DT, int LX, int LW, int EPI, int BM, int BN, int WM, int WN, bool ALIGNED>
 struct Gemm {
     static constexpr int NT = WM * WN * 64, EB = Elem<DT>::B, KPS = SLAB / EB;
-    static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-    static constexpr bool GATED = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
-    static constexpr int PARTS = GATED ? 2 : 1, FP = FN / PARTS, BNP = BN / PARTS;             // a gated tile is BN / 2 columns of each half: rows [0, BN/2) of the W slab gate, the rest up
-    static constexpr int CG = LW == M_ROWS ? 1 : (FP < 4 ? FP : 4);                           // fragments whose runs of 4 join in one lane
-    static constexpr int RUN = 4 * CG, GROUPS = FP / CG;
-    static constexpr int HASH_W = CG == 4 ? 4 : CG == 2 ? 3 : 2;
-    typedef Stage<LX, BM, EB, NT, 2> SX;
-    typedef Stage<LW, BN, EB, NT, HASH_W> SW;
+    typedef Out<DT, EPI, BM, BN, WM, WN, 16> O;
+    static constexpr int FM = O::FM, FN = O::FN, BNP = O::BNP;
+    static constexpr bool GATED = O::GATED;
+    typedef Stage<LX, BM, EB, NT> SX;
+    typedef Stage<LW, BN, EB, NT> SW;
     static constexpr int BUF = SX::BYTES + SW::BYTES, LDS_BYTES = 2 * BUF;
     static_assert(!GATED || LW == K_ROWS, "gated products read the weights by rows");
     static_assert(!GATED || SW::PIECES % 2 == 0, "a piece of the W slab belongs to one half");
 
-    // byte address (inside the slab) of a lane's first K_ROWS chunk: step s adds XOR 64
-    static __device__ __forceinline__ int x_row(int wm, int f, int lane) { return wm * (BM / WM) + 16 * f + (lane & 15); }
-    static __device__ __forceinline__ int w_row(int wn, int f, int lane) {                     // tile row of operand row r = lane & 15 of fragment f
-        const int r = lane & 15, part = f / FP, fp = f % FP;
-        return part * BNP + wn * (BNP / WN) + 16 * CG * (fp / CG) + 4 * CG * (r >> 2) + 4 * (fp % CG) + (r & 3);
-    }
     template <typename S, int LAY>
     static __device__ __forceinline__ void frag(const uint8_t *slab, int row_of_lane, int base16, int lane, i32x4 (&v)[2]) {
         const int q = lane >> 4;
@@ -299,22 +510,8 @@ struct Gemm {
     static __device__ __forceinline__ void run(const GemmArgs &a, uint8_t *smem) {
         const int tid = threadIdx.x, lane = tid & 63;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
-        // tile of this block: consecutive blocks go round the 8 XCDs, so block b works on place (b % 8) * (tiles / 8) + b / 8 of an order in which neighbours share operand rows (each
-        // XCD's L2 then serves a compact patch of C); the order runs down groups of 8 tile rows
-        const int tiles = a.tiles_m * a.tiles_n, total = tiles * a.slices;
-        int id = blockIdx.x;
-        {
-            const int q = total / 8, r = total % 8, xcd = id % 8, at = id / 8;
-            id = xcd * q + min(xcd, r) + at;
-        }
-        const int slice = id / tiles;
-        id -= slice * tiles;
-        int tm, tn;
-        {
-            const int span = 8 * a.tiles_n, g = id / span, first = g * 8, rows = min(8, a.tiles_m - first), in = id - g * span;
-            tm = first + in % rows;
-            tn = in / rows;
-        }
+        int slice, tm, tn;
+        tile_of_block(a, slice, tm, tn);
         const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BNP;
         const int64_t slabs = (a.K + KPS - 1) / KPS;
         const int64_t s_begin = slabs * slice / a.slices, s_end = slabs * (slice + 1) / a.slices;
@@ -329,7 +526,7 @@ struct Gemm {
         if (GATED) sw2.base = a.w2 + w_at;
         else if (a.k_split > 0) { sw2.base = a.w2 + w_at - a.k_split * a.ldw; sw2.k = a.k_split + a.w_rows; }
 
-        f32x4 acc[FM][FN];
+        typename O::Acc acc;
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -374,9 +571,9 @@ struct Gemm {
             const uint8_t *bx = smem + cur * BUF, *bw = bx + SX::BYTES;
             i32x4 xf[FM][2], wf[FN][2];
 #pragma unroll
-            for (int j = 0; j < FN; ++j) frag<SW, LW>(bw, w_row(wn, j, lane), wn * FN + j, lane, wf[j]);
+            for (int j = 0; j < FN; ++j) frag<SW, LW>(bw, O::w_row(wn, j, lane), wn * FN + j, lane, wf[j]);
 #pragma unroll
-            for (int i = 0; i < FM; ++i) frag<SX, LX>(bx, x_row(wm, i, lane), wm * FM + i, lane, xf[i]);
+            for (int i = 0; i < FM; ++i) frag<SX, LX>(bx, O::x_row(wm, i, lane), wm * FM + i, lane, xf[i]);
             const bool more = t + 1 < s_end;
             if (more) {
                 if (ALIGNED) dma(t + 1, smem + (cur ^ 1) * BUF);
@@ -390,163 +587,8 @@ struct Gemm {
                     for (int j = 0; j < FN; ++j) acc[i][j] = mfma_step<DT>(wf[j], xf[i], s, acc[i][j]);
             if (!ALIGNED && more) put(smem + (cur ^ 1) * BUF);
         }
-        epilogue(a, acc, m0, n0, slice, tm, wm, wn, lane, z1);
-    }
-
-    // first column (inside the output) of group g of a lane
-    static __device__ __forceinline__ int64_t col_of(int64_t n0, int wn, int g, int lane) { return n0 + wn * (BNP / WN) + 16 * CG * g + RUN * (lane >> 4); }
-    static __device__ __forceinline__ void gather(const f32x4 (&acc)[FM][FN], int i, int part, int g, float (&v)[RUN]) {
-#pragma unroll
-        for (int c = 0; c < CG; ++c)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[4 * c + e] = acc[i][part * FP + g * CG + c][e];
-    }
-
-    static __device__ __forceinline__ void epilogue(const GemmArgs &a, f32x4 (&acc)[FM][FN], int64_t m0, int64_t n0, int slice, int tm, int wm, int wn, int lane, bool z1) {
-        const int64_t mr = m0 + wm * (BM / WM) + (lane & 15);
-        if (a.slices > 1) {
-#pragma unroll
-            for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
-                    const int64_t n = col_of(n0, wn, g, lane);
-#pragma unroll
-                    for (int i = 0; i < FM; ++i) {
-                        const int64_t m = mr + 16 * i;
-                        if (m >= a.M) continue;
-                        float v[RUN];
-                        gather(acc, i, p, g, v);
-                        const int64_t z = (int64_t)(z1 ? a.slices : 0) + slice;
-                        store_run<W3D_DTYPE_F32, RUN>((uint8_t *)(a.part + (z * a.M + m) * a.part_ld + p * (a.part_ld / 2) + n), a.N - n, true, v);
-                    }
-                }
-            return;
-        }
-        // (fp8 rows: the output is bf16 or f16)
-        if (DT == W3D_DTYPE_FP8_E4M3) {
-            if (a.out_dt == W3D_DTYPE_BF16) finish<W3D_DTYPE_BF16>(a, acc, mr, n0, tm, wm, wn, lane, z1);
-            else finish<W3D_DTYPE_F16>(a, acc, mr, n0, tm, wm, wn, lane, z1);
-        } else finish<DT == W3D_DTYPE_FP8_E4M3 ? W3D_DTYPE_BF16 : DT>(a, acc, mr, n0, tm, wm, wn, lane, z1);
-    }
-
-    template <int OT>
-    static __device__ __forceinline__ void finish(const GemmArgs &a, f32x4 (&acc)[FM][FN], int64_t mr, int64_t n0, int tm, int wm, int wn, int lane, bool z1) {
-        constexpr int OB = Elem<OT>::B;
-        const bool vec = a.vec_io != 0;
-        if (EPI == EPI_STORE) {
-            uint8_t *out = z1 ? a.out2 : a.out;
-#pragma unroll
-            for (int g = 0; g < GROUPS; ++g) {
-                const int64_t n = col_of(n0, wn, g, lane);
-#pragma unroll
-                for (int i = 0; i < FM; ++i) {
-                    const int64_t m = mr + 16 * i;
-                    if (m >= a.M) continue;
-                    float v[RUN];
-                    gather(acc, i, 0, g, v);
-                    store_run<OT, RUN>(out + m * a.ld_out + n * OB, a.N - n, vec, v);
-                }
-            }
-            return;
-        }
-        with_act(a.act, [&](auto act_c) {
-            constexpr int ACT = decltype(act_c)::value;
-#pragma unroll
-            for (int g = 0; g < GROUPS; ++g) {
-                const int64_t n = col_of(n0, wn, g, lane);
-                float b0[RUN], b1[RUN], c0[RUN], c1[RUN];
-#pragma unroll
-                for (int e = 0; e < RUN; ++e) {
-                    b0[e] = bias_at<OT>(a.bias, a.bias_f32, n + e, a.N);
-                    if (GATED) b1[e] = bias_at<OT>(a.bias2, a.bias_f32, n + e, a.N);
-                    c0[e] = c1[e] = 0.f;
-                }
-                int s0[RUN], s1[RUN];                    // fp8: the sums are scaled by 2^(row exponent of x + row exponent of w), exactly
-                if (DT == W3D_DTYPE_FP8_E4M3) {
-#pragma unroll
-                    for (int e = 0; e < RUN; ++e) {
-                        s0[e] = n + e < a.N ? a.ws[n + e] - 254 : 0;
-                        if (GATED) s1[e] = n + e < a.N ? a.ws2[n + e] - 254 : 0;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < FM; ++i) {
-                    const int64_t m = mr + 16 * i;
-                    const bool live = m < a.M;
-                    float v[RUN], u[RUN], t[RUN];
-                    gather(acc, i, 0, g, v);
-                    if (GATED) gather(acc, i, 1, g, u);
-                    if (DT == W3D_DTYPE_FP8_E4M3) {
-                        const int xs = live ? a.xs[m] : 0;
-#pragma unroll
-                        for (int e = 0; e < RUN; ++e) { v[e] = __builtin_ldexpf(v[e], xs + s0[e]); if (GATED) u[e] = __builtin_ldexpf(u[e], xs + s1[e]); }
-                    }
-#pragma unroll
-                    for (int e = 0; e < RUN; ++e) { v[e] += b0[e]; if (GATED) u[e] += b1[e]; }
-                    if (EPI == EPI_LINEAR || EPI == EPI_GATED) {
-                        if (!live) continue;
-                        if (EPI == EPI_LINEAR && a.res) load_run<OT, RUN>(a.res + (m * a.N + n) * OB, a.N - n, vec, t);
-#pragma unroll
-                        for (int e = 0; e < RUN; ++e) {
-                            v[e] = act_fwd<ACT>(v[e]);
-                            if (EPI == EPI_GATED) v[e] *= u[e];
-                            else if (a.res) v[e] += t[e];
-                        }
-                        store_run<OT, RUN>(a.out + m * a.ld_out + n * OB, a.N - n, vec, v);
-                    } else {
-                        // dz of the rows and columns that exist, zeros in the padding columns (they are part of the contraction of dx); column sums in f32 before the rounding
-                        if (live) load_run<OT, RUN>(a.dy + (m * a.N + n) * OB, a.N - n, vec, t);
-#pragma unroll
-                        for (int e = 0; e < RUN; ++e) {
-                            float act, der;
-                            act_both<ACT>(v[e], act, der);
-                            const bool in = live && n + e < a.N;
-                            if (EPI == EPI_LINEAR_BWD) v[e] = in ? t[e] * der : 0.f;
-                            else { v[e] = in ? t[e] * (u[e] * der) : 0.f; u[e] = in ? t[e] * act : 0.f; c1[e] += u[e]; }
-                            c0[e] += v[e];
-                        }
-                        if (!live) continue;
-                        const int64_t pad = (EPI == EPI_GATED_BWD ? a.half_out : a.ld_out) / OB - n;      // columns of the padded row from here: a multiple of 8 (16 bits) or 4
-                        uint8_t *o = a.out + m * a.ld_out + n * OB;
-                        constexpr int CH = 16 / OB;
-#pragma unroll
-                        for (int c = 0; c < RUN / CH; ++c) {
-                            float h[CH];
-                            if (c * CH < pad) {
-#pragma unroll
-                                for (int e = 0; e < CH; ++e) h[e] = v[c * CH + e];
-                                store_run<OT, CH>(o + c * 16, CH, true, h);
-                                if (EPI == EPI_GATED_BWD) {
-#pragma unroll
-                                    for (int e = 0; e < CH; ++e) h[e] = u[c * CH + e];
-                                    store_run<OT, CH>(o + a.half_out + c * 16, CH, true, h);
-                                }
-                            }
-                        }
-                    }
-                }
-                if ((EPI == EPI_LINEAR_BWD || EPI == EPI_GATED_BWD) && a.colsum) {
-                    // the 16 lanes of a DPP row hold 16 rows of the same columns: their sum ends in the row's last lane
-#pragma unroll
-                    for (int e = 0; e < RUN; ++e) {
-                        c0[e] = row_sum(c0[e]);
-                        if (GATED) c1[e] = row_sum(c1[e]);
-                    }
-                    if ((lane & 15) == 15) {
-                        float *o = a.colsum + ((int64_t)tm * WM + wm) * a.colsum_ld + n;
-#pragma unroll
-                        for (int e = 0; e < RUN; ++e)
-                            if (n + e < a.N) { o[e] = c0[e]; if (GATED) o[a.colsum_ld / 2 + e] = c1[e]; }
-                    }
-                }
-            }
-        });
-    }
-    static __device__ __forceinline__ float row_sum(float v) {
-        v = dpp_add_step<0x111, 0xf>(v);
-        v = dpp_add_step<0x112, 0xf>(v);
-        v = dpp_add_step<0x114, 0xf>(v);
-        return dpp_add_step<0x118, 0xf>(v);
+        __syncthreads();                                 // the slabs' LDS becomes the waves' patches
+        O::epilogue(a, acc, m0, n0, slice, tm, wm, wn, lane, z1, smem + wave * O::PATCH);
     }
 };
 

@@ -2,7 +2,7 @@
 //
 // Three kernels do the products (gemm_tile.h has the tile):
 //   * few rows (<= SKINNY_ROWS): the weights are read once, straight into MFMA fragments, by as many waves as there are; the rows are the other operand
-//   * tiles of 128 x 128 through LDS
+//   * tiles of 256 x 256 (gemm_pipe.h) or 128 x 128 (gemm_tile.h) through LDS
 //   * when the tiles are few for 256 CUs the contraction is cut into slices; partial tiles are added in slice order, and the epilogue applied, by a second launch
 //
 // Backward keeps nothing of the forward pass but its inputs: z is formed again and turned into dz in the epilogue, where the column sums for the bias
@@ -10,7 +10,7 @@
 // (R x N x 12 bytes written and read, against 2 R N K operations).  dz is rounded once to the operands' type (it is an operand of two products); sums are f32.
 //
 // One translation unit per operand type (W3D_LIN_DT: the tiles), one for the entry points.
-#include "gemm_tile.h"
+#include "gemm_pipe.h"
 
 int w3d_fold_columns(const float *part, int parts, int64_t ld, int64_t n, void *out, int out_dtype, hipStream_t st);      // columns.hip
 int w3d_column_strips(int64_t R, int64_t n);
@@ -22,10 +22,10 @@ constexpr int SKINNY_ROWS = 64;
 }  // namespace
 
 // launches of one operand type's kernels
-int w3d_lin_tiles_f32(const GemmArgs &a, int prod, bool aligned, int z, hipStream_t st);
-int w3d_lin_tiles_bf16(const GemmArgs &a, int prod, bool aligned, int z, hipStream_t st);
-int w3d_lin_tiles_f16(const GemmArgs &a, int prod, bool aligned, int z, hipStream_t st);
-int w3d_lin_tiles_fp8(const GemmArgs &a, int prod, bool aligned, int z, hipStream_t st);
+int w3d_lin_tiles_f32(const GemmArgs &a, int prod, bool big, bool aligned, int z, hipStream_t st);
+int w3d_lin_tiles_bf16(const GemmArgs &a, int prod, bool big, bool aligned, int z, hipStream_t st);
+int w3d_lin_tiles_f16(const GemmArgs &a, int prod, bool big, bool aligned, int z, hipStream_t st);
+int w3d_lin_tiles_fp8(const GemmArgs &a, int prod, bool big, bool aligned, int z, hipStream_t st);
 int w3d_lin_skinny_f32(const GemmArgs &a, int prod, hipStream_t st);
 int w3d_lin_skinny_bf16(const GemmArgs &a, int prod, hipStream_t st);
 int w3d_lin_skinny_f16(const GemmArgs &a, int prod, hipStream_t st);
@@ -34,34 +34,35 @@ int w3d_lin_skinny_fp8(const GemmArgs &a, int prod, hipStream_t st);
 #ifdef W3D_LIN_DT
 namespace {
 
-template <int LX, int LW, int EPI, int BM, int BN, int WM, int WN, bool ALIGNED>
-int launch_tiles(const GemmArgs &a, int z, hipStream_t st) {
-    typedef Gemm<W3D_LIN_DT, LX, LW, EPI, BM, BN, WM, WN, ALIGNED> G;
-    auto kernel = gemm_kernel<W3D_LIN_DT, LX, LW, EPI, BM, BN, WM, WN, ALIGNED>;
-    if (G::LDS_BYTES > 65536) W3D_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS_BYTES));
+int launch_kernel(void (*kernel)(GemmArgs), int threads, int lds, const GemmArgs &a, int z, hipStream_t st) {
+    if (lds > 65536) W3D_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     const int64_t blocks = (int64_t)a.tiles_m * a.tiles_n * a.slices;
     if (blocks < 1 || blocks > 0x7fffffff) return W3D_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, 1, z), dim3(G::NT), G::LDS_BYTES, st, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, 1, z), dim3(threads), lds, st, a);
     W3D_CHECK_LAUNCH();
     return W3D_OK;
 }
 template <int LX, int LW, int EPI>
-int launch_shape(const GemmArgs &a, bool aligned, int z, hipStream_t st) {
-    if (!aligned) return launch_tiles<LX, LW, EPI, 128, 128, 2, 2, false>(a, z, st);
-    return launch_tiles<LX, LW, EPI, 128, 128, 2, 2, true>(a, z, st);
+int launch_shape(const GemmArgs &a, bool big, bool aligned, int z, hipStream_t st) {
+    if constexpr (W3D_LIN_DT != W3D_DTYPE_F32) {
+        if (big) return launch_kernel(gemm_pipe_kernel<W3D_LIN_DT, LX, LW, EPI>, 512, Pipe<W3D_LIN_DT, LX, LW, EPI>::LDS_BYTES, a, z, st);
+    }
+    typedef Gemm<W3D_LIN_DT, LX, LW, EPI, 128, 128, 2, 2, true> G;
+    if (aligned) return launch_kernel(gemm_kernel<W3D_LIN_DT, LX, LW, EPI, 128, 128, 2, 2, true>, G::NT, G::LDS_BYTES, a, z, st);
+    return launch_kernel(gemm_kernel<W3D_LIN_DT, LX, LW, EPI, 128, 128, 2, 2, false>, G::NT, G::LDS_BYTES, a, z, st);
 }
-int launch_prod(const GemmArgs &a, int prod, bool aligned, int z, hipStream_t st) {
+int launch_prod(const GemmArgs &a, int prod, bool big, bool aligned, int z, hipStream_t st) {
     switch (prod) {
-        case PROD_LINEAR: return launch_shape<K_ROWS, K_ROWS, EPI_LINEAR>(a, aligned, z, st);
-        case PROD_GATED: return launch_shape<K_ROWS, K_ROWS, EPI_GATED>(a, aligned, z, st);
+        case PROD_LINEAR: return launch_shape<K_ROWS, K_ROWS, EPI_LINEAR>(a, big, aligned, z, st);
+        case PROD_GATED: return launch_shape<K_ROWS, K_ROWS, EPI_GATED>(a, big, aligned, z, st);
         default: break;
     }
     if constexpr (W3D_LIN_DT != W3D_DTYPE_FP8_E4M3) {
         switch (prod) {
-            case PROD_LINEAR_BWD: return launch_shape<K_ROWS, K_ROWS, EPI_LINEAR_BWD>(a, aligned, z, st);
-            case PROD_GATED_BWD: return launch_shape<K_ROWS, K_ROWS, EPI_GATED_BWD>(a, aligned, z, st);
-            case PROD_DX: return launch_shape<K_ROWS, M_ROWS, EPI_STORE>(a, aligned, z, st);
-            case PROD_DW: return launch_shape<M_ROWS, M_ROWS, EPI_STORE>(a, aligned, z, st);
+            case PROD_LINEAR_BWD: return launch_shape<K_ROWS, K_ROWS, EPI_LINEAR_BWD>(a, big, aligned, z, st);
+            case PROD_GATED_BWD: return launch_shape<K_ROWS, K_ROWS, EPI_GATED_BWD>(a, big, aligned, z, st);
+            case PROD_DX: return launch_shape<K_ROWS, M_ROWS, EPI_STORE>(a, big, aligned, z, st);
+            case PROD_DW: return launch_shape<M_ROWS, M_ROWS, EPI_STORE>(a, big, aligned, z, st);
             default: break;
         }
     }
@@ -194,7 +195,7 @@ int launch_skinny(const GemmArgs &a, hipStream_t st) {
 #else
 #define W3D_LIN_NAME(f) f##_fp8
 #endif
-int W3D_LIN_NAME(w3d_lin_tiles)(const GemmArgs &a, int prod, bool aligned, int z, hipStream_t st) { return launch_prod(a, prod, aligned, z, st); }
+int W3D_LIN_NAME(w3d_lin_tiles)(const GemmArgs &a, int prod, bool big, bool aligned, int z, hipStream_t st) { return launch_prod(a, prod, big, aligned, z, st); }
 int W3D_LIN_NAME(w3d_lin_skinny)(const GemmArgs &a, int prod, hipStream_t st) {
     return prod == PROD_GATED ? launch_skinny<EPI_GATED>(a, st) : launch_skinny<EPI_LINEAR>(a, st);
 }
@@ -203,70 +204,81 @@ int W3D_LIN_NAME(w3d_lin_skinny)(const GemmArgs &a, int prod, hipStream_t st) {
 
 namespace {
 
-// Partial sums of a sliced product: part[slice][m][ld] -> the epilogue of the product, one lane per column, a strip of rows per block (column sums of dz per strip)
-constexpr int JOIN_ROWS = 32;
+// Partial sums of a sliced product: part[slice][m][ld] -> the epilogue of the product.  A block takes 64 columns of a strip of JOIN_ROWS rows, four rows at a time (one per wave), so that
+// the column sums of dz are complete per strip; the slices' loads are independent.
+constexpr int JOIN_ROWS = 16;
 template <int OT, int EPI>
-__global__ __launch_bounds__(256) void join_slices_kernel(GemmArgs a, int z_first) {
+__global__ __launch_bounds__(256) void join_slices_kernel(GemmArgs a) {
     constexpr int OB = Elem<OT>::B;
     constexpr bool GATED = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
-    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x, r0 = (int64_t)blockIdx.y * JOIN_ROWS;
-    const int64_t r1 = min(a.M, r0 + JOIN_ROWS);
+    __shared__ float sums[2][4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t n = (int64_t)blockIdx.x * 64 + lane, r0 = (int64_t)blockIdx.y * JOIN_ROWS;
     const int64_t pad = EPI == EPI_LINEAR_BWD ? a.ld_out / OB : EPI == EPI_GATED_BWD ? a.half_out / OB : a.N;
-    if (n >= pad) return;
-    const bool in = n < a.N;
+    const bool in = n < a.N, store = n < pad;
     const float b0 = bias_at<OT>(a.bias, a.bias_f32, n, a.N), b1 = GATED ? bias_at<OT>(a.bias2, a.bias_f32, n, a.N) : 0.f;
     const int s0 = a.ws && in ? a.ws[n] - 254 : 0, s1 = GATED && a.ws2 && in ? a.ws2[n] - 254 : 0;
-    const int64_t z = blockIdx.z + z_first;
+    const int64_t z = blockIdx.z, slice = a.M * a.part_ld;
+    float v[JOIN_ROWS / 4], u[JOIN_ROWS / 4];
+#pragma unroll
+    for (int i = 0; i < JOIN_ROWS / 4; ++i) {
+        v[i] = u[i] = 0.f;
+        const int64_t m = r0 + 4 * i + wave;
+        if (!in || m >= a.M) continue;
+        const float *p = a.part + (z * a.slices * a.M + m) * a.part_ld + n;
+        for (int s = 0; s < a.slices; ++s) {
+            v[i] += p[s * slice];
+            if (GATED) u[i] += p[s * slice + a.part_ld / 2];
+        }
+    }
     with_act(a.act, [&](auto act_c) {
         constexpr int ACT = decltype(act_c)::value;
         float c0 = 0.f, c1 = 0.f;
-        for (int64_t m = r0; m < r1; ++m) {
-            float v = 0.f, u = 0.f;
-            if (in)
-                for (int s = 0; s < a.slices; ++s) {
-                    const float *p = a.part + ((z * a.slices + s) * a.M + m) * a.part_ld + n;
-                    v += p[0];
-                    if (GATED) u += p[a.part_ld / 2];
-                }
-            if (a.xs) { v = __builtin_ldexpf(v, a.xs[m] + s0); if (GATED) u = __builtin_ldexpf(u, a.xs[m] + s1); }
-            v += b0; u += b1;
+#pragma unroll
+        for (int i = 0; i < JOIN_ROWS / 4; ++i) {
+            const int64_t m = r0 + 4 * i + wave;
+            if (!store || m >= a.M) continue;
+            float x = v[i], y = u[i];
+            if (a.xs) { x = __builtin_ldexpf(x, a.xs[m] + s0); if (GATED) y = __builtin_ldexpf(y, a.xs[m] + s1); }
+            x += b0; y += b1;
             uint8_t *o = (EPI == EPI_STORE && z ? a.out2 : a.out) + m * a.ld_out + n * OB;
-            if (EPI == EPI_STORE) store1<OT>(o, v);
+            if (EPI == EPI_STORE) store1<OT>(o, x);
             else if (EPI == EPI_LINEAR) {
-                v = act_fwd<ACT>(v);
-                if (a.res) v += load1<OT>(a.res + (m * a.N + n) * OB);
-                store1<OT>(o, v);
-            } else if (EPI == EPI_GATED) store1<OT>(o, act_fwd<ACT>(v) * u);
+                x = act_fwd<ACT>(x);
+                if (a.res) x += load1<OT>(a.res + (m * a.N + n) * OB);
+                store1<OT>(o, x);
+            } else if (EPI == EPI_GATED) store1<OT>(o, act_fwd<ACT>(x) * y);
             else {
                 float act, der;
-                act_both<ACT>(v, act, der);
+                act_both<ACT>(x, act, der);
                 const float dy = in ? load1<OT>(a.dy + (m * a.N + n) * OB) : 0.f;
-                if (EPI == EPI_LINEAR_BWD) v = in ? dy * der : 0.f;
-                else { v = in ? dy * (u * der) : 0.f; u = in ? dy * act : 0.f; store1<OT>(o + a.half_out, u); c1 += u; }
-                store1<OT>(o, v);
-                c0 += v;
+                if (EPI == EPI_LINEAR_BWD) x = in ? dy * der : 0.f;
+                else { x = in ? dy * (y * der) : 0.f; y = in ? dy * act : 0.f; store1<OT>(o + a.half_out, y); c1 += y; }
+                store1<OT>(o, x);
+                c0 += x;
             }
         }
-        if ((EPI == EPI_LINEAR_BWD || EPI == EPI_GATED_BWD) && a.colsum && in) {
-            float *o = a.colsum + (int64_t)blockIdx.y * a.colsum_ld + n;
-            o[0] = c0;
-            if (GATED) o[a.colsum_ld / 2] = c1;
+        if ((EPI == EPI_LINEAR_BWD || EPI == EPI_GATED_BWD) && a.colsum) {
+            sums[0][wave][lane] = c0;
+            if (GATED) sums[1][wave][lane] = c1;
+            __syncthreads();
+            if (wave < (GATED ? 2 : 1) && in)
+                a.colsum[(int64_t)blockIdx.y * a.colsum_ld + wave * (a.colsum_ld / 2) + n] = (sums[wave][0][lane] + sums[wave][1][lane]) + (sums[wave][2][lane] + sums[wave][3][lane]);
         }
     });
 }
 template <int OT>
 int join_as(const GemmArgs &a, int prod, int z, hipStream_t st) {
     const int64_t cols = prod == PROD_LINEAR_BWD ? a.ld_out / Elem<OT>::B : prod == PROD_GATED_BWD ? a.half_out / Elem<OT>::B : a.N;
-    // (grid.y is limited to 65 535: longer matrices in turns of whole strips)
     const int64_t strips = (a.M + JOIN_ROWS - 1) / JOIN_ROWS;
-    if (strips > 65535) return W3D_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)((cols + 255) / 256), (unsigned)strips, z), block(256);
+    if (strips > 65535) return W3D_ERR_UNSUPPORTED;                      // (sliced products have few tiles: see cut_of)
+    const dim3 grid((unsigned)((cols + 63) / 64), (unsigned)strips, z), block(256);
     switch (prod) {
-        case PROD_LINEAR: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_LINEAR>), grid, block, 0, st, a, 0); break;
-        case PROD_GATED: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_GATED>), grid, block, 0, st, a, 0); break;
-        case PROD_LINEAR_BWD: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_LINEAR_BWD>), grid, block, 0, st, a, 0); break;
-        case PROD_GATED_BWD: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_GATED_BWD>), grid, block, 0, st, a, 0); break;
-        default: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_STORE>), grid, block, 0, st, a, 0); break;
+        case PROD_LINEAR: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_LINEAR>), grid, block, 0, st, a); break;
+        case PROD_GATED: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_GATED>), grid, block, 0, st, a); break;
+        case PROD_LINEAR_BWD: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_LINEAR_BWD>), grid, block, 0, st, a); break;
+        case PROD_GATED_BWD: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_GATED_BWD>), grid, block, 0, st, a); break;
+        default: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_STORE>), grid, block, 0, st, a); break;
     }
     W3D_CHECK_LAUNCH();
     return W3D_OK;
@@ -277,20 +289,28 @@ bool float_dtype(int t) { return t == W3D_DTYPE_F32 || t == W3D_DTYPE_BF16 || t 
 int64_t ceil_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 bool aligned16(const void *p, int64_t ld) { return !(((uintptr_t)p) & 15) && ld % 16 == 0; }
 
-// How a product is cut.  When the tiles are fewer than the CUs, the contraction is cut until the blocks are about two per CU, each slice at least four slabs long (a slice costs a round
-// trip of its f32 tile).
-struct Cut { int slices; int64_t tiles_m, tiles_n; };
-Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool gated, int batch) {
-    const int bn = gated ? 64 : 128;
-    Cut c;
-    c.tiles_m = (M + 127) / 128; c.tiles_n = (N + bn - 1) / bn;
-    const int64_t tiles = c.tiles_m * c.tiles_n * batch, slabs = (K * eb_of(dtype) + SLAB - 1) / SLAB;
-    int64_t s = 1;
-    if (tiles < 256) s = 512 / tiles;
-    if (s > slabs / 4) s = slabs / 4;
-    if (s > 32) s = 32;
-    c.slices = (int)(s < 1 ? 1 : s);
-    return c;
+// How a product is cut: tile size and slices of the contraction, by the time they would take.  Microseconds per 128-byte slab of a full chip, measured: 256 x 256 tiles, one block a CU;
+// 128 x 128 tiles, two blocks a CU; a round of tiles starts and ends once (fill, epilogue).  Slices write and read their f32 tiles (4 TB/s) and take a second launch.
+struct Cut { bool big; int slices; int64_t tiles_m, tiles_n; };
+Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool gated, bool aligned, int batch) {
+    const int parts = gated ? 2 : 1;
+    const int64_t slabs = (K * eb_of(dtype) + SLAB - 1) / SLAB;
+    Cut best = {};
+    double best_t = 0;
+    for (int big = 0; big < (aligned && dtype != W3D_DTYPE_F32 ? 2 : 1); ++big) {
+        const int b = big ? 256 : 128;
+        const int64_t tm = (M + b - 1) / b, tn = (N * parts + b - 1) / b, tiles = tm * tn * batch;
+        const double slab_us = big ? (dtype == W3D_DTYPE_FP8_E4M3 ? 0.9 : 1.15) : dtype == W3D_DTYPE_F32 ? 6.0 : 1.6, round_us = big ? 6.0 : 5.0, slots = big ? 256 : 512;
+        for (int s = 1; s <= 32 && (s == 1 || slabs / s >= 4); ++s) {
+            const double rounds = (double)((tiles * s + (int64_t)slots - 1) / (int64_t)slots);
+            // (a partial round of the small tiles runs with one block a CU, in less time than two)
+            const double fill = !big && tiles * s <= 256 ? 0.6 : 1.0;
+            double t = rounds * (fill * slab_us * (double)((slabs + s - 1) / s) + round_us);
+            if (s > 1) t += 4.0 + 8.0 * (double)s * (double)batch * (double)M * (double)N * parts / 4e6;
+            if (best_t == 0 || t < best_t) { best_t = t; best = {big != 0, s, tm, tn}; }
+        }
+    }
+    return best;
 }
 size_t part_bytes(const Cut &c, int64_t M, int64_t N, bool gated, int batch) {
     return c.slices > 1 ? (size_t)batch * c.slices * M * ceil_to(N, 16) * (gated ? 2 : 1) * 4 : 0;
@@ -303,10 +323,10 @@ int run_product(GemmArgs &a, int prod, int dtype, const Cut &c, bool aligned, in
     a.part_ld = ceil_to(a.N, 16) * (prod == PROD_GATED || prod == PROD_GATED_BWD ? 2 : 1);
     int rc;
     switch (dtype) {
-        case W3D_DTYPE_F32: rc = w3d_lin_tiles_f32(a, prod, aligned, z, st); break;
-        case W3D_DTYPE_BF16: rc = w3d_lin_tiles_bf16(a, prod, aligned, z, st); break;
-        case W3D_DTYPE_F16: rc = w3d_lin_tiles_f16(a, prod, aligned, z, st); break;
-        default: rc = w3d_lin_tiles_fp8(a, prod, aligned, z, st); break;
+        case W3D_DTYPE_F32: rc = w3d_lin_tiles_f32(a, prod, c.big, aligned, z, st); break;
+        case W3D_DTYPE_BF16: rc = w3d_lin_tiles_bf16(a, prod, c.big, aligned, z, st); break;
+        case W3D_DTYPE_F16: rc = w3d_lin_tiles_f16(a, prod, c.big, aligned, z, st); break;
+        default: rc = w3d_lin_tiles_fp8(a, prod, c.big, aligned, z, st); break;
     }
     if (rc != W3D_OK || c.slices == 1) return rc;
     switch (a.out_dt) {
@@ -344,15 +364,17 @@ int forward(const void *x, const int32_t *xs, const void *w, const int32_t *ws, 
         }
     }
     const bool aligned = aligned16(x, ld) && aligned16(w, ld) && aligned16(w2, ld);
-    const Cut c = cut_of(R, N, K, dtype, gated, 1);
+    const Cut c = cut_of(R, N, K, dtype, gated, aligned, 1);
     if (c.slices > 1 && (!workspace || (((uintptr_t)workspace) & 15) || workspace_bytes < part_bytes(c, R, N, gated, 1))) return W3D_ERR_WORKSPACE;
     a.part = (float *)workspace;
     return run_product(a, prod, dtype, c, aligned, 1, st);
 }
 
+// the larger of the two cuts a call may take (its alignment is not known to the workspace query)
 size_t forward_bytes(int64_t R, int64_t K, int64_t N, int dtype, bool gated) {
     if (R <= SKINNY_ROWS || K < 1 || N < 1) return 0;
-    return part_bytes(cut_of(R, N, K, dtype, gated, 1), R, N, gated, 1);
+    const size_t p = part_bytes(cut_of(R, N, K, dtype, gated, true, 1), R, N, gated, 1), q = part_bytes(cut_of(R, N, K, dtype, gated, false, 1), R, N, gated, 1);
+    return p > q ? p : q;
 }
 
 // ---- backward.  Workspace: dz | column sums | partial tiles (of one product at a time)
@@ -361,6 +383,8 @@ struct Bwd {
     int64_t dz_bytes, strips, colsum_ld, colsum_bytes, part;
 };
 int64_t max64(int64_t a, int64_t b) { return a > b ? a : b; }
+// strips of partial column sums that the product forming dz writes: two per tile row, or the joining launch's
+int64_t strips_of(const Cut &c, int64_t R) { return c.slices > 1 ? (R + JOIN_ROWS - 1) / JOIN_ROWS : c.tiles_m * 2; }
 Bwd bwd_plan(int64_t R, int64_t K, int64_t N, int dtype, bool gated, bool no_act) {
     Bwd b;
     const int eb = eb_of(dtype), parts = gated ? 2 : 1;
@@ -369,10 +393,15 @@ Bwd bwd_plan(int64_t R, int64_t K, int64_t N, int dtype, bool gated, bool no_act
     b.dz_bytes = no_act ? 0 : ceil_to(R * b.ld_dz, 256);
     b.colsum_ld = ceil_to(N, 16) * parts;
     b.part = 0;
-    const Cut z = cut_of(R, N, K, dtype, gated, 1), dx = cut_of(R, K, gated ? 2 * b.pad : N, dtype, false, 1), dw = cut_of(N, K, R, dtype, false, parts);
-    b.strips = no_act ? w3d_column_strips(R, N) : z.slices > 1 ? (R + JOIN_ROWS - 1) / JOIN_ROWS : z.tiles_m * 2;
-    if (!no_act) b.part = (int64_t)part_bytes(z, R, N, gated, 1);
-    b.part = max64(b.part, max64((int64_t)part_bytes(dx, R, K, false, 1), (int64_t)part_bytes(dw, N, K, false, parts)));
+    b.strips = no_act ? w3d_column_strips(R, N) : 0;
+    for (int al = 0; al < 2; ++al) {
+        const Cut z = cut_of(R, N, K, dtype, gated, al, 1), dx = cut_of(R, K, gated ? 2 * b.pad : N, dtype, false, al, 1), dw = cut_of(N, K, R, dtype, false, al, parts);
+        if (!no_act) {
+            b.strips = max64(b.strips, strips_of(z, R));
+            b.part = max64(b.part, (int64_t)part_bytes(z, R, N, gated, 1));
+        }
+        b.part = max64(b.part, max64((int64_t)part_bytes(dx, R, K, false, 1), (int64_t)part_bytes(dw, N, K, false, parts)));
+    }
     b.colsum_bytes = ceil_to(b.strips * b.colsum_ld * 4, 256);
     return b;
 }
@@ -403,10 +432,10 @@ int backward(const void *x, const void *w, const void *w2, const void *bias, con
         a.vec_io = aligned16(dy, N * eb);
         a.colsum = db || db2 ? colsum : nullptr; a.colsum_ld = b.colsum_ld; a.part = part;
         const bool al = aligned16(x, K * eb) && aligned16(w, K * eb) && aligned16(w2, K * eb);
-        const Cut c = cut_of(R, N, K, dtype, gated, 1);
+        const Cut c = cut_of(R, N, K, dtype, gated, al, 1);
         const int rc = run_product(a, gated ? PROD_GATED_BWD : PROD_LINEAR_BWD, dtype, c, al, 1, st);
         if (rc != W3D_OK) return rc;
-        strips = b.strips;
+        strips = strips_of(c, R);
         dz = ws; ld_dz = b.ld_dz;
     } else if (R > 0 && db) {
         const int rc = w3d_column_sums(dy, R, N, dtype, colsum, b.colsum_ld, st);
@@ -422,7 +451,7 @@ int backward(const void *x, const void *w, const void *w2, const void *bias, con
         a.out = (uint8_t *)dx; a.ld_out = K * eb; a.out_dt = dtype; a.part = part;
         a.vec_io = aligned16(dx, K * eb);
         const bool al = aligned16(dz, ld_dz) && aligned16(w, K * eb) && aligned16(w2, K * eb);
-        const int rc = run_product(a, PROD_DX, dtype, cut_of(R, K, a.K, dtype, false, 1), al, 1, st);
+        const int rc = run_product(a, PROD_DX, dtype, cut_of(R, K, a.K, dtype, false, al, 1), al, 1, st);
         if (rc != W3D_OK) return rc;
     }
     // weight gradients: the two halves of a gated layer are one launch (blockIdx.z) when both are wanted
@@ -442,7 +471,7 @@ int backward(const void *x, const void *w, const void *w2, const void *bias, con
         a.out = (uint8_t *)o; a.out2 = (uint8_t *)dw2; a.ld_out = K * eb; a.out_dt = dtype; a.part = part;
         a.vec_io = aligned16(o, K * eb) && aligned16(both ? dw2 : nullptr, 0);
         const bool al = aligned16(a.x, ld_dz) && aligned16(x, K * eb);
-        const int rc = run_product(a, PROD_DW, dtype, cut_of(N, K, R, dtype, false, parts), al, both ? 2 : 1, st);
+        const int rc = run_product(a, PROD_DW, dtype, cut_of(N, K, R, dtype, false, al, parts), al, both ? 2 : 1, st);
         if (rc != W3D_OK) return rc;
     }
     return W3D_OK;

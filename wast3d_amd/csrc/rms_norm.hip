@@ -3,6 +3,7 @@
 //
 //   s = x + residual;  r = 1 / sqrt(mean(s^2) + eps);  y = s r w
 //   given dy (and ds, what reaches s from elsewhere):  g = dy w;  x^ = s r;  dx = r (g - x^ mean(g x^)) + ds;  dw = sum over rows of dy x^
+// The backward pass forms s again from x and the residual, unrounded: from the rounded s its error would show in dw (1.5 x the error of one rounding).
 //
 // Bound by HBM: every element is read once and written once.  A row stays in registers between its sum and its output, in f32; sums are f32.
 // G lanes share a row (a wave holds 64 / G rows), 8 elements per lane and vector, NV vectors per lane: G x NV is the smallest that covers the row, wide
@@ -31,6 +32,18 @@ __device__ __forceinline__ void load_weight(const char *w, int w_f32, int c, int
         for (int i = 0; i < 8; ++i) v[i] = 1.f;
     } else if (w_f32) load8<W3D_DTYPE_F32>(w + (int64_t)c * 4, d - c, v);
     else load8<DT>(w + (int64_t)c * Elem<DT>::B, d - c, v);
+}
+
+// 8 elements of s = x + residual, in f32
+template <int DT, typename A>
+__device__ __forceinline__ void sum_row(const A &a, int64_t at, int c, float (&s)[8]) {
+    load8<DT>(a.x + (at + c) * Elem<DT>::B, a.d - c, s);
+    if (a.res) {
+        float t[8];
+        load8<DT>(a.res + (at + c) * Elem<DT>::B, a.d - c, t);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] += t[i];
+    }
 }
 
 // sum / maximum over the G lanes of a row; G = 256: over the block (red: 4 floats of LDS per slot; every lane of the block calls)
@@ -89,13 +102,7 @@ __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_kernel(NormArgs a) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int c = c0 + v * G * 8;
-            load8<DT>(a.x + (at + c) * EB, a.d - c, s[v]);
-            if (a.res) {
-                float t[8];
-                load8<DT>(a.res + (at + c) * EB, a.d - c, t);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) s[v][i] += t[i];
-            }
+            sum_row<DT>(a, at, c, s[v]);
         }
 #pragma unroll
         for (int v = 0; v < NV; ++v)
@@ -130,16 +137,6 @@ __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_kernel(NormArgs a) {
 }
 
 // rows of more than 256 x 8 x 4 elements: one block per row, the row read again for every pass over it
-template <int DT>
-__device__ __forceinline__ void sum_row(const NormArgs &a, int64_t at, int c, float (&s)[8]) {
-    load8<DT>(a.x + (at + c) * Elem<DT>::B, a.d - c, s);
-    if (a.res) {
-        float t[8];
-        load8<DT>(a.res + (at + c) * Elem<DT>::B, a.d - c, t);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s[i] += t[i];
-    }
-}
 template <int DT>
 __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_wide_kernel(NormArgs a) {
     constexpr int EB = Elem<DT>::B;
@@ -181,7 +178,7 @@ __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_wide_kernel(NormArgs a) {
 // ---- backward: the rows of a block are walked by the same lanes, so every lane keeps the weight gradient of its own columns in registers; the block's rows are folded in LDS, the
 // blocks' partial sums by a second launch in a fixed order (no atomics: the same bits every time)
 struct NormBwdArgs {
-    const char *s, *w, *dy, *ds;
+    const char *x, *res, *w, *dy, *ds;
     const float *rstd;
     char *dx;
     float *part;                 // [gridDim.x][d] or NULL
@@ -212,7 +209,7 @@ __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_bwd_kernel(NormBwdArgs a)
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int c = c0 + v * G * 8;
-            load8<DT>(a.s + (at + c) * EB, a.d - c, x[v]);
+            sum_row<DT>(a, at, c, x[v]);
             load8<DT>(a.dy + (at + c) * EB, a.d - c, g[v]);
         }
 #pragma unroll
@@ -268,7 +265,7 @@ __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_bwd_wide_kernel(NormBwdAr
         const float rs = a.rstd[r];
         float dot = 0.f, x[8], g[8], w[8];
         for (int c = threadIdx.x * 8; c < a.d; c += NORM_BLOCK * 8) {
-            load8<DT>(a.s + (at + c) * EB, a.d - c, x);
+            sum_row<DT>(a, at, c, x);
             load8<DT>(a.dy + (at + c) * EB, a.d - c, g);
             load_weight<DT>(a.w, a.w_f32, c, a.d, w);
 #pragma unroll
@@ -277,7 +274,7 @@ __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_bwd_wide_kernel(NormBwdAr
         dot = group_reduce<256, false>(dot, red) * a.inv_d;
         for (int c = threadIdx.x * 8; c < a.d; c += NORM_BLOCK * 8) {
             float t[8];
-            load8<DT>(a.s + (at + c) * EB, a.d - c, x);
+            sum_row<DT>(a, at, c, x);
             load8<DT>(a.dy + (at + c) * EB, a.d - c, g);
             load_weight<DT>(a.w, a.w_f32, c, a.d, w);
             if (a.ds) load8<DT>(a.ds + (at + c) * EB, a.d - c, t);
@@ -296,7 +293,7 @@ __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_dw_wide_kernel(NormBwdArg
     float dw[8] = {};
     for (int64_t r = blockIdx.y; r < a.R; r += gridDim.y) {
         float x[8], g[8];
-        load8<DT>(a.s + (r * a.d + c) * EB, a.d - c, x);
+        sum_row<DT>(a, r * a.d, c, x);
         load8<DT>(a.dy + (r * a.d + c) * EB, a.d - c, g);
         const float rs = a.rstd[r];
 #pragma unroll
@@ -404,16 +401,16 @@ extern "C" size_t w3d_rms_norm_bwd_workspace_bytes(int64_t R, int d) {
 }
 int w3d_fold_columns(const float *part, int parts, int64_t ld, int64_t n, void *out, int out_dtype, hipStream_t st);      // columns.hip
 
-extern "C" int w3d_rms_norm_bwd(const void *s, const void *weight, int weight_dtype, const float *rstd, const void *dy, const void *ds, int64_t R, int d, int dtype, void *dx,
+extern "C" int w3d_rms_norm_bwd(const void *x, const void *residual, const void *weight, int weight_dtype, const float *rstd, const void *dy, const void *ds, int64_t R, int d, int dtype, void *dx,
                                 void *dweight, void *workspace, size_t workspace_bytes, w3d_stream_t stream) {
     if (R < 0 || d < 1 || !dtype_ok(dtype) || (!dx && !dweight)) return W3D_ERR_ARG;
     if ((weight || dweight) && weight_dtype != dtype && weight_dtype != W3D_DTYPE_F32) return W3D_ERR_ARG;
-    if (R > 0 && (!s || !rstd || !dy)) return W3D_ERR_ARG;
+    if (R > 0 && (!x || !rstd || !dy)) return W3D_ERR_ARG;
     hipStream_t st = w3d_s(stream);
     const int blocks = R > 0 ? blocks_for(R, d) : 0;
     if (R > 0) {
         if (dweight && (!workspace || workspace_bytes < w3d_rms_norm_bwd_workspace_bytes(R, d))) return W3D_ERR_WORKSPACE;
-        NormBwdArgs a = {(const char *)s, (const char *)weight, (const char *)dy, (const char *)ds, rstd, (char *)dx, dweight ? (float *)workspace : nullptr, R, d,
+        NormBwdArgs a = {(const char *)x, (const char *)residual, (const char *)weight, (const char *)dy, (const char *)ds, rstd, (char *)dx, dweight ? (float *)workspace : nullptr, R, d,
                          weight_dtype == W3D_DTYPE_F32 && dtype != W3D_DTYPE_F32, 1.0f / (float)d};
         if (dtype == W3D_DTYPE_F32) launch_bwd<W3D_DTYPE_F32>(a, blocks, st);
         else if (dtype == W3D_DTYPE_BF16) launch_bwd<W3D_DTYPE_BF16>(a, blocks, st);

@@ -1451,12 +1451,12 @@ def raw_rms_norm(x, weight, residual, eps: float, y, s=None, rstd=None):
           "w3d_rms_norm_fwd")
 
 
-def raw_rms_norm_bwd(s, weight, rstd, dy, ds, dx=None, dweight=None):
-    """dx [R,d] and / or dweight [d] of contiguous rows (s: what the norm was taken of)."""
-    R, d = s.shape
-    ws = _scratch(lib().w3d_rms_norm_bwd_workspace_bytes(R, d) if dweight is not None else 0, s.device)
+def raw_rms_norm_bwd(x, residual, weight, rstd, dy, ds, dx=None, dweight=None):
+    """dx [R,d] (also the residual's gradient) and / or dweight [d] of contiguous rows."""
+    R, d = x.shape
+    ws = _scratch(lib().w3d_rms_norm_bwd_workspace_bytes(R, d) if dweight is not None else 0, x.device)
     wdt = _dtype_code(weight) if weight is not None else 0
-    check(lib().w3d_rms_norm_bwd(ptr(s), ptr(weight), wdt, ptr(rstd), ptr(dy), ptr(ds), R, d, _dtype_code(s), ptr(dx), ptr(dweight), ptr(ws), ws.numel() if ws is not None else 0,
+    check(lib().w3d_rms_norm_bwd(ptr(x), ptr(residual), ptr(weight), wdt, ptr(rstd), ptr(dy), ptr(ds), R, d, _dtype_code(x), ptr(dx), ptr(dweight), ptr(ws), ws.numel() if ws is not None else 0,
                                  stream_ptr()), "w3d_rms_norm_bwd")
 
 
@@ -1465,37 +1465,33 @@ class _RmsNorm(torch.autograd.Function):
     def forward(ctx, x, weight, residual, eps):
         xc = x.contiguous()
         wc = weight.contiguous() if weight is not None else None
+        rc = residual.contiguous() if residual is not None else None
         d = xc.shape[-1]
         rows = xc.view(-1, d)
         y = torch.empty_like(xc)
-        s = torch.empty_like(xc) if residual is not None else None
+        s = torch.empty_like(xc) if rc is not None else None
         rstd = torch.empty(rows.shape[0], dtype=torch.float32, device=x.device)
         with _on_device_of(x):
-            raw_rms_norm(rows, wc, residual.contiguous().view(-1, d) if residual is not None else None, eps, y, s, rstd)
-        ctx.save_for_backward(s if s is not None else xc, wc, rstd)
+            raw_rms_norm(rows, wc, rc, eps, y, s, rstd)
+        ctx.save_for_backward(xc, rc, wc, rstd)
         ctx.set_materialize_grads(False)
         return y if s is None else (y, s)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gy, gs=None):
-        s, w, rstd = ctx.saved_tensors
+        x, res, w, rstd = ctx.saved_tensors
         want_x, want_w, want_r, _ = ctx.needs_input_grad
-        d = s.shape[-1]
-        dw = None
-        if gy is None:                                             # only s was used: its gradient passes through
-            dx = gs
-            if want_w:
-                dw = torch.zeros_like(w)
+        d = x.shape[-1]
+        dw = torch.empty_like(w) if want_w else None
+        if gy is None or x.numel() == 0:                           # only s was used: its gradient passes through
+            dx = gs if gy is None else torch.empty_like(x)
+            dw = dw.zero_() if want_w else None
         else:
-            dx = torch.empty_like(s) if want_x or want_r else None
-            dw = torch.empty_like(w) if want_w else None
-            if s.numel() == 0:
-                dw = dw.zero_() if dw is not None else None
-            else:
-                with _on_device_of(s):
-                    clear_stale_hip_error()
-                    raw_rms_norm_bwd(s.view(-1, d), w, rstd, gy.contiguous(), gs.contiguous() if gs is not None else None, dx, dw)
+            dx = torch.empty_like(x) if want_x or want_r else None
+            with _on_device_of(x):
+                clear_stale_hip_error()
+                raw_rms_norm_bwd(x.view(-1, d), res, w, rstd, gy.contiguous(), gs.contiguous() if gs is not None else None, dx, dw)
         return dx if want_x else None, dw, dx if want_r else None, None
 
 
