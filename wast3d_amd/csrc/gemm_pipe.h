@@ -84,24 +84,30 @@ struct Pipe {
         const int64_t wk = LW == M_ROWS ? a.w_rows : a.K;                                      // contraction elements of W that exist (per stacked matrix)
         const bool split = LW == M_ROWS && !GATED && a.k_split > 0;
 
-        auto start = [&](int64_t t) {
-            uint8_t *buf = smem + (int)(t & (PIPE_RING - 1)) * BUF + wave * 1024;
+        // transfers of slab t: addresses, then the four issues.  Slabs past the contraction's end are all out of range (nothing is read), so that every turn is alike.
+        const uint8_t *bx, *bw, *bw1;
+        uint32_t off[4];
+        uint8_t *to;
+        auto prepare = [&](int64_t t) {
             const int64_t k0 = t * KPS;
             const bool second = split && k0 >= a.k_split;
-            const int64_t xl = a.K - k0, wl = (second ? a.k_split + wk : wk) - k0;
-            const uint8_t *bx = mx.base + t * mx.step, *bw = (second ? mw.base2 : mw.base) + t * mw.step, *bw1 = GATED ? mw.base2 + t * mw.step : bw;
-            uint32_t o[4] = {mx.off[0], mx.off[1], mw.off[0], mw.off[1]};
-            if (xl < KPS || wl < KPS) {                                                        // the last slab: pieces behind the end are zeros
+            const int64_t xl64 = a.K - k0, wl64 = (second ? a.k_split + wk : wk) - k0;
+            const int xl = (int)(xl64 < KPS ? xl64 : KPS), wl = (int)(wl64 < KPS ? wl64 : KPS);
+            bx = mx.base + t * mx.step;
+            bw = (second ? mw.base2 : mw.base) + t * mw.step;
+            bw1 = GATED ? mw.base2 + t * mw.step : bw;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    if (mx.k_of[i] >= xl) o[i] = OUT_OF_RANGE;
-                    if (mw.k_of[i] >= wl) o[2 + i] = OUT_OF_RANGE;
-                }
+            for (int i = 0; i < 2; ++i) {
+                off[i] = mx.k_of[i] < xl ? mx.off[i] : OUT_OF_RANGE;
+                off[2 + i] = mw.k_of[i] < wl ? mw.off[i] : OUT_OF_RANGE;
             }
-            issue(bx, o[0], buf);
-            issue(bx, o[1], buf + NT * 16);
-            issue(bw, o[2], buf + SIDE);
-            issue(bw1, o[3], buf + SIDE + NT * 16);
+            to = smem + (int)(t & (PIPE_RING - 1)) * BUF + wave * 1024;
+        };
+        auto fire = [&]() {
+            issue(bx, off[0], to);
+            issue(bx, off[1], to + NT * 16);
+            issue(bw, off[2], to + SIDE);
+            issue(bw1, off[3], to + SIDE + NT * 16);
         };
 
         typename O::Acc acc;
@@ -136,10 +142,8 @@ struct Pipe {
         }
 
 #pragma unroll
-        for (int i = 0; i < 3; ++i)
-            if (t0 + i < t1) start(t0 + i);
-        if (t0 + 3 <= t1) __builtin_amdgcn_s_waitcnt(W3D_WAIT_VM(8));
-        else __builtin_amdgcn_s_waitcnt(W3D_WAIT_VM(0));
+        for (int i = 0; i < 3; ++i) { prepare(t0 + i); fire(); }
+        __builtin_amdgcn_s_waitcnt(W3D_WAIT_VM(8));
         __builtin_amdgcn_s_barrier();
         if (group == 1) __builtin_amdgcn_s_barrier();                                          // half a turn behind
         for (int64_t t = t0; t < t1; ++t) {
@@ -147,12 +151,13 @@ struct Pipe {
             i32x4 xf[8], wf[4];                                                                // fp8: pairs of them are one operand
             read_side<LX, 8>(ax, at, xf);
             read_side<LW, 4>(aw, at, wf);
+            prepare(t + 3);
             __builtin_amdgcn_sched_barrier(0);
-            if (t + 3 < t1) { start(t + 3); __builtin_amdgcn_s_waitcnt(W3D_WAIT_VM(8)); }
-            else __builtin_amdgcn_s_waitcnt(W3D_WAIT_VM(0));
+            __builtin_amdgcn_s_waitcnt(W3D_WAIT_VM(4));
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_setprio(1);
+            fire();
             if constexpr (MS == 16) {
 #pragma unroll
                 for (int i = 0; i < FM; ++i)
@@ -169,10 +174,18 @@ struct Pipe {
                     for (int j = 0; j < FN; ++j)
                         acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(join8(wf[2 * j], wf[2 * j + 1]), join8(xf[2 * i], xf[2 * i + 1]), acc[i][j], 0, 0, 0, 127, 0, 127);
             }
-            __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, MS == 16 ? 6 : 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, MS == 16 ? 8 : 0, 0);
             __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_s_barrier();
         }
+        __builtin_amdgcn_s_waitcnt(W3D_WAIT_VM(0));
+        __builtin_amdgcn_s_barrier();                                                          // nothing is in flight into the slabs' LDS, which becomes the waves' patches
         if (group == 0) __builtin_amdgcn_s_barrier();                                          // as many barriers as the other group
         O::epilogue(a, acc, m0, n0, slice, tm, wm, wn, lane, z1, smem + wave * O::PATCH);
     }

@@ -218,9 +218,9 @@ struct Out {
     static constexpr int PARTS = GATED ? 2 : 1, BNP = BN / PARTS;                              // a gated tile is BN / 2 columns of each half: rows [0, BN/2) of the W slab gate, the rest up
     static constexpr int FM = BM / WM / MS, FN = BN / WN / MS, FP = FN / PARTS;
     static constexpr int COLS = BN / WN, PCOLS = COLS / PARTS, LPR = PCOLS / 8, RPP = 64 / LPR;      // lanes per row, rows per pass
-    static constexpr int ROWS = 64, CHUNKS = BM / WM / ROWS, PASSES = ROWS / RPP, AHEAD = 4;
+    static constexpr int ROWS = 64, CHUNKS = BM / WM / ROWS, PASSES = ROWS / RPP, AHEAD = 4, UN = EPI == EPI_GATED_BWD ? 1 : 2;      // UN passes at a time: their LDS reads, arithmetic and stores overlap
     static constexpr int PATCH = ROWS * COLS * 4;
-    static_assert(COLS == 64 && BM / WM % ROWS == 0 && AHEAD <= PASSES, "a patch row is 16 chunks; whole chunks of rows");
+    static_assert(COLS == 64 && BM / WM % ROWS == 0 && AHEAD <= PASSES && PASSES % UN == 0, "a patch row is 16 chunks; whole chunks of rows");
     typedef typename std::conditional<MS == 32, f32x16, f32x4>::type acc_t;
     typedef acc_t Acc[FM][FN];
 
@@ -242,15 +242,14 @@ struct Out {
             }
     }
     static __device__ __forceinline__ void get(const uint8_t *patch, int row, int part, int lane, float (&v)[8]) {
+        const int first = part * (PCOLS / 4) + 2 * (lane % LPR);
+        f32x4 t[2];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int chunk = part * (PCOLS / 4) + 2 * (lane % LPR) + c;
-            const f32x4 t = *reinterpret_cast<const f32x4 *>(patch + row * (COLS * 4) + ((chunk ^ (row & 15)) << 4));
+        for (int c = 0; c < 2; ++c) t[c] = *reinterpret_cast<const f32x4 *>(patch + row * (COLS * 4) + (((first + c) ^ (row & 15)) << 4));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[4 * c + e] = t[e];
-        }
+        for (int e = 0; e < 8; ++e) v[e] = t[e / 4][e % 4];
     }
-    // f(row m, row in the patch, 8 elements of src) for every row this lane finishes.  src: [M][N] of type OT or NULL; n: the lane's first column
+    // f(row m, row in the patch, 8 elements of src per pass) for every UN rows, RPP apart, that this lane finishes.  src: [M][N] of type OT or NULL; n: the lane's first column
     template <int OT, typename F>
     static __device__ __forceinline__ void each_row(const GemmArgs &a, const Acc &acc, const uint8_t *src, int64_t m0, int64_t n, int wm, int lane, uint8_t *patch, F f) {
         constexpr int OB = Elem<OT>::B, RAW = OB * 8 / 16;
@@ -276,17 +275,21 @@ struct Out {
             for (int i = 0; i < ROWS / MS; ++i) put(acc, c * (ROWS / MS) + i, lane, patch);
             __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
-            for (int p = 0; p < PASSES; ++p) {
+            for (int p = 0; p < PASSES; p += UN) {
                 const int64_t m = mw + c * ROWS + p * RPP;
-                float t[8] = {};
+                float t[UN][8] = {};
                 if (src) {
-                    if (fast) unpack8<OT>(ring[0], t);
-                    else if (m < a.M) load_run<OT, 8>(src + (m * a.N + n) * OB, a.N - n, false, t);
 #pragma unroll
-                    for (int k = 0; k + 1 < AHEAD; ++k)
+                    for (int k = 0; k < UN; ++k) {
+                        if (fast) unpack8<OT>(ring[k], t[k]);
+                        else if (m + k * RPP < a.M) load_run<OT, 8>(src + ((m + k * RPP) * a.N + n) * OB, a.N - n, false, t[k]);
+                    }
 #pragma unroll
-                        for (int q = 0; q < RAW; ++q) ring[k][q] = ring[k + 1][q];
-                    fetch(ring[AHEAD - 1]);
+                    for (int k = 0; k + UN < AHEAD; ++k)
+#pragma unroll
+                        for (int q = 0; q < RAW; ++q) ring[k][q] = ring[k + UN][q];
+#pragma unroll
+                    for (int k = 0; k < UN; ++k) fetch(ring[AHEAD - UN + k]);
                 }
                 f(m, p * RPP + lane / LPR, t);
             }
@@ -298,12 +301,14 @@ struct Out {
         const int64_t n = n0 + wn * PCOLS + 8 * (lane % LPR);
         if (a.slices > 1) {
             const int64_t z = (int64_t)(z1 ? a.slices : 0) + slice;
-            each_row<W3D_DTYPE_F32>(a, acc, nullptr, m0, n, wm, lane, patch, [&](int64_t m, int row, float (&)[8]) {
+            each_row<W3D_DTYPE_F32>(a, acc, nullptr, m0, n, wm, lane, patch, [&](int64_t m, int row, float (&)[UN][8]) {
+                float v[UN * PARTS][8];
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) {
-                    float v[8];
-                    get(patch, row, p, lane, v);
-                    if (m < a.M) store_run<W3D_DTYPE_F32, 8>((uint8_t *)(a.part + (z * a.M + m) * a.part_ld + p * (a.part_ld / 2) + n), a.N - n, true, v);
+                for (int k = 0; k < UN * PARTS; ++k) get(patch, row + k / PARTS * RPP, k % PARTS, lane, v[k]);
+#pragma unroll
+                for (int k = 0; k < UN * PARTS; ++k) {
+                    const int64_t mk = m + k / PARTS * RPP;
+                    if (mk < a.M) store_run<W3D_DTYPE_F32, 8>((uint8_t *)(a.part + (z * a.M + mk) * a.part_ld + k % PARTS * (a.part_ld / 2) + n), a.N - n, true, v[k]);
                 }
             });
             return;
@@ -321,10 +326,13 @@ struct Out {
         const bool vec = a.vec_io != 0;
         if constexpr (EPI == EPI_STORE) {
             uint8_t *out = z1 ? a.out2 : a.out;
-            each_row<OT>(a, acc, nullptr, m0, n, wm, lane, patch, [&](int64_t m, int row, float (&)[8]) {
-                float v[8];
-                get(patch, row, 0, lane, v);
-                if (m < a.M) store_run<OT, 8>(out + m * a.ld_out + n * OB, a.N - n, vec, v);
+            each_row<OT>(a, acc, nullptr, m0, n, wm, lane, patch, [&](int64_t m, int row, float (&)[UN][8]) {
+                float v[UN][8];
+#pragma unroll
+                for (int k = 0; k < UN; ++k) get(patch, row + k * RPP, 0, lane, v[k]);
+#pragma unroll
+                for (int k = 0; k < UN; ++k)
+                    if (m + k * RPP < a.M) store_run<OT, 8>(out + (m + k * RPP) * a.ld_out + n * OB, a.N - n, vec, v[k]);
             });
             return;
         }
@@ -338,48 +346,60 @@ struct Out {
             s0[e] = s1[e] = 0;
             if (DT == W3D_DTYPE_FP8_E4M3 && n + e < a.N) { s0[e] = a.ws[n + e] - 254; if (GATED) s1[e] = a.ws2[n + e] - 254; }
         }
-        each_row<OT>(a, acc, BWD ? a.dy : a.res, m0, n, wm, lane, patch, [&](int64_t m, int row, float (&t)[8]) {
-            const bool live = m < a.M;
-            float v[8], u[8];
-            get(patch, row, 0, lane, v);
-            if (GATED) get(patch, row, 1, lane, u);
-            if (DT == W3D_DTYPE_FP8_E4M3) {
-                const int xs = live ? a.xs[m] : 0;
+        each_row<OT>(a, acc, BWD ? a.dy : a.res, m0, n, wm, lane, patch, [&](int64_t m, int row, float (&t)[UN][8]) {
+            float v[UN][8], u[UN][8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) { v[e] = __builtin_ldexpf(v[e], xs + s0[e]); if (GATED) u[e] = __builtin_ldexpf(u[e], xs + s1[e]); }
+            for (int k = 0; k < UN; ++k) {
+                get(patch, row + k * RPP, 0, lane, v[k]);
+                if (GATED) get(patch, row + k * RPP, 1, lane, u[k]);
             }
+            if (DT == W3D_DTYPE_FP8_E4M3)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { v[e] += b0[e]; if (GATED) u[e] += b1[e]; }
+                for (int k = 0; k < UN; ++k) {
+                    const int xs = m + k * RPP < a.M ? a.xs[m + k * RPP] : 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) { v[k][e] = __builtin_ldexpf(v[k][e], xs + s0[e]); if (GATED) u[k][e] = __builtin_ldexpf(u[k][e], xs + s1[e]); }
+                }
             with_act(a.act, [&](auto act_c) {
                 constexpr int ACT = decltype(act_c)::value;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (!BWD) {
-                        v[e] = act_fwd<ACT>(v[e]);
-                        if (EPI == EPI_GATED) v[e] *= u[e];
-                    } else {
-                        float act, der;
-                        act_both<ACT>(v[e], act, der);
-                        if (EPI == EPI_LINEAR_BWD) v[e] = t[e] * der;
-                        else { v[e] = t[e] * (u[e] * der); u[e] = t[e] * act; }
+                for (int k = 0; k < UN; ++k)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float &z = v[k][e], &up = u[k][e];
+                        z += b0[e];
+                        if (GATED) up += b1[e];
+                        if (!BWD) {
+                            z = act_fwd<ACT>(z);
+                            if (EPI == EPI_GATED) z *= up;
+                        } else {
+                            float act, der;
+                            act_both<ACT>(z, act, der);
+                            if (EPI == EPI_LINEAR_BWD) z = t[k][e] * der;
+                            else { z = t[k][e] * (up * der); up = t[k][e] * act; }
+                        }
                     }
-                }
             });
-            if (!BWD) {
-                if (EPI == EPI_LINEAR && a.res)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] += t[e];
-                if (live) store_run<OT, 8>(a.out + m * a.ld_out + n * OB, a.N - n, vec, v);
-            } else {
-                // dz; zeros in the padding columns (dy is read as zero there and z is finite: W has no such rows, the bias no such elements), which are part of the contraction of dx.
-                // Column sums in f32 before the rounding.
+            for (int k = 0; k < UN; ++k) {
+                const int64_t mk = m + k * RPP;
+                const bool live = mk < a.M;
+                if (!BWD) {
+                    if (EPI == EPI_LINEAR && a.res)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) { c0[e] += live ? v[e] : 0.f; if (GATED) c1[e] += live ? u[e] : 0.f; }
-                const int64_t pad = (EPI == EPI_GATED_BWD ? a.half_out : a.ld_out) / OB - n;      // columns of the padded row from here: a multiple of 8 (16 bits) or 4
-                uint8_t *o = a.out + m * a.ld_out + n * OB;
-                if (live && pad > 0) {
-                    store_run<OT, 8>(o, pad, true, v);
-                    if (EPI == EPI_GATED_BWD) store_run<OT, 8>(o + a.half_out, pad, true, u);
+                        for (int e = 0; e < 8; ++e) v[k][e] += t[k][e];
+                    if (live) store_run<OT, 8>(a.out + mk * a.ld_out + n * OB, a.N - n, vec, v[k]);
+                } else {
+                    // dz; zeros in the padding columns (dy is read as zero there and z is finite: W has no such rows, the bias no such elements), which are part of the contraction
+                    // of dx.  Column sums in f32 before the rounding.
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) { c0[e] += live ? v[k][e] : 0.f; if (GATED) c1[e] += live ? u[k][e] : 0.f; }
+                    const int64_t pad = (EPI == EPI_GATED_BWD ? a.half_out : a.ld_out) / OB - n;      // columns of the padded row from here: a multiple of 8 (16 bits) or 4
+                    uint8_t *o = a.out + mk * a.ld_out + n * OB;
+                    if (live && pad > 0) {
+                        store_run<OT, 8>(o, pad, true, v[k]);
+                        if (EPI == EPI_GATED_BWD) store_run<OT, 8>(o + a.half_out, pad, true, u[k]);
+                    }
                 }
             }
         });

@@ -45,7 +45,7 @@ int launch_kernel(void (*kernel)(GemmArgs), int threads, int lds, const GemmArgs
 template <int LX, int LW, int EPI>
 int launch_shape(const GemmArgs &a, bool big, bool aligned, int z, hipStream_t st) {
     if constexpr (W3D_LIN_DT != W3D_DTYPE_F32) {
-        if (big) return launch_kernel(gemm_pipe_kernel<W3D_LIN_DT, LX, LW, EPI>, 512, Pipe<W3D_LIN_DT, LX, LW, EPI>::LDS_BYTES, a, z, st);
+        if (big) return launch_kernel(gemm_pipe_kernel<W3D_LIN_DT, LX, LW, EPI>, Pipe<W3D_LIN_DT, LX, LW, EPI>::NT, Pipe<W3D_LIN_DT, LX, LW, EPI>::LDS_BYTES, a, z, st);
     }
     typedef Gemm<W3D_LIN_DT, LX, LW, EPI, 128, 128, 2, 2, true> G;
     if (aligned) return launch_kernel(gemm_kernel<W3D_LIN_DT, LX, LW, EPI, 128, 128, 2, 2, true>, G::NT, G::LDS_BYTES, a, z, st);
@@ -291,6 +291,10 @@ bool aligned16(const void *p, int64_t ld) { return !(((uintptr_t)p) & 15) && ld 
 
 // How a product is cut: tile size and slices of the contraction, by the time they would take.  Microseconds per 128-byte slab of a full chip, measured: 256 x 256 tiles, one block a CU;
 // 128 x 128 tiles, two blocks a CU; a round of tiles starts and ends once (fill, epilogue).  Slices write and read their f32 tiles (4 TB/s) and take a second launch.
+#ifndef W3D_BIG
+#define W3D_BIG 256, 256, 1
+#endif
+constexpr int BIGS[3] = {W3D_BIG}, BIG_M = BIGS[0], BIG_N = BIGS[1], BIG_PER_CU = BIGS[2];
 struct Cut { bool big; int slices; int64_t tiles_m, tiles_n; };
 Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool gated, bool aligned, int batch) {
     const int parts = gated ? 2 : 1;
@@ -298,9 +302,9 @@ Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool gated, bool aligned,
     Cut best = {};
     double best_t = 0;
     for (int big = 0; big < (aligned && dtype != W3D_DTYPE_F32 ? 2 : 1); ++big) {
-        const int b = big ? 256 : 128;
-        const int64_t tm = (M + b - 1) / b, tn = (N * parts + b - 1) / b, tiles = tm * tn * batch;
-        const double slab_us = big ? (dtype == W3D_DTYPE_FP8_E4M3 ? 0.9 : 1.15) : dtype == W3D_DTYPE_F32 ? 6.0 : 1.6, round_us = big ? 6.0 : 5.0, slots = big ? 256 : 512;
+        const int bm = big ? BIG_M : 128, bn = (big ? BIG_N : 128) / parts;
+        const int64_t tm = (M + bm - 1) / bm, tn = (N + bn - 1) / bn, tiles = tm * tn * batch;
+        const double slab_us = big ? (dtype == W3D_DTYPE_FP8_E4M3 ? 0.9 : 1.15) : dtype == W3D_DTYPE_F32 ? 6.0 : 1.6, round_us = big ? 6.0 : 5.0, slots = big ? 256 * BIG_PER_CU : 512;
         for (int s = 1; s <= 32 && (s == 1 || slabs / s >= 4); ++s) {
             const double rounds = (double)((tiles * s + (int64_t)slots - 1) / (int64_t)slots);
             // (a partial round of the small tiles runs with one block a CU, in less time than two)
