@@ -3,11 +3,11 @@
 // Why this shape.  A 256 x 256 tile moves 32 KB from L2 per 64 bytes of contraction, 32 B per clock and CU at the full matrix rate; 128 x 128 tiles would need twice that, more than the
 // L2s give (they stopped at 0.66 PFLOP/s).  A wave owns 128 x 64 outputs: 128 accumulator registers, 12 KB of fragments from LDS for 512 cycles of matrix instructions.
 //
-// Schedule.  The two waves of a SIMD belong to two groups that run half a turn apart: while one group issues its 32 matrix instructions, the other reads its next fragments from LDS and
-// starts the transfers of a slab three ahead; s_barrier swaps them.  So the matrix unit always has one wave that only computes, LDS latency is never waited for by it, and a slab has three
-// turns to arrive.  Ring of four slabs of 64 bytes of contraction (4 x 32 KB).
-//   turn t of a wave:  read fragments of slab t | start slab t + 3 (into the buffer of t - 1, which both groups have read) | wait until its own part of slab t + 1 has landed | barrier |
-//                      matrix instructions of slab t | barrier
+// Schedule.  The two waves of a SIMD belong to two groups that run half a turn apart: while one group issues its 32 matrix instructions, the other reads its next fragments from LDS; s_barrier
+// swaps them.  So the matrix unit always has one wave that only computes, and LDS latency is never waited for by it.  The transfers of a slab three ahead are issued between the matrix
+// instructions (their issue takes as long as the LDS reads and would be added to them: 909 -> 813 us at 8192^3, dx).  Ring of four slabs of 64 bytes of contraction (4 x 32 KB).
+//   turn t of a wave:  read fragments of slab t | wait until its own part of slab t + 1 has landed | barrier |
+//                      matrix instructions of slab t, transfers of slab t + 3 (into the buffer of t - 1, which both groups have read) | barrier
 // The LDS reads are one asm block that ends with its own wait: as compiler-visible loads they would be made to wait for the transfers in flight (which might alias), and an output register
 // must not be free before its data arrives.
 #pragma once
@@ -27,7 +27,7 @@ struct Pipe {
     static constexpr bool GATED = O::GATED;
 
     // 16-byte chunk permutation inside an LDS row.  K_ROWS (64-byte rows): 8 neighbouring lanes read 8 rows, two of which share the banks of 128 bytes.  M_ROWS (512-byte rows of one k):
-    // the four k of a transposing read go to different 32-byte pieces.
+    // the four k of one 16-lane part of a transposing read, and those of two parts (8 k apart), go to different 32-byte pieces of 256 bytes.
     static __device__ __forceinline__ int swizzle_k(int row) { return (row >> 1) & 3; }
 
     struct Mover {                            // one side's transfers: two 16-byte pieces per lane and slab
@@ -48,7 +48,7 @@ struct Pipe {
                 m.k_of[i] = chunk * (16 / EB);
                 m.off[i] = row < rows ? (uint32_t)row * (uint32_t)ld + (uint32_t)chunk * 16u : OUT_OF_RANGE;
             } else {
-                const int row = p >> 5, chunk = (p & 31) ^ ((row & 3) << 1);
+                const int row = p >> 5, chunk = (p & 31) ^ (((row & 3) | ((row >> 3) & 1) << 2) << 1);
                 m.k_of[i] = row;
                 m.off[i] = (int64_t)chunk * 8 < rows ? (uint32_t)row * (uint32_t)ld + (uint32_t)chunk * 16u : OUT_OF_RANGE;
             }
@@ -129,7 +129,7 @@ struct Pipe {
                 else { ax[0] = lds0 + row * PIPE_SLAB + (((lane >> 5) ^ sw) << 4); ax[1] = ax[0] ^ 32u; }
             } else {
 #pragma unroll
-                for (int f = 0; f < 4; ++f) ax[f] = lds0 + (8 * q + (j >> 2)) * 512 + wm * 256 + (((f ^ (j >> 2)) & 3) << 5) + (j & 3) * 8;
+                for (int f = 0; f < 4; ++f) ax[f] = lds0 + (8 * q + (j >> 2)) * 512 + wm * 256 + ((q & 1) << 7) + (((f ^ (j >> 2)) & 3) << 5) + (j & 3) * 8;
             }
             if (LW == K_ROWS) {
                 const int row = O::w_row(wn, 0, lane), sw = swizzle_k(row);
@@ -137,7 +137,7 @@ struct Pipe {
                 else { aw[0] = lds0 + SIDE + row * PIPE_SLAB + (((lane >> 5) ^ sw) << 4); aw[1] = aw[0] ^ 32u; }
             } else {
 #pragma unroll
-                for (int f = 0; f < 4; ++f) aw[f] = lds0 + SIDE + (8 * q + (j >> 2)) * 512 + wn * 128 + (((f ^ (j >> 2)) & 3) << 5) + (j & 3) * 8;
+                for (int f = 0; f < 4; ++f) aw[f] = lds0 + SIDE + (8 * q + (j >> 2)) * 512 + (wn >> 1) * 256 + (((wn ^ q) & 1) << 7) + (((f ^ (j >> 2)) & 3) << 5) + (j & 3) * 8;
             }
         }
 
@@ -215,16 +215,16 @@ struct Pipe {
         } else {
             typedef int i32x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-            for (int g = 0; g < N / 4; ++g) {                                                  // fragments 4 g .. + 3: 128 bytes of the row further
+            for (int g = 0; g < N / 4; ++g) {                                                  // fragments 4 g .. + 3: the other 128 bytes of a 256-byte piece of the row
+                const uint32_t flip = g << 7;
                 i32x2 l[4], h[4];
                 asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\tds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
                              "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\tds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
                              "s_waitcnt lgkmcnt(0)"
                              : "=&v"(l[0]), "=&v"(h[0]), "=&v"(l[1]), "=&v"(h[1]), "=&v"(l[2]), "=&v"(h[2]), "=&v"(l[3]), "=&v"(h[3])
-                             : "v"(a[0] + at), "v"(a[1] + at), "v"(a[2] + at), "v"(a[3] + at), "n"(0), "n"(2048) : "memory");
+                             : "v"((a[0] + at) ^ flip), "v"((a[1] + at) ^ flip), "v"((a[2] + at) ^ flip), "v"((a[3] + at) ^ flip), "n"(0), "n"(2048) : "memory");
 #pragma unroll
                 for (int f = 0; f < 4; ++f) v[4 * g + f] = __builtin_shufflevector(l[f], h[f], 0, 1, 2, 3);
-                if (g + 1 < N / 4) at += 128;
             }
         }
     }

@@ -175,11 +175,11 @@ struct Stage {
     static constexpr int CPR = LAY == K_ROWS ? SLAB / 16 : ROWS * EB / 16;                     // chunks per LDS row
     static_assert(BYTES % (16 * NT) == 0, "whole pieces");
 
-    // permutation of the 16-byte chunks of an LDS row.  K_ROWS: 8 lanes read the same chunk of 8 neighbouring rows.  M_ROWS, 16 bits: four consecutive k share a transposing read of 16
-    // lanes; f32: k and k + 4 share a read's halves.
+    // permutation of the 16-byte chunks of an LDS row.  K_ROWS: 8 lanes read the same chunk of 8 neighbouring rows.  M_ROWS, 16 bits: a transposing read takes four
+    // consecutive k per 16 lanes and parts 8 k apart; f32: k and k + 4 share a read's halves.
     static __device__ __forceinline__ int swizzle(int row) {
         if (LAY == K_ROWS) return row & 7;
-        return EB == 4 ? ((row >> 2) & 1) << 2 : (row & 3) << 1;
+        return EB == 4 ? ((row >> 2) & 1) << 2 : ((row & 3) | ((row >> 3) & 1) << 2) << 1;
     }
     static __device__ __forceinline__ void place(int tid, int i, int &row, int &chunk) {      // storage row inside the slab and source chunk of piece i
         const int p = i * NT + tid;

@@ -1409,19 +1409,30 @@ def _head_act(activation) -> int:
         raise W3dError(f"unknown activation {activation!r} (None, 'relu', 'gelu', 'silu' or 'sigmoid')") from None
 
 
-def _head_check(what: str, x, width: int, dtype, **others):
-    """Shapes, types and devices of one call: others = name -> (tensor or None, shape, may it be f32 next to 16-bit rows)."""
-    if x.dim() < 1 or x.shape[-1] != width or width < 1:
-        raise W3dError(f"{what}: rows of width {width} expected, got a tensor of shape {tuple(x.shape)}")
-    for name, (t, shape, wide) in others.items():
-        if t is None:
-            continue
-        if tuple(t.shape) != tuple(shape):
-            raise W3dError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-        if t.dtype != dtype and not (wide and t.dtype == torch.float32):
-            raise W3dError(f"{what}: {name} is {t.dtype}, expected {dtype}" + (" or torch.float32" if wide else ""))
-        if t.device != x.device:
-            raise W3dError(f"{what}: {name} is on {t.device}, the rows are on {x.device}")
+_DTYPE_CODES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+
+
+def _head_rows(what: str, x):
+    """Type code of the rows; the rest of a call's tensors is checked against them (_head_arg)."""
+    if not x.is_cuda:
+        require_cuda(x)
+    code = _DTYPE_CODES.get(x.dtype)
+    if code is None:
+        raise W3dError(f"{what}: unsupported dtype {x.dtype} (float32, bfloat16 or float16)")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise W3dError(f"{what}: rows of at least one element expected, got a tensor of shape {tuple(x.shape)}")
+    return code
+
+
+def _head_arg(what: str, name: str, t, shape, dtype, device, wide: bool = False):
+    """Shape, type and device of one tensor of a call (wide: f32 is taken next to 16-bit rows) -> the contiguous tensor."""
+    if t.shape != shape:
+        raise W3dError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype != dtype and not (wide and t.dtype == torch.float32):
+        raise W3dError(f"{what}: {name} is {t.dtype}, expected {dtype}" + (" or torch.float32" if wide else ""))
+    if t.device != device:
+        raise W3dError(f"{what}: {name} is on {t.device}, the rows are on {device}")
+    return t.contiguous()
 
 
 def _head_eps(eps) -> float:
@@ -1431,9 +1442,19 @@ def _head_eps(eps) -> float:
     return eps
 
 
-def _on_device_of(t: torch.Tensor):
-    """The launches go to the current stream of the tensors' own device."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _launch(what: str, device, fn, *args):
+    """One call of the library on the current stream of the tensors' own device (tensors travel as their addresses; the stream is the last argument)."""
+    index = device.index
+    args = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
+    if index == torch.cuda.current_device():
+        clear_stale_hip_error()
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            clear_stale_hip_error()
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        check(code, what)
 
 
 def _scratch(nbytes: int, device):
@@ -1441,39 +1462,39 @@ def _scratch(nbytes: int, device):
 
 
 def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _code(t) -> int:
+    return 0 if t is None else _DTYPE_CODES[t.dtype]
 
 
 def raw_rms_norm(x, weight, residual, eps: float, y, s=None, rstd=None):
-    """y (and s = x + residual, and rstd f32 [R]) of contiguous rows x [R,d]."""
-    R, d = x.shape
-    check(lib().w3d_rms_norm_fwd(ptr(x), ptr(residual), ptr(weight), _dtype_code(weight) if weight is not None else 0, R, d, _dtype_code(x), eps, ptr(y), ptr(s), ptr(rstd), stream_ptr()),
-          "w3d_rms_norm_fwd")
+    """y (and s = x + residual, and rstd f32 [R]) of contiguous rows x [..., d]."""
+    d = x.shape[-1]
+    _launch("w3d_rms_norm_fwd", x.device, lib().w3d_rms_norm_fwd, x, residual, weight, _code(weight), x.numel() // d, d, _code(x), eps, y, s, rstd)
 
 
 def raw_rms_norm_bwd(x, residual, weight, rstd, dy, ds, dx=None, dweight=None):
-    """dx [R,d] (also the residual's gradient) and / or dweight [d] of contiguous rows."""
-    R, d = x.shape
-    ws = _scratch(lib().w3d_rms_norm_bwd_workspace_bytes(R, d) if dweight is not None else 0, x.device)
-    wdt = _dtype_code(weight) if weight is not None else 0
-    check(lib().w3d_rms_norm_bwd(ptr(x), ptr(residual), ptr(weight), wdt, ptr(rstd), ptr(dy), ptr(ds), R, d, _dtype_code(x), ptr(dx), ptr(dweight), ptr(ws), ws.numel() if ws is not None else 0,
-                                 stream_ptr()), "w3d_rms_norm_bwd")
+    """dx [..., d] (also the residual's gradient) and / or dweight [d] of contiguous rows."""
+    d = x.shape[-1]
+    R = x.numel() // d
+    nbytes = lib().w3d_rms_norm_bwd_workspace_bytes(R, d) if dweight is not None else 0
+    _launch("w3d_rms_norm_bwd", x.device, lib().w3d_rms_norm_bwd, x, residual, weight, _code(weight), rstd, dy, ds, R, d, _code(x), dx, dweight, _scratch(nbytes, x.device), nbytes)
 
 
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
-        xc = x.contiguous()
-        wc = weight.contiguous() if weight is not None else None
-        rc = residual.contiguous() if residual is not None else None
-        d = xc.shape[-1]
-        rows = xc.view(-1, d)
-        y = torch.empty_like(xc)
-        s = torch.empty_like(xc) if rc is not None else None
-        rstd = torch.empty(rows.shape[0], dtype=torch.float32, device=x.device)
-        with _on_device_of(x):
-            raw_rms_norm(rows, wc, rc, eps, y, s, rstd)
-        ctx.save_for_backward(xc, rc, wc, rstd)
+        y = torch.empty_like(x)
+        s = torch.empty_like(x) if residual is not None else None
+        rstd = torch.empty(x.numel() // x.shape[-1], dtype=torch.float32, device=x.device)
+        raw_rms_norm(x, weight, residual, eps, y, s, rstd)
+        ctx.save_for_backward(x, residual, weight, rstd)
         ctx.set_materialize_grads(False)
         return y if s is None else (y, s)
 
@@ -1482,16 +1503,13 @@ class _RmsNorm(torch.autograd.Function):
     def backward(ctx, gy, gs=None):
         x, res, w, rstd = ctx.saved_tensors
         want_x, want_w, want_r, _ = ctx.needs_input_grad
-        d = x.shape[-1]
         dw = torch.empty_like(w) if want_w else None
         if gy is None or x.numel() == 0:                           # only s was used: its gradient passes through
             dx = gs if gy is None else torch.empty_like(x)
             dw = dw.zero_() if want_w else None
         else:
             dx = torch.empty_like(x) if want_x or want_r else None
-            with _on_device_of(x):
-                clear_stale_hip_error()
-                raw_rms_norm_bwd(x.view(-1, d), res, w, rstd, gy.contiguous(), gs.contiguous() if gs is not None else None, dx, dw)
+            raw_rms_norm_bwd(x, res, w, rstd, gy.contiguous(), gs.contiguous() if gs is not None else None, dx, dw)
         return dx if want_x else None, dw, dx if want_r else None, None
 
 
@@ -1499,71 +1517,65 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-6):
     """y = s / sqrt(mean(s^2) + eps) * weight over the last dimension of s = x + residual.  x [..., d] f32 / bf16 / f16, residual like x, weight [d] of x's type or f32.
     Returns y, or (y, s) with a residual (s rounded to x's type: what the next block adds to).  The norm is taken of the unrounded sum; sums are f32.
     Differentiable in x, weight and residual."""
-    require_cuda(x, weight, residual)
-    d = x.shape[-1] if x.dim() else 0
-    _dtype_code(x)
-    _head_check("rms_norm", x, d, x.dtype, weight=(weight, (d,), True), residual=(residual, x.shape, False))
+    _head_rows("rms_norm", x)
     eps = _head_eps(eps)
-    if _wants_grad(x, weight, residual):
-        return _RmsNorm.apply(x, weight, residual, eps)
     xc = x.contiguous()
+    if weight is not None:
+        weight = _head_arg("rms_norm", "weight", weight, x.shape[-1:], x.dtype, x.device, True)
+    if residual is not None:
+        residual = _head_arg("rms_norm", "residual", residual, x.shape, x.dtype, x.device)
+    if _wants_grad(x, weight, residual):
+        return _RmsNorm.apply(xc, weight, residual, eps)
     y = torch.empty_like(xc)
     s = torch.empty_like(xc) if residual is not None else None
-    with _on_device_of(x):
-        raw_rms_norm(xc.view(-1, d), weight.contiguous() if weight is not None else None, residual.contiguous() if residual is not None else None, eps, y, s)
+    raw_rms_norm(xc, weight, residual, eps, y, s)
     return y if s is None else (y, s)
 
 
 def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-6):
     """rms_norm with its rows in 8 bits: (q uint8 [R,d] = OCP e4m3 bytes, scale int32 [R] = E8M0 exponents) as of quantize_rows_fp8, and s [R,d] behind them with a residual.
     x [R,d].  The rows are quantised from the f32 values, by quantize_rows_fp8's rule; they go straight into raw_knn_match_fp8 (d = 128, 256) or the _fp8 layers.  No gradient."""
-    require_cuda(x, weight, residual)
+    code = _head_rows("rms_norm_fp8", x)
     if x.dim() != 2:
         raise W3dError(f"rms_norm_fp8: rows [R,d] expected, got a tensor of shape {tuple(x.shape)}")
+    eps = _head_eps(eps)
     if _wants_grad(x, weight, residual):
         raise W3dError("rms_norm_fp8 has no gradient: call it under torch.no_grad() or on detached tensors")
     R, d = x.shape
-    _dtype_code(x)
-    _head_check("rms_norm_fp8", x, d, x.dtype, weight=(weight, (d,), True), residual=(residual, x.shape, False))
-    eps = _head_eps(eps)
     xc = x.contiguous()
+    if weight is not None:
+        weight = _head_arg("rms_norm_fp8", "weight", weight, x.shape[-1:], x.dtype, x.device, True)
+    if residual is not None:
+        residual = _head_arg("rms_norm_fp8", "residual", residual, x.shape, x.dtype, x.device)
     q = torch.empty(R, d, dtype=torch.uint8, device=x.device)
     scale = torch.empty(R, dtype=torch.int32, device=x.device)
     s = torch.empty_like(xc) if residual is not None else None
-    wc = weight.contiguous() if weight is not None else None
-    rc = residual.contiguous() if residual is not None else None
-    with _on_device_of(x):
-        check(lib().w3d_rms_norm_fp8(ptr(xc), ptr(rc), ptr(wc), _dtype_code(wc) if wc is not None else 0, R, d, _dtype_code(xc), eps, ptr(q), ptr(scale), ptr(s), stream_ptr()),
-              "w3d_rms_norm_fp8")
+    _launch("w3d_rms_norm_fp8", x.device, lib().w3d_rms_norm_fp8, xc, residual, weight, _code(weight), R, d, code, eps, q, scale, s)
     return (q, scale) if s is None else (q, scale, s)
 
 
 def raw_linear(x, w, bias, residual, act: int, y):
-    """y [R,N] = act(x [R,K] w [N,K]^T + bias) + residual, contiguous."""
-    (R, K), N, dt = x.shape, w.shape[0], _dtype_code(x)
-    ws = _scratch(lib().w3d_linear_workspace_bytes(R, K, N, dt, 0), x.device)
-    check(lib().w3d_linear_fwd(ptr(x), ptr(w), ptr(bias), _dtype_code(bias) if bias is not None else 0, ptr(residual), R, K, N, dt, act, ptr(y), ptr(ws),
-                               ws.numel() if ws is not None else 0, stream_ptr()), "w3d_linear_fwd")
+    """y [..., N] = act(x [..., K] w [N,K]^T + bias) + residual, contiguous."""
+    N, K = w.shape
+    R, dt = x.numel() // K, _code(x)
+    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, dt, 0)
+    _launch("w3d_linear_fwd", x.device, lib().w3d_linear_fwd, x, w, bias, _code(bias), residual, R, K, N, dt, act, y, _scratch(nbytes, x.device), nbytes)
 
 
 def raw_gated_linear(x, wg, wu, bg, bu, act: int, y):
-    """y [R,N] = act(x wg^T + bg) * (x wu^T + bu), contiguous."""
-    (R, K), N, dt = x.shape, wg.shape[0], _dtype_code(x)
-    b = bg if bg is not None else bu
-    ws = _scratch(lib().w3d_linear_workspace_bytes(R, K, N, dt, 1), x.device)
-    check(lib().w3d_gated_linear_fwd(ptr(x), ptr(wg), ptr(wu), ptr(bg), ptr(bu), _dtype_code(b) if b is not None else 0, R, K, N, dt, act, ptr(y), ptr(ws),
-                                     ws.numel() if ws is not None else 0, stream_ptr()), "w3d_gated_linear_fwd")
+    """y [..., N] = act(x wg^T + bg) * (x wu^T + bu), contiguous."""
+    N, K = wg.shape
+    R, dt = x.numel() // K, _code(x)
+    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, dt, 1)
+    _launch("w3d_gated_linear_fwd", x.device, lib().w3d_gated_linear_fwd, x, wg, wu, bg, bu, _code(bg if bg is not None else bu), R, K, N, dt, act, y, _scratch(nbytes, x.device), nbytes)
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, residual, act):
-        xc, wc = x.contiguous(), w.contiguous()
-        bc = bias.contiguous() if bias is not None else None
-        y = torch.empty(*x.shape[:-1], w.shape[0], dtype=x.dtype, device=x.device)
-        with _on_device_of(x):
-            raw_linear(xc.view(-1, xc.shape[-1]), wc, bc, residual.contiguous() if residual is not None else None, act, y)
-        ctx.save_for_backward(xc, wc, bc)
+        y = x.new_empty(x.shape[:-1] + w.shape[:1])
+        raw_linear(x, w, bias, residual, act, y)
+        ctx.save_for_backward(x, w, bias)
         ctx.act = act
         return y
 
@@ -1572,8 +1584,7 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, gy):
         x, w, bias = ctx.saved_tensors
         want_x, want_w, want_b, want_r, _ = ctx.needs_input_grad
-        gyc = gy.contiguous()
-        K, N = x.shape[-1], w.shape[0]
+        N, K = w.shape
         dx = torch.empty_like(x) if want_x else None
         dw = torch.empty_like(w) if want_w else None
         db = torch.empty_like(bias) if want_b else None
@@ -1581,42 +1592,43 @@ class _Linear(torch.autograd.Function):
         if R == 0:
             dw, db = (t.zero_() if t is not None else None for t in (dw, db))
         elif want_x or want_w or want_b:
-            dt = _dtype_code(x)
-            with _on_device_of(x):
-                clear_stale_hip_error()
-                ws = _scratch(lib().w3d_linear_bwd_workspace_bytes(R, K, N, dt, ctx.act, 0), x.device)
-                check(lib().w3d_linear_bwd(ptr(x), ptr(w), ptr(bias), _dtype_code(bias) if bias is not None else 0, ptr(gyc), R, K, N, dt, ctx.act, ptr(dx), ptr(dw), ptr(db), ptr(ws),
-                                           ws.numel() if ws is not None else 0, stream_ptr()), "w3d_linear_bwd")
+            dt = _code(x)
+            nbytes = lib().w3d_linear_bwd_workspace_bytes(R, K, N, dt, ctx.act, 0)
+            _launch("w3d_linear_bwd", x.device, lib().w3d_linear_bwd, x, w, bias, _code(bias), gy.contiguous(), R, K, N, dt, ctx.act, dx, dw, db, _scratch(nbytes, x.device), nbytes)
         return dx, dw, db, gy if want_r else None, None
+
+
+def _head_weight(what: str, name: str, w):
+    if w.dim() != 2 or w.shape[0] < 1:
+        raise W3dError(f"{what}: {name} [N,K] expected, got shape {tuple(w.shape)}")
+    return w.shape
 
 
 def linear(x, weight, bias=None, activation=None, residual=None):
     """y = act(x weight^T + bias) + residual in one launch.  x [..., K] f32 / bf16 / f16, weight [N,K] and residual [..., N] of x's type, bias [N] of x's type or f32;
     activation None, 'relu', 'gelu' (z Phi(z)), 'silu' or 'sigmoid'.  Sums in f32, one rounding at the end.  Differentiable in everything; nothing but the inputs is kept for it."""
-    require_cuda(x, weight, bias, residual)
-    _dtype_code(x)
+    _head_rows("linear", x)
     act = _head_act(activation)
-    if weight.dim() != 2 or weight.shape[0] < 1:
-        raise W3dError(f"linear: weight [N,K] expected, got shape {tuple(weight.shape)}")
-    N, K = weight.shape
-    _head_check("linear", x, K, x.dtype, weight=(weight, (N, K), False), bias=(bias, (N,), True), residual=(residual, (*x.shape[:-1], N), False))
+    N, _ = _head_weight("linear", "weight", weight)
+    weight = _head_arg("linear", "weight", weight, (N, x.shape[-1]), x.dtype, x.device)
+    if bias is not None:
+        bias = _head_arg("linear", "bias", bias, (N,), x.dtype, x.device, True)
+    if residual is not None:
+        residual = _head_arg("linear", "residual", residual, (*x.shape[:-1], N), x.dtype, x.device)
+    xc = x.contiguous()
     if _wants_grad(x, weight, bias, residual):
-        return _Linear.apply(x, weight, bias, residual, act)
-    y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
-    with _on_device_of(x):
-        raw_linear(x.contiguous().view(-1, K), weight.contiguous(), bias.contiguous() if bias is not None else None, residual.contiguous() if residual is not None else None, act, y)
+        return _Linear.apply(xc, weight, bias, residual, act)
+    y = xc.new_empty((*x.shape[:-1], N))
+    raw_linear(xc, weight, bias, residual, act, y)
     return y
 
 
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wg, wu, bg, bu, act):
-        xc, wgc, wuc = x.contiguous(), wg.contiguous(), wu.contiguous()
-        bgc, buc = (b.contiguous() if b is not None else None for b in (bg, bu))
-        y = torch.empty(*x.shape[:-1], wg.shape[0], dtype=x.dtype, device=x.device)
-        with _on_device_of(x):
-            raw_gated_linear(xc.view(-1, xc.shape[-1]), wgc, wuc, bgc, buc, act, y)
-        ctx.save_for_backward(xc, wgc, wuc, bgc, buc)
+        y = x.new_empty(x.shape[:-1] + wg.shape[:1])
+        raw_gated_linear(x, wg, wu, bg, bu, act, y)
+        ctx.save_for_backward(x, wg, wu, bg, bu)
         ctx.act = act
         return y
 
@@ -1624,52 +1636,49 @@ class _GatedLinear(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
         x, wg, wu, bg, bu = ctx.saved_tensors
-        want = ctx.needs_input_grad
-        K, N = x.shape[-1], wg.shape[0]
-        grads = [torch.empty_like(t) if need else None for t, need in zip((x, wg, wu, bg, bu), want)]
+        N, K = wg.shape
+        grads = [torch.empty_like(t) if need else None for t, need in zip((x, wg, wu, bg, bu), ctx.needs_input_grad)]
         R = x.numel() // K
         if R == 0:
             grads = [t.zero_() if t is not None else None for t in grads]
         else:
-            gyc, dt, b = gy.contiguous(), _dtype_code(x), bg if bg is not None else bu
-            with _on_device_of(x):
-                clear_stale_hip_error()
-                ws = _scratch(lib().w3d_linear_bwd_workspace_bytes(R, K, N, dt, ctx.act, 1), x.device)
-                check(lib().w3d_gated_linear_bwd(ptr(x), ptr(wg), ptr(wu), ptr(bg), ptr(bu), _dtype_code(b) if b is not None else 0, ptr(gyc), R, K, N, dt, ctx.act,
-                                                 *(ptr(t) for t in grads), ptr(ws), ws.numel() if ws is not None else 0, stream_ptr()), "w3d_gated_linear_bwd")
+            dt = _code(x)
+            nbytes = lib().w3d_linear_bwd_workspace_bytes(R, K, N, dt, ctx.act, 1)
+            _launch("w3d_gated_linear_bwd", x.device, lib().w3d_gated_linear_bwd, x, wg, wu, bg, bu, _code(bg if bg is not None else bu), gy.contiguous(), R, K, N, dt, ctx.act, *grads,
+                    _scratch(nbytes, x.device), nbytes)
         return (*grads, None)
 
 
-def _gated_check(what, x, wg, wu, bg, bu, dtype, bias_dtype):
-    if wg.dim() != 2 or wg.shape[0] < 1:
-        raise W3dError(f"{what}: w_gate [N,K] expected, got shape {tuple(wg.shape)}")
-    N, K = wg.shape
-    _head_check(what, x, K, dtype, w_gate=(wg, (N, K), False), w_up=(wu, (N, K), False))
-    _head_check(what, x, K, bias_dtype, b_gate=(bg, (N,), True), b_up=(bu, (N,), True))
+def _gated_args(what, x, wg, wu, bg, bu, dtype, bias_dtype):
+    N, _ = _head_weight(what, "w_gate", wg)
+    wg, wu = (_head_arg(what, name, w, (N, x.shape[-1]), dtype, x.device) for name, w in (("w_gate", wg), ("w_up", wu)))
+    bg, bu = (_head_arg(what, name, b, (N,), bias_dtype, x.device, True) if b is not None else None for name, b in (("b_gate", bg), ("b_up", bu)))
     if bg is not None and bu is not None and bg.dtype != bu.dtype:
         raise W3dError(f"{what}: b_gate is {bg.dtype}, b_up is {bu.dtype}")
-    return N, K
+    return N, wg, wu, bg, bu
 
 
 def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     """y = act(x w_gate^T + b_gate) * (x w_up^T + b_up): both products, the activation and the product in one launch.  x [..., K] f32 / bf16 / f16, weights [N,K] of x's type, biases
     [N] of x's type or f32 (both alike); activation as in linear.  Sums in f32, one rounding at the end.  Differentiable in everything; nothing but the inputs is kept for it."""
-    require_cuda(x, w_gate, w_up, b_gate, b_up)
-    _dtype_code(x)
+    _head_rows("gated_linear", x)
     act = _head_act(activation)
-    N, K = _gated_check("gated_linear", x, w_gate, w_up, b_gate, b_up, x.dtype, x.dtype)
+    N, w_gate, w_up, b_gate, b_up = _gated_args("gated_linear", x, w_gate, w_up, b_gate, b_up, x.dtype, x.dtype)
+    xc = x.contiguous()
     if _wants_grad(x, w_gate, w_up, b_gate, b_up):
-        return _GatedLinear.apply(x, w_gate, w_up, b_gate, b_up, act)
-    y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
-    with _on_device_of(x):
-        raw_gated_linear(x.contiguous().view(-1, K), w_gate.contiguous(), w_up.contiguous(), *(b.contiguous() if b is not None else None for b in (b_gate, b_up)), act, y)
+        return _GatedLinear.apply(xc, w_gate, w_up, b_gate, b_up, act)
+    y = xc.new_empty((*x.shape[:-1], N))
+    raw_gated_linear(xc, w_gate, w_up, b_gate, b_up, act, y)
     return y
 
 
 def _fp8_rows(what, name, q, scale, device):
-    if q.dtype != torch.uint8 or q.dim() != 2 or scale.dtype != torch.int32 or tuple(scale.shape) != (q.shape[0],) or q.device != device or scale.device != device:
+    if not q.is_cuda:
+        require_cuda(q)
+    if q.dtype != torch.uint8 or q.dim() != 2 or q.shape[1] < 1 or scale.dtype != torch.int32 or scale.shape != q.shape[:1] or q.device != device or scale.device != device:
         raise W3dError(f"{what}: {name} expected as e4m3 bytes uint8 [rows,K] + E8M0 exponents int32 [rows] on {device}, got {q.dtype} {tuple(q.shape)} on {q.device} and "
                        f"{scale.dtype} {tuple(scale.shape)} on {scale.device}")
+    return q.contiguous(), scale.contiguous()
 
 
 def _fp8_out(what, out_dtype, *tensors):
@@ -1677,45 +1686,40 @@ def _fp8_out(what, out_dtype, *tensors):
         raise W3dError(f"{what}: out_dtype {out_dtype} (torch.bfloat16 or torch.float16)")
     if _wants_grad(*tensors):
         raise W3dError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+    return _DTYPE_CODES[out_dtype]
 
 
 def linear_fp8(q, scale, weight_q, weight_scale, bias=None, activation=None, residual=None, out_dtype=torch.bfloat16):
     """linear on 8-bit rows: q [R,K], weight_q [N,K] e4m3 bytes with one E8M0 exponent a row (quantize_rows_fp8, rms_norm_fp8), products on the fp8 matrix cores, the exponents applied to
     the f32 sums.  y [R,N] of out_dtype (bf16 / f16), residual [R,N] of out_dtype, bias [N] of out_dtype or f32.  No gradient."""
-    require_cuda(q, scale, weight_q, weight_scale, bias, residual)
-    act = _head_act(activation)
-    for name, a, b in (("q, scale", q, scale), ("weight_q, weight_scale", weight_q, weight_scale)):
-        _fp8_rows("linear_fp8", name, a, b, q.device)
-    _fp8_out("linear_fp8", out_dtype, bias, residual)
+    act, dev = _head_act(activation), q.device
+    q, scale = _fp8_rows("linear_fp8", "q, scale", q, scale, dev)
+    weight_q, weight_scale = _fp8_rows("linear_fp8", "weight_q, weight_scale", weight_q, weight_scale, dev)
+    code = _fp8_out("linear_fp8", out_dtype, bias, residual)
     (R, K), N = q.shape, weight_q.shape[0]
-    if weight_q.shape[1] != K or K < 1 or N < 1:
+    if weight_q.shape[1] != K or N < 1:
         raise W3dError(f"linear_fp8: rows {tuple(q.shape)} against weights {tuple(weight_q.shape)}")
-    _head_check("linear_fp8", q, K, out_dtype, bias=(bias, (N,), True), residual=(residual, (R, N), False))
-    y = torch.empty(R, N, dtype=out_dtype, device=q.device)
-    qc, sc, wc, wsc = (t.contiguous() for t in (q, scale, weight_q, weight_scale))
-    bc, rc = (t.contiguous() if t is not None else None for t in (bias, residual))
-    with _on_device_of(q):
-        ws = _scratch(lib().w3d_linear_workspace_bytes(R, K, N, FP8, 0), q.device)
-        check(lib().w3d_linear_fp8_fwd(ptr(qc), ptr(sc), ptr(wc), ptr(wsc), ptr(bc), _dtype_code(bc) if bc is not None else 0, ptr(rc), R, K, N, _dtype_code(y), act, ptr(y), ptr(ws),
-                                       ws.numel() if ws is not None else 0, stream_ptr()), "w3d_linear_fp8_fwd")
+    if bias is not None:
+        bias = _head_arg("linear_fp8", "bias", bias, (N,), out_dtype, dev, True)
+    if residual is not None:
+        residual = _head_arg("linear_fp8", "residual", residual, (R, N), out_dtype, dev)
+    y = torch.empty(R, N, dtype=out_dtype, device=dev)
+    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, FP8, 0)
+    _launch("w3d_linear_fp8_fwd", dev, lib().w3d_linear_fp8_fwd, q, scale, weight_q, weight_scale, bias, _code(bias), residual, R, K, N, code, act, y, _scratch(nbytes, dev), nbytes)
     return y
 
 
 def gated_linear_fp8(q, scale, gate_q, gate_scale, up_q, up_scale, b_gate=None, b_up=None, activation="silu", out_dtype=torch.bfloat16):
     """gated_linear on 8-bit rows and weights (see linear_fp8).  y [R,N] of out_dtype.  No gradient."""
-    require_cuda(q, scale, gate_q, gate_scale, up_q, up_scale, b_gate, b_up)
-    act = _head_act(activation)
-    for name, a, b in (("q, scale", q, scale), ("gate_q, gate_scale", gate_q, gate_scale), ("up_q, up_scale", up_q, up_scale)):
-        _fp8_rows("gated_linear_fp8", name, a, b, q.device)
-    _fp8_out("gated_linear_fp8", out_dtype, b_gate, b_up)
-    N, K = _gated_check("gated_linear_fp8", q, gate_q, up_q, b_gate, b_up, torch.uint8, out_dtype)
-    R = q.shape[0]
-    y = torch.empty(R, N, dtype=out_dtype, device=q.device)
-    qc, sc, gc, gsc, uc, usc = (t.contiguous() for t in (q, scale, gate_q, gate_scale, up_q, up_scale))
-    bgc, buc = (t.contiguous() if t is not None else None for t in (b_gate, b_up))
-    b = bgc if bgc is not None else buc
-    with _on_device_of(q):
-        ws = _scratch(lib().w3d_linear_workspace_bytes(R, K, N, FP8, 1), q.device)
-        check(lib().w3d_gated_linear_fp8_fwd(ptr(qc), ptr(sc), ptr(gc), ptr(gsc), ptr(uc), ptr(usc), ptr(bgc), ptr(buc), _dtype_code(b) if b is not None else 0, R, K, N,
-                                             _dtype_code(y), act, ptr(y), ptr(ws), ws.numel() if ws is not None else 0, stream_ptr()), "w3d_gated_linear_fp8_fwd")
+    act, dev = _head_act(activation), q.device
+    q, scale = _fp8_rows("gated_linear_fp8", "q, scale", q, scale, dev)
+    gate_q, gate_scale = _fp8_rows("gated_linear_fp8", "gate_q, gate_scale", gate_q, gate_scale, dev)
+    up_q, up_scale = _fp8_rows("gated_linear_fp8", "up_q, up_scale", up_q, up_scale, dev)
+    code = _fp8_out("gated_linear_fp8", out_dtype, b_gate, b_up)
+    N, gate_q, up_q, b_gate, b_up = _gated_args("gated_linear_fp8", q, gate_q, up_q, b_gate, b_up, torch.uint8, out_dtype)
+    R, K = q.shape
+    y = torch.empty(R, N, dtype=out_dtype, device=dev)
+    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, FP8, 1)
+    _launch("w3d_gated_linear_fp8_fwd", dev, lib().w3d_gated_linear_fp8_fwd, q, scale, gate_q, gate_scale, up_q, up_scale, b_gate, b_up, _code(b_gate if b_gate is not None else b_up), R, K, N,
+            code, act, y, _scratch(nbytes, dev), nbytes)
     return y
