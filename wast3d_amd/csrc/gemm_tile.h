@@ -179,7 +179,8 @@ struct Stage {
     // consecutive k per 16 lanes and parts 8 k apart; f32: k and k + 4 share a read's halves.
     static __device__ __forceinline__ int swizzle(int row) {
         if (LAY == K_ROWS) return row & 7;
-        return EB == 4 ? ((row >> 2) & 1) << 2 : ((row & 3) | ((row >> 3) & 1) << 2) << 1;
+        if (EB == 4) return ((row >> 2) & 1) << 2;
+        return ((row & 3) | (CPR >= 16 ? ((row >> 3) & 1) << 2 : 0)) << 1;                      // (rows of 64 elements are 8 chunks)
     }
     static __device__ __forceinline__ void place(int tid, int i, int &row, int &chunk) {      // storage row inside the slab and source chunk of piece i
         const int p = i * NT + tid;
@@ -218,9 +219,11 @@ struct Out {
     static constexpr int PARTS = GATED ? 2 : 1, BNP = BN / PARTS;                              // a gated tile is BN / 2 columns of each half: rows [0, BN/2) of the W slab gate, the rest up
     static constexpr int FM = BM / WM / MS, FN = BN / WN / MS, FP = FN / PARTS;
     static constexpr int COLS = BN / WN, PCOLS = COLS / PARTS, LPR = PCOLS / 8, RPP = 64 / LPR;      // lanes per row, rows per pass
-    static constexpr int ROWS = 64, CHUNKS = BM / WM / ROWS, PASSES = ROWS / RPP, AHEAD = 4, UN = EPI == EPI_GATED_BWD ? 1 : 2;      // UN passes at a time: their LDS reads, arithmetic and stores overlap
+    static constexpr int ROWS = BM / WM < 64 ? BM / WM : 64, CHUNKS = BM / WM / ROWS, PASSES = ROWS / RPP;
+    static constexpr int UN = EPI == EPI_GATED_BWD || PASSES < 2 ? 1 : 2;                      // UN passes at a time: their LDS reads, arithmetic and stores overlap
+    static constexpr int AHEAD = PASSES < 4 ? PASSES : 4;
     static constexpr int PATCH = ROWS * COLS * 4;
-    static_assert(COLS == 64 && BM / WM % ROWS == 0 && AHEAD <= PASSES && PASSES % UN == 0, "a patch row is 16 chunks; whole chunks of rows");
+    static_assert(COLS == 64 && BM / WM % ROWS == 0 && PASSES % UN == 0, "a patch row is 16 chunks; whole chunks of rows");
     typedef typename std::conditional<MS == 32, f32x16, f32x4>::type acc_t;
     typedef acc_t Acc[FM][FN];
 

@@ -2,7 +2,7 @@
 //
 // Three kernels do the products (gemm_tile.h has the tile):
 //   * few rows (<= SKINNY_ROWS): the weights are read once, straight into MFMA fragments, by as many waves as there are; the rows are the other operand
-//   * tiles of 256 x 256 (gemm_pipe.h) or 128 x 128 (gemm_tile.h) through LDS
+//   * tiles of 256 x 256 (gemm_pipe.h), 128 x 128 or 64 x 64 (gemm_tile.h) through LDS
 //   * when the tiles are few for 256 CUs the contraction is cut into slices; partial tiles are added in slice order, and the epilogue applied, by a second launch
 //
 // Backward keeps nothing of the forward pass but its inputs: z is formed again and turned into dz in the epilogue, where the column sums for the bias
@@ -22,10 +22,10 @@ constexpr int SKINNY_ROWS = 64;
 }  // namespace
 
 // launches of one operand type's kernels
-int w3d_lin_tiles_f32(const GemmArgs &a, int prod, bool big, bool aligned, int z, hipStream_t st);
-int w3d_lin_tiles_bf16(const GemmArgs &a, int prod, bool big, bool aligned, int z, hipStream_t st);
-int w3d_lin_tiles_f16(const GemmArgs &a, int prod, bool big, bool aligned, int z, hipStream_t st);
-int w3d_lin_tiles_fp8(const GemmArgs &a, int prod, bool big, bool aligned, int z, hipStream_t st);
+int w3d_lin_tiles_f32(const GemmArgs &a, int prod, int tile, bool aligned, int z, hipStream_t st);
+int w3d_lin_tiles_bf16(const GemmArgs &a, int prod, int tile, bool aligned, int z, hipStream_t st);
+int w3d_lin_tiles_f16(const GemmArgs &a, int prod, int tile, bool aligned, int z, hipStream_t st);
+int w3d_lin_tiles_fp8(const GemmArgs &a, int prod, int tile, bool aligned, int z, hipStream_t st);
 int w3d_lin_skinny_f32(const GemmArgs &a, int prod, hipStream_t st);
 int w3d_lin_skinny_bf16(const GemmArgs &a, int prod, hipStream_t st);
 int w3d_lin_skinny_f16(const GemmArgs &a, int prod, hipStream_t st);
@@ -42,27 +42,33 @@ int launch_kernel(void (*kernel)(GemmArgs), int threads, int lds, const GemmArgs
     W3D_CHECK_LAUNCH();
     return W3D_OK;
 }
-template <int LX, int LW, int EPI>
-int launch_shape(const GemmArgs &a, bool big, bool aligned, int z, hipStream_t st) {
-    if constexpr (W3D_LIN_DT != W3D_DTYPE_F32) {
-        if (big) return launch_kernel(gemm_pipe_kernel<W3D_LIN_DT, LX, LW, EPI>, Pipe<W3D_LIN_DT, LX, LW, EPI>::NT, Pipe<W3D_LIN_DT, LX, LW, EPI>::LDS_BYTES, a, z, st);
-    }
-    typedef Gemm<W3D_LIN_DT, LX, LW, EPI, 128, 128, 2, 2, true> G;
-    if (aligned) return launch_kernel(gemm_kernel<W3D_LIN_DT, LX, LW, EPI, 128, 128, 2, 2, true>, G::NT, G::LDS_BYTES, a, z, st);
-    return launch_kernel(gemm_kernel<W3D_LIN_DT, LX, LW, EPI, 128, 128, 2, 2, false>, G::NT, G::LDS_BYTES, a, z, st);
+template <int LX, int LW, int EPI, int BM, int BN, int WM, int WN, bool ALIGNED>
+int launch_tile(const GemmArgs &a, int z, hipStream_t st) {
+    typedef Gemm<W3D_LIN_DT, LX, LW, EPI, BM, BN, WM, WN, ALIGNED> G;
+    return launch_kernel(gemm_kernel<W3D_LIN_DT, LX, LW, EPI, BM, BN, WM, WN, ALIGNED>, G::NT, G::LDS_BYTES, a, z, st);
 }
-int launch_prod(const GemmArgs &a, int prod, bool big, bool aligned, int z, hipStream_t st) {
+template <int LX, int LW, int EPI>
+int launch_shape(const GemmArgs &a, int tile, bool aligned, int z, hipStream_t st) {
+    if constexpr (W3D_LIN_DT != W3D_DTYPE_F32) {
+        if (tile == 256) return launch_kernel(gemm_pipe_kernel<W3D_LIN_DT, LX, LW, EPI>, Pipe<W3D_LIN_DT, LX, LW, EPI>::NT, Pipe<W3D_LIN_DT, LX, LW, EPI>::LDS_BYTES, a, z, st);
+    }
+    if (tile == 128 && aligned) return launch_tile<LX, LW, EPI, 128, 128, 2, 2, true>(a, z, st);
+    if (tile == 128) return launch_tile<LX, LW, EPI, 128, 128, 2, 2, false>(a, z, st);
+    if (aligned) return launch_tile<LX, LW, EPI, 64, 64, 4, 1, true>(a, z, st);
+    return launch_tile<LX, LW, EPI, 64, 64, 4, 1, false>(a, z, st);
+}
+int launch_prod(const GemmArgs &a, int prod, int tile, bool aligned, int z, hipStream_t st) {
     switch (prod) {
-        case PROD_LINEAR: return launch_shape<K_ROWS, K_ROWS, EPI_LINEAR>(a, big, aligned, z, st);
-        case PROD_GATED: return launch_shape<K_ROWS, K_ROWS, EPI_GATED>(a, big, aligned, z, st);
+        case PROD_LINEAR: return launch_shape<K_ROWS, K_ROWS, EPI_LINEAR>(a, tile, aligned, z, st);
+        case PROD_GATED: return launch_shape<K_ROWS, K_ROWS, EPI_GATED>(a, tile, aligned, z, st);
         default: break;
     }
     if constexpr (W3D_LIN_DT != W3D_DTYPE_FP8_E4M3) {
         switch (prod) {
-            case PROD_LINEAR_BWD: return launch_shape<K_ROWS, K_ROWS, EPI_LINEAR_BWD>(a, big, aligned, z, st);
-            case PROD_GATED_BWD: return launch_shape<K_ROWS, K_ROWS, EPI_GATED_BWD>(a, big, aligned, z, st);
-            case PROD_DX: return launch_shape<K_ROWS, M_ROWS, EPI_STORE>(a, big, aligned, z, st);
-            case PROD_DW: return launch_shape<M_ROWS, M_ROWS, EPI_STORE>(a, big, aligned, z, st);
+            case PROD_LINEAR_BWD: return launch_shape<K_ROWS, K_ROWS, EPI_LINEAR_BWD>(a, tile, aligned, z, st);
+            case PROD_GATED_BWD: return launch_shape<K_ROWS, K_ROWS, EPI_GATED_BWD>(a, tile, aligned, z, st);
+            case PROD_DX: return launch_shape<K_ROWS, M_ROWS, EPI_STORE>(a, tile, aligned, z, st);
+            case PROD_DW: return launch_shape<M_ROWS, M_ROWS, EPI_STORE>(a, tile, aligned, z, st);
             default: break;
         }
     }
@@ -195,7 +201,7 @@ int launch_skinny(const GemmArgs &a, hipStream_t st) {
 #else
 #define W3D_LIN_NAME(f) f##_fp8
 #endif
-int W3D_LIN_NAME(w3d_lin_tiles)(const GemmArgs &a, int prod, bool big, bool aligned, int z, hipStream_t st) { return launch_prod(a, prod, big, aligned, z, st); }
+int W3D_LIN_NAME(w3d_lin_tiles)(const GemmArgs &a, int prod, int tile, bool aligned, int z, hipStream_t st) { return launch_prod(a, prod, tile, aligned, z, st); }
 int W3D_LIN_NAME(w3d_lin_skinny)(const GemmArgs &a, int prod, hipStream_t st) {
     return prod == PROD_GATED ? launch_skinny<EPI_GATED>(a, st) : launch_skinny<EPI_LINEAR>(a, st);
 }
@@ -289,29 +295,39 @@ bool float_dtype(int t) { return t == W3D_DTYPE_F32 || t == W3D_DTYPE_BF16 || t 
 int64_t ceil_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 bool aligned16(const void *p, int64_t ld) { return !(((uintptr_t)p) & 15) && ld % 16 == 0; }
 
-// How a product is cut: tile size and slices of the contraction, by the time they would take.  Microseconds per 128-byte slab of a full chip, measured: 256 x 256 tiles, one block a CU;
-// 128 x 128 tiles, two blocks a CU; a round of tiles starts and ends once (fill, epilogue).  Slices write and read their f32 tiles (4 TB/s) and take a second launch.
-#ifndef W3D_BIG
-#define W3D_BIG 256, 256, 1
+// How a product is cut: tile size and slices of the contraction, by the time they would take.  Microseconds, fitted to every tile with 1, 2 and 4 slices on 12 sizes of rows 100 .. 65 536 and
+// widths 100 .. 4 096: `lone`, a 128-byte slab of a block that has its CU for itself; `busy`, the same of a block among others, per block on the CU; `round`, start and epilogue of a block.
+// Slices write and read their f32 tiles (2.5 TB/s with the second launch's start).
+struct TileCost { double lone[3], busy[3], round[3]; };      // of 64, 128, 256
+constexpr TileCost COST_16 = {{0.35, 0.6, 1.2}, {0.22, 0.6, 1.3}, {4, 5, 10}}, COST_FP8 = {{0.35, 0.6, 0.9}, {0.22, 0.6, 0.9}, {4, 5, 10}},
+                   COST_UNALIGNED = {{2.0, 3.5, 0}, {0.5, 1.2, 0}, {4, 5, 0}}, COST_F32 = {{0.72, 2.25, 0}, {0.62, 2.25, 0}, {4, 5, 0}};
+#ifndef W3D_FORCE_TILE
+#define W3D_FORCE_TILE 0
 #endif
-constexpr int BIGS[3] = {W3D_BIG}, BIG_M = BIGS[0], BIG_N = BIGS[1], BIG_PER_CU = BIGS[2];
-struct Cut { bool big; int slices; int64_t tiles_m, tiles_n; };
+#ifndef W3D_FORCE_SLICES
+#define W3D_FORCE_SLICES 0
+#endif
+struct Cut { int tile, slices; int64_t tiles_m, tiles_n; };
 Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool gated, bool aligned, int batch) {
     const int parts = gated ? 2 : 1;
     const int64_t slabs = (K * eb_of(dtype) + SLAB - 1) / SLAB;
     Cut best = {};
     double best_t = 0;
-    for (int big = 0; big < (aligned && dtype != W3D_DTYPE_F32 ? 2 : 1); ++big) {
-        const int bm = big ? BIG_M : 128, bn = (big ? BIG_N : 128) / parts;
-        const int64_t tm = (M + bm - 1) / bm, tn = (N + bn - 1) / bn, tiles = tm * tn * batch;
-        const double slab_us = big ? (dtype == W3D_DTYPE_FP8_E4M3 ? 0.9 : 1.15) : dtype == W3D_DTYPE_F32 ? 6.0 : 1.6, round_us = big ? 6.0 : 5.0, slots = big ? 256 * BIG_PER_CU : 512;
+    for (int tile = 64; tile <= 256; tile *= 2) {
+        if (tile == 256 && (!aligned || dtype == W3D_DTYPE_F32)) break;
+        if (W3D_FORCE_TILE && tile != W3D_FORCE_TILE) continue;
+        const int bn = tile / parts;
+        const int64_t tm = (M + tile - 1) / tile, tn = (N + bn - 1) / bn, tiles = tm * tn * batch;
+        const int k = tile == 64 ? 0 : tile == 128 ? 1 : 2;
+        const TileCost &c = dtype == W3D_DTYPE_F32 ? COST_F32 : !aligned ? COST_UNALIGNED : dtype == W3D_DTYPE_FP8_E4M3 ? COST_FP8 : COST_16;
+        const int per_cu = tile == 256 ? 1 : tile == 128 ? 2 : 4;
         for (int s = 1; s <= 32 && (s == 1 || slabs / s >= 4); ++s) {
-            const double rounds = (double)((tiles * s + (int64_t)slots - 1) / (int64_t)slots);
-            // (a partial round of the small tiles runs with one block a CU, in less time than two)
-            const double fill = !big && tiles * s <= 256 ? 0.6 : 1.0;
-            double t = rounds * (fill * slab_us * (double)((slabs + s - 1) / s) + round_us);
-            if (s > 1) t += 4.0 + 8.0 * (double)s * (double)batch * (double)M * (double)N * parts / 4e6;
-            if (best_t == 0 || t < best_t) { best_t = t; best = {big != 0, s, tm, tn}; }
+            if (W3D_FORCE_SLICES && s != W3D_FORCE_SLICES) continue;
+            const double cu = (double)((tiles * s + 255) / 256), rounds = (double)((tiles * s + 256 * per_cu - 1) / (256 * per_cu)), n = (double)((slabs + s - 1) / s);
+            const double a = n * c.busy[k] * cu, b = n * c.lone[k] * rounds;
+            double t = (a > b ? a : b) + c.round[k] * rounds;
+            if (s > 1) t += 5.0 + 8.0 * (double)s * (double)batch * (double)M * (double)N * parts / 2.5e6;
+            if (best_t == 0 || t < best_t) { best_t = t; best = {tile, s, tm, tn}; }
         }
     }
     return best;
@@ -327,10 +343,10 @@ int run_product(GemmArgs &a, int prod, int dtype, const Cut &c, bool aligned, in
     a.part_ld = ceil_to(a.N, 16) * (prod == PROD_GATED || prod == PROD_GATED_BWD ? 2 : 1);
     int rc;
     switch (dtype) {
-        case W3D_DTYPE_F32: rc = w3d_lin_tiles_f32(a, prod, c.big, aligned, z, st); break;
-        case W3D_DTYPE_BF16: rc = w3d_lin_tiles_bf16(a, prod, c.big, aligned, z, st); break;
-        case W3D_DTYPE_F16: rc = w3d_lin_tiles_f16(a, prod, c.big, aligned, z, st); break;
-        default: rc = w3d_lin_tiles_fp8(a, prod, c.big, aligned, z, st); break;
+        case W3D_DTYPE_F32: rc = w3d_lin_tiles_f32(a, prod, c.tile, aligned, z, st); break;
+        case W3D_DTYPE_BF16: rc = w3d_lin_tiles_bf16(a, prod, c.tile, aligned, z, st); break;
+        case W3D_DTYPE_F16: rc = w3d_lin_tiles_f16(a, prod, c.tile, aligned, z, st); break;
+        default: rc = w3d_lin_tiles_fp8(a, prod, c.tile, aligned, z, st); break;
     }
     if (rc != W3D_OK || c.slices == 1) return rc;
     switch (a.out_dt) {
@@ -387,8 +403,8 @@ struct Bwd {
     int64_t dz_bytes, strips, colsum_ld, colsum_bytes, part;
 };
 int64_t max64(int64_t a, int64_t b) { return a > b ? a : b; }
-// strips of partial column sums that the product forming dz writes: two per tile row, or the joining launch's
-int64_t strips_of(const Cut &c, int64_t R) { return c.slices > 1 ? (R + JOIN_ROWS - 1) / JOIN_ROWS : c.tiles_m * 2; }
+// strips of partial column sums that the product forming dz writes: one per tile row and row of waves, or the joining launch's
+int64_t strips_of(const Cut &c, int64_t R) { return c.slices > 1 ? (R + JOIN_ROWS - 1) / JOIN_ROWS : c.tiles_m * (c.tile == 64 ? 4 : 2); }
 Bwd bwd_plan(int64_t R, int64_t K, int64_t N, int dtype, bool gated, bool no_act) {
     Bwd b;
     const int eb = eb_of(dtype), parts = gated ? 2 : 1;
@@ -399,7 +415,7 @@ Bwd bwd_plan(int64_t R, int64_t K, int64_t N, int dtype, bool gated, bool no_act
     b.part = 0;
     b.strips = no_act ? w3d_column_strips(R, N) : 0;
     for (int al = 0; al < 2; ++al) {
-        const Cut z = cut_of(R, N, K, dtype, gated, al, 1), dx = cut_of(R, K, gated ? 2 * b.pad : N, dtype, false, al, 1), dw = cut_of(N, K, R, dtype, false, al, parts);
+        const Cut z = cut_of(R, gated ? b.pad : N, K, dtype, gated, al, 1), dx = cut_of(R, K, gated ? 2 * b.pad : N, dtype, false, al, 1), dw = cut_of(N, K, R, dtype, false, al, parts);
         if (!no_act) {
             b.strips = max64(b.strips, strips_of(z, R));
             b.part = max64(b.part, (int64_t)part_bytes(z, R, N, gated, 1));
@@ -436,7 +452,7 @@ int backward(const void *x, const void *w, const void *w2, const void *bias, con
         a.vec_io = aligned16(dy, N * eb);
         a.colsum = db || db2 ? colsum : nullptr; a.colsum_ld = b.colsum_ld; a.part = part;
         const bool al = aligned16(x, K * eb) && aligned16(w, K * eb) && aligned16(w2, K * eb);
-        const Cut c = cut_of(R, N, K, dtype, gated, al, 1);
+        const Cut c = cut_of(R, gated ? b.pad : N, K, dtype, gated, al, 1);                   // (the tiles write the padding columns too)
         const int rc = run_product(a, gated ? PROD_GATED_BWD : PROD_LINEAR_BWD, dtype, c, al, 1, st);
         if (rc != W3D_OK) return rc;
         strips = strips_of(c, R);
