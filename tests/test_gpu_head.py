@@ -74,7 +74,7 @@ def deriv_error(z, ez, name):
 SIZES = [(1, 1, 1), (1, 4096, 17), (3, 7, 5), (16, 64, 64), (17, 130, 33), (33, 40, 256), (64, 256, 48), (65, 128, 128), (100, 1000, 3), (129, 72, 200), (257, 515, 131), (300, 2048, 96),
          (1000, 64, 1024), (700, 999, 515), (4100, 136, 264)]
 # 16-bit (and 8-bit) rows in numbers that take the 256 x 256 tile: whole tiles, odd edges everywhere, a contraction tail, sliced contractions
-LARGE = [(4096, 512, 2048), (9001, 264, 1304), (16400, 72, 1032), (1030, 2056, 1016), (5000, 1032, 520)]
+LARGE = [(4096, 512, 2048), (9001, 264, 1304), (16400, 72, 1032), (1030, 2056, 1016), (5000, 1032, 520), (6000, 520, 1301)]
 
 
 def linear_case(R, K, N, dt, act, bias, res, seed=0, bias_dt=None):

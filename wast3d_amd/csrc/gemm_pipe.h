@@ -1,4 +1,4 @@
-// The large tile: 256 x 256 outputs, 8 waves, 16-bit or fp8 operands whose rows are multiples of 16 bytes.  (gemm_tile.h: operand orders, output layout, epilogues.)
+// The large tile: 256 x 256 outputs, 8 waves, 16-bit or fp8 operands and outputs whose rows are aligned multiples of 16 bytes.  (gemm_tile.h: operand orders, output layout, epilogues.)
 //
 // Why this shape.  A 256 x 256 tile moves 32 KB from L2 per 64 bytes of contraction, 32 B per clock and CU at the full matrix rate; 128 x 128 tiles would need twice that, more than the
 // L2s give (they stopped at 0.66 PFLOP/s).  A wave owns 128 x 64 outputs: 128 accumulator registers, 12 KB of fragments from LDS for 512 cycles of matrix instructions.
@@ -22,8 +22,9 @@ template <int DT, int LX, int LW, int EPI>
 struct Pipe {
     static constexpr int BM = 256, BN = 256, WM = 2, WN = 4, NT = 512, EB = Elem<DT>::B, KPS = PIPE_SLAB / EB, MS = DT == W3D_DTYPE_FP8_E4M3 ? 32 : 16;
     static_assert(EB <= 2 && (EB == 2 || (LX == K_ROWS && LW == K_ROWS)), "16-bit operands in any order, fp8 rows of contiguous k");
-    typedef Out<DT, EPI, BM, BN, WM, WN, MS> O;
+    typedef Out<DT, EPI, BM, BN, WM, WN, MS, true> O;
     static constexpr int FM = O::FM, FN = O::FN, BNP = O::BNP, SIDE = 256 * PIPE_SLAB, BUF = 2 * SIDE, LDS_BYTES = PIPE_RING * BUF;
+    static_assert(LDS_BYTES >= WM * WN * O::PATCH, "the slabs' LDS becomes the waves' patches");
     static constexpr bool GATED = O::GATED;
 
     // 16-byte chunk permutation inside an LDS row.  K_ROWS (64-byte rows): 8 neighbouring lanes read 8 rows, two of which share the banks of 128 bytes.  M_ROWS (512-byte rows of one k):

@@ -138,6 +138,15 @@ __device__ __forceinline__ void unpack8(const i32x4 (&r)[Elem<DT>::B / 2], float
         }
     }
 }
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {                                  // two 16-bit elements, round to nearest even, in one instruction
+    const f32x2 v = {a, b};
+    if (DT == W3D_DTYPE_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+}
 template <int DT, int CNT>
 __device__ __forceinline__ void store_run(uint8_t *p, int64_t n, bool vec, const float (&v)[CNT]) {
     constexpr int EB = Elem<DT>::B;
@@ -146,11 +155,7 @@ __device__ __forceinline__ void store_run(uint8_t *p, int64_t n, bool vec, const
 #pragma unroll
         for (int i = 0; i < CNT * EB / 4; ++i) {
             if (DT == W3D_DTYPE_F32) w[i] = __float_as_uint(v[i]);
-            else {
-                const uint16_t a = DT == W3D_DTYPE_BF16 ? f32_to_bf16(v[2 * i]) : f32_to_f16(v[2 * i]);
-                const uint16_t b = DT == W3D_DTYPE_BF16 ? f32_to_bf16(v[2 * i + 1]) : f32_to_f16(v[2 * i + 1]);
-                w[i] = (uint32_t)a | ((uint32_t)b << 16);
-            }
+            else w[i] = pack2<DT>(v[2 * i], v[2 * i + 1]);
         }
         if (CNT * EB >= 16) {
 #pragma unroll
@@ -209,30 +214,34 @@ __device__ __forceinline__ f32x4 mfma_step(const i32x4 (&w)[2], const i32x4 (&x)
 }
 
 // ---- what becomes of a wave's accumulators.  MS: rows of the matrix instruction (16 or 32): a lane holds groups of four consecutive n of one row m.  They go through a patch of LDS that the
-// wave has to itself, 64 rows at a time and in f32, and come back as runs of 8 n: 8 (gated: 4) lanes hold a row's 64 (32) columns, so that every load and store of the epilogue is whole
+// wave has to itself, ROWS rows at a time and in f32, and come back as runs of 8 n: 8 (gated: 4) lanes hold a row's 64 (32) columns, so that every load and store of the epilogue is whole
 // 128-byte (64-byte) pieces of a row.  (Straight from the accumulators a store writes 16-byte pieces of 16 rows: 14 us per 256 x 256 tile instead of 8.)
+// 16 rows at a time, unrolled (the accumulators cannot be indexed at run time): 55 us for 65536 x 256 -> 1024 where 64 rows and a loop take 64.  Gradients take up to 64 rows and loop over
+// them a few passes at a time: unrolled as a whole, derivative, dy and column sums spill.
 // What the epilogue reads (residual, dy) is loaded AHEAD passes early: a pass is a fraction of the memory's latency.
-template <int DT, int EPI, int BM, int BN, int WM, int WN, int MS>
+// VEC: rows of C (and of residual and dy) are whole, aligned runs of 8: a run is inside or outside, and there is no path by element (unrolled as often as here it costs registers: spills).
+template <int DT, int EPI, int BM, int BN, int WM, int WN, int MS, bool VEC>
 struct Out {
     static constexpr int EB = Elem<DT>::B;
     static constexpr bool GATED = EPI == EPI_GATED || EPI == EPI_GATED_BWD, BWD = EPI == EPI_LINEAR_BWD || EPI == EPI_GATED_BWD;
     static constexpr int PARTS = GATED ? 2 : 1, BNP = BN / PARTS;                              // a gated tile is BN / 2 columns of each half: rows [0, BN/2) of the W slab gate, the rest up
     static constexpr int FM = BM / WM / MS, FN = BN / WN / MS, FP = FN / PARTS;
     static constexpr int COLS = BN / WN, PCOLS = COLS / PARTS, LPR = PCOLS / 8, RPP = 64 / LPR;      // lanes per row, rows per pass
-    static constexpr int ROWS = BM / WM < 64 ? BM / WM : 64, CHUNKS = BM / WM / ROWS, PASSES = ROWS / RPP;
-    static constexpr int UN = EPI == EPI_GATED_BWD || PASSES < 2 ? 1 : 2;                      // UN passes at a time: their LDS reads, arithmetic and stores overlap
-    static constexpr int AHEAD = PASSES < 4 ? PASSES : 4;
+    static constexpr int ROWS = !BWD ? 16 : BM / WM < 64 ? BM / WM : 64, CHUNKS = BM / WM / ROWS, PASSES = ROWS / RPP, ALL = CHUNKS * PASSES, AHEAD = PASSES < 2 ? 1 : ALL < 4 || GATED ? 2 : 4;
+    static constexpr int TURN = BWD ? AHEAD : PASSES;                                          // passes unrolled at a time
     static constexpr int PATCH = ROWS * COLS * 4;
-    static_assert(COLS == 64 && BM / WM % ROWS == 0 && PASSES % UN == 0, "a patch row is 16 chunks; whole chunks of rows");
+    static_assert(COLS == 64 && BM / WM % ROWS == 0 && ROWS % 16 == 0 && PASSES % TURN == 0 && TURN % AHEAD == 0 || !BWD, "a patch row is 16 chunks");
     typedef typename std::conditional<MS == 32, f32x16, f32x4>::type acc_t;
     typedef acc_t Acc[FM][FN];
 
     static __device__ __forceinline__ int w_row(int wn, int f, int lane) { return (f / FP) * BNP + wn * PCOLS + MS * (f % FP) + (lane & (MS - 1)); }     // tile row of the lane's operand row
     static __device__ __forceinline__ int x_row(int wm, int f, int lane) { return wm * (BM / WM) + MS * f + (lane & (MS - 1)); }
 
-    // chunks of 16 bytes are permuted by XOR with the row: lanes that write (read) neighbouring rows touch different banks
-    static __device__ __forceinline__ void put(const Acc &acc, int i, int lane, uint8_t *patch) {
-        const int row = MS * (i % (ROWS / MS)) + (lane & (MS - 1));
+    // 16 rows of the wave (step 0, 1, ..) into the patch; chunks of 16 bytes are permuted by XOR with the row: lanes that write (read) neighbouring rows touch different banks
+    static __device__ __forceinline__ void put(const Acc &acc, int step, int lane, uint8_t *patch) {
+        const int row = lane & 15;
+        if (MS == 32 && ((lane >> 4) & 1) != (step & 1)) return;                               // half of a 32-row fragment
+        const int i = step / (MS / 16);
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
@@ -241,101 +250,98 @@ struct Out {
                 f32x4 v;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * b + e];
-                *reinterpret_cast<f32x4 *>(patch + row * (COLS * 4) + ((chunk ^ (row & 15)) << 4)) = v;
+                *reinterpret_cast<f32x4 *>(patch + (16 * (step % (ROWS / 16)) + row) * (COLS * 4) + ((chunk ^ row) << 4)) = v;
             }
     }
-    static __device__ __forceinline__ void get(const uint8_t *patch, int row, int part, int lane, float (&v)[8]) {
-        const int first = part * (PCOLS / 4) + 2 * (lane % LPR);
+    static __device__ __forceinline__ void get(const uint8_t *patch, int pass, int part, int lane, float (&v)[8]) {
+        const int row = pass * RPP + lane / LPR, first = part * (PCOLS / 4) + 2 * (lane % LPR);
         f32x4 t[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) t[c] = *reinterpret_cast<const f32x4 *>(patch + row * (COLS * 4) + (((first + c) ^ (row & 15)) << 4));
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = t[e / 4][e % 4];
     }
-    // f(row m, row in the patch, 8 elements of src per pass) for every UN rows, RPP apart, that this lane finishes.  src: [M][N] of type OT or NULL; n: the lane's first column
-    template <int OT, typename F>
-    static __device__ __forceinline__ void each_row(const GemmArgs &a, const Acc &acc, const uint8_t *src, int64_t m0, int64_t n, int wm, int lane, uint8_t *patch, F f) {
+    // f(pass of the patch, row of the wave, is the row inside C, 8 elements of src, byte offset of the row's run past the wave's first row of dst) for every row this lane finishes.
+    // SRC: there is a src, [M][N] of type OT; n: the lane's first column, c0: the wave's; ld: bytes from row to row of dst, DB: bytes of its elements.  (SRC at compile time: a load that may
+    // be in flight makes the passes of a tile without one wait for their own stores.)
+    template <int OT, int DB, bool SRC, typename F>
+    static __device__ __forceinline__ void each_row(const GemmArgs &a, const Acc &acc, const uint8_t *src, int64_t ld, int64_t m0, int64_t n, int64_t c0, int wm, int lane, uint8_t *patch, F f) {
         constexpr int OB = Elem<OT>::B, RAW = OB * 8 / 16;
-        const int64_t mw = m0 + wm * (BM / WM) + lane / LPR;
-        const bool fast = src && a.vec_io && n + 8 <= a.N;
-        i32x4 ring[AHEAD][RAW];
-        const uint8_t *at = src + (mw * a.N + n) * OB;
-        const int64_t step = RPP * a.N * OB;
-        int64_t next = mw;
-        auto fetch = [&](i32x4 (&r)[RAW]) {
-            if (fast && next < a.M)
+        const int64_t mw = m0 + wm * (BM / WM), left64 = a.M - mw - lane / LPR;
+        const int left = (int)(left64 < BM ? left64 < -BM ? -BM : left64 : BM);                // rows from the lane's first that exist (<= 0: none)
+        const bool any = a.M > mw && a.N > c0;                                                 // the wave's corner is inside C (uniform)
+        const bool fast = VEC || (a.vec_io && n + 8 <= a.N);
+        i32x4 ring[AHEAD][RAW];                                                                // src of the next passes (indexed at compile time: a rotation would wait for the loads)
+        const uint32_t src_ld = (uint32_t)(a.N * OB);
+        const uint8_t *from = src + mw * a.N * OB + c0 * OB;                                   // the wave's corner: uniform, lanes add 32 bits
+        // VEC: loads are unconditional (the compiler counts them): rows and columns outside C read the tile's last row and the wave's first columns
+        const uint32_t col = VEC && n >= a.N ? 0u : (uint32_t)(n - c0) * OB;
+        auto fetch = [&](int q, int slot) {
+            const int r = VEC ? (q * RPP < left ? q * RPP : left - 1) : q * RPP;
+            if (VEC ? any : fast && r < left)
 #pragma unroll
-                for (int k = 0; k < RAW; ++k) r[k] = reinterpret_cast<const i32x4 *>(at)[k];
-            at += step;
-            next += RPP;
+                for (int k = 0; k < RAW; ++k) ring[slot][k] = reinterpret_cast<const i32x4 *>(from + (uint32_t)(lane / LPR + r) * src_ld + col)[k];
         };
-        if (src)
+        if (SRC)
 #pragma unroll
-            for (int k = 0; k < AHEAD; ++k) fetch(ring[k]);
+            for (int k = 0; k < AHEAD; ++k) fetch(k, k);
+        uint32_t off = (uint32_t)(lane / LPR) * (uint32_t)ld + (uint32_t)(n - c0) * DB;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
 #pragma unroll
-            for (int i = 0; i < ROWS / MS; ++i) put(acc, c * (ROWS / MS) + i, lane, patch);
+            for (int s = 0; s < ROWS / 16; ++s) put(acc, c * (ROWS / 16) + s, lane, patch);
             __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
-            for (int p = 0; p < PASSES; p += UN) {
-                const int64_t m = mw + c * ROWS + p * RPP;
-                float t[UN][8] = {};
-                if (src) {
+            for (int p0 = 0; p0 < PASSES; p0 += TURN)
 #pragma unroll
-                    for (int k = 0; k < UN; ++k) {
-                        if (fast) unpack8<OT>(ring[k], t[k]);
-                        else if (m + k * RPP < a.M) load_run<OT, 8>(src + ((m + k * RPP) * a.N + n) * OB, a.N - n, false, t[k]);
+                for (int k = 0; k < TURN; ++k) {
+                    const int p = p0 + k, q = c * PASSES + p, row = q * RPP;
+                    float t[8] = {};
+                    if (SRC) {
+                        if (fast) unpack8<OT>(ring[(c * PASSES + k) % AHEAD], t);
+                        else if (!VEC && row < left) load_run<OT, 8>(from + (uint32_t)(lane / LPR + row) * src_ld + (uint32_t)(n - c0) * OB, a.N - n, false, t);
+                        if (q + AHEAD < ALL) fetch(q + AHEAD, (c * PASSES + k) % AHEAD);
                     }
-#pragma unroll
-                    for (int k = 0; k + UN < AHEAD; ++k)
-#pragma unroll
-                        for (int q = 0; q < RAW; ++q) ring[k][q] = ring[k + UN][q];
-#pragma unroll
-                    for (int k = 0; k < UN; ++k) fetch(ring[AHEAD - UN + k]);
+                    f(p, row, row < left, t, off);
+                    off += RPP * (uint32_t)ld;
                 }
-                f(m, p * RPP + lane / LPR, t);
-            }
             __builtin_amdgcn_wave_barrier();
         }
     }
 
     static __device__ __forceinline__ void epilogue(const GemmArgs &a, const Acc &acc, int64_t m0, int64_t n0, int slice, int tm, int wm, int wn, int lane, bool z1, uint8_t *patch) {
-        const int64_t n = n0 + wn * PCOLS + 8 * (lane % LPR);
+        const int64_t c0 = n0 + wn * PCOLS, n = c0 + 8 * (lane % LPR);
         if (a.slices > 1) {
-            const int64_t z = (int64_t)(z1 ? a.slices : 0) + slice;
-            each_row<W3D_DTYPE_F32>(a, acc, nullptr, m0, n, wm, lane, patch, [&](int64_t m, int row, float (&)[UN][8]) {
-                float v[UN * PARTS][8];
+            const int64_t z = (int64_t)(z1 ? a.slices : 0) + slice, ld = a.part_ld * 4;
+            uint8_t *out = (uint8_t *)a.part + (z * a.M + m0 + wm * (BM / WM)) * ld + c0 * 4;
+            each_row<W3D_DTYPE_F32, 4, false>(a, acc, nullptr, ld, m0, n, c0, wm, lane, patch, [&](int pass, int, bool live, float (&)[8], uint32_t off) {
 #pragma unroll
-                for (int k = 0; k < UN * PARTS; ++k) get(patch, row + k / PARTS * RPP, k % PARTS, lane, v[k]);
-#pragma unroll
-                for (int k = 0; k < UN * PARTS; ++k) {
-                    const int64_t mk = m + k / PARTS * RPP;
-                    if (mk < a.M) store_run<W3D_DTYPE_F32, 8>((uint8_t *)(a.part + (z * a.M + mk) * a.part_ld + k % PARTS * (a.part_ld / 2) + n), a.N - n, true, v[k]);
+                for (int p = 0; p < PARTS; ++p) {
+                    float v[8];
+                    get(patch, pass, p, lane, v);
+                    if (live && n < a.N) store_run<W3D_DTYPE_F32, 8>(out + off + p * (ld / 2), VEC ? 8 : a.N - n, true, v);
                 }
             });
             return;
         }
         // (fp8 rows: the output is bf16 or f16)
         if constexpr (DT == W3D_DTYPE_FP8_E4M3) {
-            if (a.out_dt == W3D_DTYPE_BF16) finish<W3D_DTYPE_BF16>(a, acc, m0, n, tm, wm, lane, z1, patch);
-            else finish<W3D_DTYPE_F16>(a, acc, m0, n, tm, wm, lane, z1, patch);
-        } else finish<DT>(a, acc, m0, n, tm, wm, lane, z1, patch);
+            if (a.out_dt == W3D_DTYPE_BF16) finish<W3D_DTYPE_BF16>(a, acc, m0, n, c0, tm, wm, lane, z1, patch);
+            else finish<W3D_DTYPE_F16>(a, acc, m0, n, c0, tm, wm, lane, z1, patch);
+        } else finish<DT>(a, acc, m0, n, c0, tm, wm, lane, z1, patch);
     }
 
     template <int OT>
-    static __device__ __forceinline__ void finish(const GemmArgs &a, const Acc &acc, int64_t m0, int64_t n, int tm, int wm, int lane, bool z1, uint8_t *patch) {
+    static __device__ __forceinline__ void finish(const GemmArgs &a, const Acc &acc, int64_t m0, int64_t n, int64_t col0, int tm, int wm, int lane, bool z1, uint8_t *patch) {
         constexpr int OB = Elem<OT>::B;
         const bool vec = a.vec_io != 0;
+        const int64_t mw = m0 + wm * (BM / WM);
+        uint8_t *out = (EPI == EPI_STORE && z1 ? a.out2 : a.out) + mw * a.ld_out + col0 * OB;
         if constexpr (EPI == EPI_STORE) {
-            uint8_t *out = z1 ? a.out2 : a.out;
-            each_row<OT>(a, acc, nullptr, m0, n, wm, lane, patch, [&](int64_t m, int row, float (&)[UN][8]) {
-                float v[UN][8];
-#pragma unroll
-                for (int k = 0; k < UN; ++k) get(patch, row + k * RPP, 0, lane, v[k]);
-#pragma unroll
-                for (int k = 0; k < UN; ++k)
-                    if (m + k * RPP < a.M) store_run<OT, 8>(out + (m + k * RPP) * a.ld_out + n * OB, a.N - n, vec, v[k]);
+            each_row<OT, OB, false>(a, acc, nullptr, a.ld_out, m0, n, col0, wm, lane, patch, [&](int pass, int, bool live, float (&)[8], uint32_t off) {
+                float v[8];
+                get(patch, pass, 0, lane, v);
+                if (live && n < a.N) store_run<OT, 8>(out + off, VEC ? 8 : a.N - n, VEC || vec, v);
             });
             return;
         }
@@ -349,63 +355,52 @@ struct Out {
             s0[e] = s1[e] = 0;
             if (DT == W3D_DTYPE_FP8_E4M3 && n + e < a.N) { s0[e] = a.ws[n + e] - 254; if (GATED) s1[e] = a.ws2[n + e] - 254; }
         }
-        each_row<OT>(a, acc, BWD ? a.dy : a.res, m0, n, wm, lane, patch, [&](int64_t m, int row, float (&t)[UN][8]) {
-            float v[UN][8], u[UN][8];
+        const int64_t pad = (EPI == EPI_GATED_BWD ? a.half_out : a.ld_out) / OB - n;           // BWD: columns of the padded row from here, a multiple of 8 (16 bits) or 4
+        auto row = [&](auto act_c, auto src_c, int pass, int r, bool live, float (&t)[8], uint32_t off) {
+            float v[8], u[8];
+            get(patch, pass, 0, lane, v);
+            if (GATED) get(patch, pass, 1, lane, u);
+            if (DT == W3D_DTYPE_FP8_E4M3) {
+                const int xs = live ? a.xs[mw + lane / LPR + r] : 0;
 #pragma unroll
-            for (int k = 0; k < UN; ++k) {
-                get(patch, row + k * RPP, 0, lane, v[k]);
-                if (GATED) get(patch, row + k * RPP, 1, lane, u[k]);
+                for (int e = 0; e < 8; ++e) { v[e] = __builtin_ldexpf(v[e], xs + s0[e]); if (GATED) u[e] = __builtin_ldexpf(u[e], xs + s1[e]); }
             }
-            if (DT == W3D_DTYPE_FP8_E4M3)
 #pragma unroll
-                for (int k = 0; k < UN; ++k) {
-                    const int xs = m + k * RPP < a.M ? a.xs[m + k * RPP] : 0;
+            for (int e = 0; e < 8; ++e) { v[e] += b0[e]; if (GATED) u[e] += b1[e]; }
+            auto apply = [&](auto act) {
+                constexpr int ACT = decltype(act)::value;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) { v[k][e] = __builtin_ldexpf(v[k][e], xs + s0[e]); if (GATED) u[k][e] = __builtin_ldexpf(u[k][e], xs + s1[e]); }
-                }
-            with_act(a.act, [&](auto act_c) {
-                constexpr int ACT = decltype(act_c)::value;
-#pragma unroll
-                for (int k = 0; k < UN; ++k)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        float &z = v[k][e], &up = u[k][e];
-                        z += b0[e];
-                        if (GATED) up += b1[e];
-                        if (!BWD) {
-                            z = act_fwd<ACT>(z);
-                            if (EPI == EPI_GATED) z *= up;
-                        } else {
-                            float act, der;
-                            act_both<ACT>(z, act, der);
-                            if (EPI == EPI_LINEAR_BWD) z = t[k][e] * der;
-                            else { z = t[k][e] * (up * der); up = t[k][e] * act; }
-                        }
-                    }
-            });
-#pragma unroll
-            for (int k = 0; k < UN; ++k) {
-                const int64_t mk = m + k * RPP;
-                const bool live = mk < a.M;
-                if (!BWD) {
-                    if (EPI == EPI_LINEAR && a.res)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[k][e] += t[k][e];
-                    if (live) store_run<OT, 8>(a.out + mk * a.ld_out + n * OB, a.N - n, vec, v[k]);
-                } else {
-                    // dz; zeros in the padding columns (dy is read as zero there and z is finite: W has no such rows, the bias no such elements), which are part of the contraction
-                    // of dx.  Column sums in f32 before the rounding.
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) { c0[e] += live ? v[k][e] : 0.f; if (GATED) c1[e] += live ? u[k][e] : 0.f; }
-                    const int64_t pad = (EPI == EPI_GATED_BWD ? a.half_out : a.ld_out) / OB - n;      // columns of the padded row from here: a multiple of 8 (16 bits) or 4
-                    uint8_t *o = a.out + mk * a.ld_out + n * OB;
-                    if (live && pad > 0) {
-                        store_run<OT, 8>(o, pad, true, v[k]);
-                        if (EPI == EPI_GATED_BWD) store_run<OT, 8>(o + a.half_out, pad, true, u[k]);
+                for (int e = 0; e < 8; ++e) {
+                    if (!BWD) {
+                        v[e] = act_fwd<ACT>(v[e]);
+                        if (EPI == EPI_GATED) v[e] *= u[e];
+                        else if (decltype(src_c)::value) v[e] += t[e];
+                    } else {
+                        float f, d;
+                        act_both<ACT>(v[e], f, d);
+                        if (EPI == EPI_LINEAR_BWD) v[e] = t[e] * d;
+                        else { v[e] = t[e] * (u[e] * d); u[e] = t[e] * f; }
                     }
                 }
+            };
+            if constexpr (BWD) with_act(a.act, apply);                                         // (per row: five copies of the whole would spill)
+            else apply(act_c);
+            if (BWD)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { c0[e] += live ? v[e] : 0.f; if (GATED) c1[e] += live ? u[e] : 0.f; }      // column sums in f32, before the rounding
+            // BWD writes dz; zeros in the padding columns (dy is read as zero there and z is finite: W has no such rows, the bias no such elements), which are part of the contraction of dx
+            if (live && (BWD ? pad > 0 : n < a.N)) {
+                store_run<OT, 8>(out + off, VEC ? 8 : BWD ? pad : a.N - n, VEC || BWD || vec, v);
+                if (EPI == EPI_GATED_BWD) store_run<OT, 8>(out + off + a.half_out, VEC ? 8 : pad, true, u);
             }
-        });
+        };
+        auto rows = [&](auto act_c, auto src_c) {
+            each_row<OT, OB, decltype(src_c)::value>(a, acc, BWD ? a.dy : a.res, a.ld_out, m0, n, col0, wm, lane, patch,
+                                                     [&](int pass, int r, bool live, float (&t)[8], uint32_t off) { row(act_c, src_c, pass, r, live, t, off); });
+        };
+        if constexpr (BWD) rows(std::integral_constant<int, ACT_NONE>(), std::true_type());
+        else if (EPI == EPI_LINEAR && a.res) with_act(a.act, [&](auto act_c) { rows(act_c, std::true_type()); });
+        else with_act(a.act, [&](auto act_c) { rows(act_c, std::false_type()); });
         if (BWD && a.colsum) {
             // lanes l, l + LPR, ... hold the same columns
 #pragma unroll
@@ -441,7 +436,7 @@ __device__ __forceinline__ void tile_of_block(const GemmArgs &a, int &slice, int
 template <int DT, int LX, int LW, int EPI, int BM, int BN, int WM, int WN, bool ALIGNED>
 struct Gemm {
     static constexpr int NT = WM * WN * 64, EB = Elem<DT>::B, KPS = SLAB / EB;
-    typedef Out<DT, EPI, BM, BN, WM, WN, 16> O;
+    typedef Out<DT, EPI, BM, BN, WM, WN, 16, false> O;
     static constexpr int FM = O::FM, FN = O::FN, BNP = O::BNP;
     static constexpr bool GATED = O::GATED;
     typedef Stage<LX, BM, EB, NT> SX;

@@ -50,7 +50,10 @@ int launch_tile(const GemmArgs &a, int z, hipStream_t st) {
 template <int LX, int LW, int EPI>
 int launch_shape(const GemmArgs &a, int tile, bool aligned, int z, hipStream_t st) {
     if constexpr (W3D_LIN_DT != W3D_DTYPE_F32) {
-        if (tile == 256) return launch_kernel(gemm_pipe_kernel<W3D_LIN_DT, LX, LW, EPI>, Pipe<W3D_LIN_DT, LX, LW, EPI>::NT, Pipe<W3D_LIN_DT, LX, LW, EPI>::LDS_BYTES, a, z, st);
+        if (tile == 256) {
+            typedef Pipe<W3D_LIN_DT, LX, LW, EPI> P;
+            return launch_kernel(gemm_pipe_kernel<W3D_LIN_DT, LX, LW, EPI>, P::NT, P::LDS_BYTES, a, z, st);
+        }
     }
     if (tile == 128 && aligned) return launch_tile<LX, LW, EPI, 128, 128, 2, 2, true>(a, z, st);
     if (tile == 128) return launch_tile<LX, LW, EPI, 128, 128, 2, 2, false>(a, z, st);
@@ -308,18 +311,19 @@ constexpr TileCost COST_16 = {{0.35, 0.6, 1.2}, {0.22, 0.6, 1.3}, {4, 5, 10}}, C
 #define W3D_FORCE_SLICES 0
 #endif
 struct Cut { int tile, slices; int64_t tiles_m, tiles_n; };
-Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool gated, bool aligned, int batch) {
+// align: 0 none, 1 operands, 2 operands and everything the epilogue touches
+Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool gated, int align, int batch) {
     const int parts = gated ? 2 : 1;
     const int64_t slabs = (K * eb_of(dtype) + SLAB - 1) / SLAB;
     Cut best = {};
     double best_t = 0;
     for (int tile = 64; tile <= 256; tile *= 2) {
-        if (tile == 256 && (!aligned || dtype == W3D_DTYPE_F32)) break;
+        if (tile == 256 && (align < 2 || dtype == W3D_DTYPE_F32)) break;
         if (W3D_FORCE_TILE && tile != W3D_FORCE_TILE) continue;
         const int bn = tile / parts;
         const int64_t tm = (M + tile - 1) / tile, tn = (N + bn - 1) / bn, tiles = tm * tn * batch;
         const int k = tile == 64 ? 0 : tile == 128 ? 1 : 2;
-        const TileCost &c = dtype == W3D_DTYPE_F32 ? COST_F32 : !aligned ? COST_UNALIGNED : dtype == W3D_DTYPE_FP8_E4M3 ? COST_FP8 : COST_16;
+        const TileCost &c = dtype == W3D_DTYPE_F32 ? COST_F32 : !align ? COST_UNALIGNED : dtype == W3D_DTYPE_FP8_E4M3 ? COST_FP8 : COST_16;
         const int per_cu = tile == 256 ? 1 : tile == 128 ? 2 : 4;
         for (int s = 1; s <= 32 && (s == 1 || slabs / s >= 4); ++s) {
             if (W3D_FORCE_SLICES && s != W3D_FORCE_SLICES) continue;
@@ -336,7 +340,8 @@ size_t part_bytes(const Cut &c, int64_t M, int64_t N, bool gated, int batch) {
     return c.slices > 1 ? (size_t)batch * c.slices * M * ceil_to(N, 16) * (gated ? 2 : 1) * 4 : 0;
 }
 
-int run_product(GemmArgs &a, int prod, int dtype, const Cut &c, bool aligned, int z, hipStream_t st) {
+int run_product(GemmArgs &a, int prod, int dtype, const Cut &c, int align, int z, hipStream_t st) {
+    const bool aligned = align > 0;
     a.slices = c.slices;
     if (c.tiles_m > 0x7fffffff || c.tiles_n > 0x7fffffff) return W3D_ERR_UNSUPPORTED;
     a.tiles_m = (int)c.tiles_m; a.tiles_n = (int)c.tiles_n;
@@ -373,7 +378,7 @@ int forward(const void *x, const int32_t *xs, const void *w, const int32_t *ws, 
     a.bias = (const uint8_t *)bias; a.bias2 = (const uint8_t *)bias2; a.bias_f32 = bias_dtype == W3D_DTYPE_F32 && out_dtype != W3D_DTYPE_F32;
     a.res = (const uint8_t *)residual; a.xs = xs; a.ws = ws; a.ws2 = ws2;
     a.out = (uint8_t *)y; a.ld_out = N * eb_of(out_dtype); a.act = act; a.out_dt = out_dtype;
-    a.vec_io = aligned16(y, a.ld_out) && aligned16(residual, 0);
+    a.vec_io = aligned16(y, a.ld_out) && aligned16(residual, 0) ? 1 : 0;
     const int prod = gated ? PROD_GATED : PROD_LINEAR;
     if (R <= SKINNY_ROWS) {
         switch (dtype) {
@@ -383,18 +388,22 @@ int forward(const void *x, const int32_t *xs, const void *w, const int32_t *ws, 
             default: return w3d_lin_skinny_fp8(a, prod, st);
         }
     }
-    const bool aligned = aligned16(x, ld) && aligned16(w, ld) && aligned16(w2, ld);
-    const Cut c = cut_of(R, N, K, dtype, gated, aligned, 1);
+    const int align = aligned16(x, ld) && aligned16(w, ld) && aligned16(w2, ld) ? 1 + a.vec_io : 0;
+    const Cut c = cut_of(R, N, K, dtype, gated, align, 1);
     if (c.slices > 1 && (!workspace || (((uintptr_t)workspace) & 15) || workspace_bytes < part_bytes(c, R, N, gated, 1))) return W3D_ERR_WORKSPACE;
     a.part = (float *)workspace;
-    return run_product(a, prod, dtype, c, aligned, 1, st);
+    return run_product(a, prod, dtype, c, align, 1, st);
 }
 
-// the larger of the two cuts a call may take (its alignment is not known to the workspace query)
+// the largest of the cuts a call may take (its alignment is not known to the workspace query)
 size_t forward_bytes(int64_t R, int64_t K, int64_t N, int dtype, bool gated) {
     if (R <= SKINNY_ROWS || K < 1 || N < 1) return 0;
-    const size_t p = part_bytes(cut_of(R, N, K, dtype, gated, true, 1), R, N, gated, 1), q = part_bytes(cut_of(R, N, K, dtype, gated, false, 1), R, N, gated, 1);
-    return p > q ? p : q;
+    size_t most = 0;
+    for (int align = 0; align < 3; ++align) {
+        const size_t b = part_bytes(cut_of(R, N, K, dtype, gated, align, 1), R, N, gated, 1);
+        most = b > most ? b : most;
+    }
+    return most;
 }
 
 // ---- backward.  Workspace: dz | column sums | partial tiles (of one product at a time)
@@ -414,7 +423,7 @@ Bwd bwd_plan(int64_t R, int64_t K, int64_t N, int dtype, bool gated, bool no_act
     b.colsum_ld = ceil_to(N, 16) * parts;
     b.part = 0;
     b.strips = no_act ? w3d_column_strips(R, N) : 0;
-    for (int al = 0; al < 2; ++al) {
+    for (int al = 0; al < 3; ++al) {
         const Cut z = cut_of(R, gated ? b.pad : N, K, dtype, gated, al, 1), dx = cut_of(R, K, gated ? 2 * b.pad : N, dtype, false, al, 1), dw = cut_of(N, K, R, dtype, false, al, parts);
         if (!no_act) {
             b.strips = max64(b.strips, strips_of(z, R));
@@ -451,7 +460,7 @@ int backward(const void *x, const void *w, const void *w2, const void *bias, con
         a.dy = (const uint8_t *)dy; a.out = ws; a.ld_out = b.ld_dz; a.half_out = b.pad * eb; a.act = act; a.out_dt = dtype;
         a.vec_io = aligned16(dy, N * eb);
         a.colsum = db || db2 ? colsum : nullptr; a.colsum_ld = b.colsum_ld; a.part = part;
-        const bool al = aligned16(x, K * eb) && aligned16(w, K * eb) && aligned16(w2, K * eb);
+        const int al = aligned16(x, K * eb) && aligned16(w, K * eb) && aligned16(w2, K * eb) ? 1 + a.vec_io : 0;
         const Cut c = cut_of(R, gated ? b.pad : N, K, dtype, gated, al, 1);                   // (the tiles write the padding columns too)
         const int rc = run_product(a, gated ? PROD_GATED_BWD : PROD_LINEAR_BWD, dtype, c, al, 1, st);
         if (rc != W3D_OK) return rc;
@@ -470,7 +479,7 @@ int backward(const void *x, const void *w, const void *w2, const void *bias, con
         a.M = R; a.N = K; a.K = gated ? 2 * b.pad : N; a.k_split = gated ? b.pad : 0; a.w_rows = N;
         a.out = (uint8_t *)dx; a.ld_out = K * eb; a.out_dt = dtype; a.part = part;
         a.vec_io = aligned16(dx, K * eb);
-        const bool al = aligned16(dz, ld_dz) && aligned16(w, K * eb) && aligned16(w2, K * eb);
+        const int al = aligned16(dz, ld_dz) && aligned16(w, K * eb) && aligned16(w2, K * eb) ? 1 + a.vec_io : 0;
         const int rc = run_product(a, PROD_DX, dtype, cut_of(R, K, a.K, dtype, false, al, 1), al, 1, st);
         if (rc != W3D_OK) return rc;
     }
@@ -490,7 +499,7 @@ int backward(const void *x, const void *w, const void *w2, const void *bias, con
         a.M = N; a.N = K; a.K = R; a.w_rows = R; a.z_x = b.pad * eb;
         a.out = (uint8_t *)o; a.out2 = (uint8_t *)dw2; a.ld_out = K * eb; a.out_dt = dtype; a.part = part;
         a.vec_io = aligned16(o, K * eb) && aligned16(both ? dw2 : nullptr, 0);
-        const bool al = aligned16(a.x, ld_dz) && aligned16(x, K * eb);
+        const int al = aligned16(a.x, ld_dz) && aligned16(x, K * eb) ? 1 + a.vec_io : 0;
         const int rc = run_product(a, PROD_DW, dtype, cut_of(N, K, R, dtype, false, al, parts), al, both ? 2 : 1, st);
         if (rc != W3D_OK) return rc;
     }
