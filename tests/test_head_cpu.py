@@ -50,9 +50,11 @@ def test_linear_arguments(L):
     assert f(P, P, P, 1, None, 4, 8, 6, 2, 0, P, None, 0, None) == ARG                          # bias bf16 next to f16
     assert f(P, P, None, 0, None, 4, 1 << 22, 6, 0, 0, P, None, 0, None) == UNSUP               # rows of 16 MB
     assert f(None, None, None, 0, None, 0, 8, 6, 0, 0, None, None, 0, None) == 0                # no rows
-    assert L.w3d_linear_workspace_bytes(300, 4096, 64, 1, 0) > 0                                # few tiles, a long contraction: slices
+    assert L.w3d_linear_workspace_bytes(300, 4096, 64, 1, 0, 0) > 0                                # few tiles, a long contraction: slices
     assert f(P, P, None, 0, None, 300, 4096, 64, 1, 0, P, None, 0, None) == WS
-    assert L.w3d_linear_workspace_bytes(1, 4096, 64, 1, 0) == 0
+    assert L.w3d_linear_workspace_bytes(1, 4096, 64, 1, 0, 1) == 0
+    assert L.w3d_linear_workspace_bytes(300, 64, 64, 1, 0, 1) >= 300 * 128 + 64 * 128 and L.w3d_linear_workspace_bytes(300, 63, 64, 1, 0, 0) >= 300 * 128 + 64 * 128      # aligned copies
+    assert f(P, P, None, 0, None, 300, 63, 64, 1, 0, P, None, 0, None) == WS
     g = L.w3d_gated_linear_fwd
     assert g(P, P, None, None, None, 0, 4, 8, 6, 0, 3, P, None, 0, None) == ARG
     e = L.w3d_linear_fp8_fwd
@@ -63,7 +65,7 @@ def test_linear_arguments(L):
     assert b(P, P, None, 0, P, 4, 8, 6, 0, 0, None, None, None, P, 4096, None) == ARG           # nothing wanted
     assert b(P, P, None, 0, None, 4, 8, 6, 0, 0, P, P, None, P, 4096, None) == ARG
     assert b(P, P, None, 0, P, 400, 8, 6, 0, 2, P, P, None, P, 16, None) == WS
-    assert L.w3d_linear_bwd_workspace_bytes(0, 8, 6, 0, 0, 0) == 0
+    assert L.w3d_linear_bwd_workspace_bytes(0, 8, 6, 0, 0, 0, 0) == 0
     assert L.w3d_gated_linear_bwd(P, P, None, None, None, 0, P, 4, 8, 6, 0, 3, P, P, P, None, None, P, 4096, None) == ARG
 
 

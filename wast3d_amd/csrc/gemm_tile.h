@@ -4,7 +4,8 @@
 //   z  = x W^T        X: x [R][K] K_ROWS,    W: W [N][K] K_ROWS
 //   dx = dz W         X: dz [R][N] K_ROWS,   W: W [N][K] M_ROWS   (contraction over N)
 //   dW = dz^T x       X: dz [R][N] M_ROWS,   W: x [R][K] M_ROWS   (contraction over R)
-// so no transposed copy of anything is ever made: M_ROWS fragments are formed by the transposing LDS read (16 bits) or single-element reads (f32).
+// so no transposed copy of anything is ever made: M_ROWS fragments are formed by the transposing LDS read (16 bits) or single-element reads (f32).  Storage rows of operands are 16-byte
+// aligned (linear.hip copies the ones that are not).
 //
 // Slabs.  The contraction advances in slabs of 128 bytes of k (32 f32, 64 16-bit, 128 fp8 elements).  A K_ROWS slab is [rows][128 B], an M_ROWS slab [k of the slab][rows x element];
 // 16-byte chunks are permuted inside a row (XOR with bits of the row) so that the fragment reads of 8 (16) neighbouring lanes touch all LDS banks.
@@ -60,17 +61,18 @@ constexpr int SLAB = 128;                        // bytes of contraction per sla
 constexpr uint32_t OUT_OF_RANGE = 0x80000000u;   // buffer offset past num_records: the load returns zeros
 
 // ---- activations.  a = act(z), d = act'(z).
-// gelu(z) = z Phi(z); Phi(-|z|) = exp(-z^2 / 2) p(t) / 2, t = 1 / (1 + 0.3275911 |z| / sqrt 2), p the degree-5 polynomial of Abramowitz & Stegun 7.1.26 (|error of erf| <= 1.5e-7): one exponential
-// serves Phi and the density in the derivative, and the tail has no cancellation.
+// gelu(z) = z Phi(z) = max(z, 0) - h Phi(-h), h = |z|.  log2 Phi(-h) is nearly a parabola: a polynomial of degree 6, fitted on [0, 5.75] to the smallest maximum of h |error of Phi|, and
+// one exponential give gelu to 2.4e-7 and Phi to 8e-7, the tail without cancellation; past 5.75, h Phi(-h) < 3e-8 stays what it is there.
+__device__ __forceinline__ float normal_tail(float h) {                                        // Phi(-h), 0 <= h <= 5.75
+    const float p = fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, 3.2983829e-5f, -7.6224754e-4f), 8.0370521e-3f), -5.3309143e-2f), -4.5887902e-1f), -1.1511532f), -1.0000001f);
+    return __builtin_amdgcn_exp2f(p);
+}
 template <int ACT>
 __device__ __forceinline__ float act_fwd(float z) {
     if (ACT == ACT_RELU) return z < 0.f ? 0.f : z;                       // (a NaN stays)
     if (ACT == ACT_GELU) {
-        const float h = fabsf(z);
-        const float t = __builtin_amdgcn_rcpf(fmaf(h, 0.3275911f * 0.70710678f, 1.0f));
-        const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-        const float tail = 0.5f * p * __expf(-0.5f * z * z);
-        return z * (z < 0.f ? tail : 1.0f - tail);
+        const float h = fminf(fabsf(z), 5.75f);
+        return fmaf(-h, normal_tail(h), z < 0.f ? 0.f : z);
     }
     if (ACT == ACT_SILU) return z * __builtin_amdgcn_rcpf(1.0f + __expf(-z));
     if (ACT == ACT_SIGMOID) return __builtin_amdgcn_rcpf(1.0f + __expf(-z));
@@ -81,12 +83,9 @@ __device__ __forceinline__ void act_both(float z, float &a, float &d) {
     if (ACT == ACT_NONE) { a = z; d = 1.f; }
     else if (ACT == ACT_RELU) { a = z < 0.f ? 0.f : z; d = z > 0.f ? 1.f : 0.f; }
     else if (ACT == ACT_GELU) {
-        const float h = fabsf(z);
-        const float t = __builtin_amdgcn_rcpf(fmaf(h, 0.3275911f * 0.70710678f, 1.0f));
-        const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-        const float e = __expf(-0.5f * z * z), tail = 0.5f * p * e, cdf = z < 0.f ? tail : 1.0f - tail;
-        a = z * cdf;
-        d = fmaf(z * 0.39894228f, e, cdf);
+        const float h = fminf(fabsf(z), 5.75f), tail = normal_tail(h), e = __builtin_amdgcn_exp2f(z * z * -0.72134752f);      // exp(-z^2 / 2)
+        a = fmaf(-h, tail, z < 0.f ? 0.f : z);
+        d = fmaf(z * 0.39894228f, e, z < 0.f ? tail : 1.0f - tail);
     } else {
         const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-z));
         if (ACT == ACT_SILU) { a = z * s; d = s * fmaf(z, 1.0f - s, 1.0f); }
@@ -433,7 +432,7 @@ __device__ __forceinline__ void tile_of_block(const GemmArgs &a, int &slice, int
     tn = in / rows;
 }
 
-template <int DT, int LX, int LW, int EPI, int BM, int BN, int WM, int WN, bool ALIGNED>
+template <int DT, int LX, int LW, int EPI, int BM, int BN, int WM, int WN>
 struct Gemm {
     static constexpr int NT = WM * WN * 64, EB = Elem<DT>::B, KPS = SLAB / EB;
     typedef Out<DT, EPI, BM, BN, WM, WN, 16, false> O;
@@ -479,23 +478,6 @@ struct Gemm {
         }
     }
 
-    // a chunk of 16 bytes whose first n elements exist (register staging: any alignment)
-    static __device__ __forceinline__ i32x4 chunk_of(const uint8_t *p, int64_t n) {
-        i32x4 v = {0, 0, 0, 0};
-        if (n >= 16 / EB) { __builtin_memcpy(&v, p, 16); return v; }
-        if (n <= 0) return v;
-        uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 16 / EB; ++i)
-            if (i < n) {
-                uint32_t b = 0;
-                __builtin_memcpy(&b, p + i * EB, EB);
-                w[i * EB / 4] |= b << (8 * ((i * EB) & 3));
-            }
-        __builtin_memcpy(&v, w, 16);
-        return v;
-    }
-
     // address and extent of piece i of a side's slab
     struct Side {
         const uint8_t *base;      // first byte of the tile's operand (K_ROWS: row 0 of the tile; M_ROWS: column 0 of the tile, contraction row 0)
@@ -515,16 +497,6 @@ struct Gemm {
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t)(lds_t)(slab + (i * NT + wave * 64) * 16), 16, (int)off, 0, 0, 0);
     }
-    template <typename S, int LAY>
-    static __device__ __forceinline__ i32x4 load_reg(const Side &sd, int64_t k0, int tid, int i) {
-        int row, chunk;
-        S::place(tid, i, row, chunk);
-        const int64_t kleft = sd.k - k0, e = (int64_t)chunk * (16 / EB);
-        const bool ok = LAY == K_ROWS ? row < sd.rows : row < kleft;
-        const int64_t n = ok ? (LAY == K_ROWS ? kleft : sd.rows) - e : 0;
-        return chunk_of(sd.base + (LAY == K_ROWS ? row * sd.ld + k0 * EB : (k0 + row) * sd.ld) + e * EB, n);
-    }
-
     static __device__ __forceinline__ void run(const GemmArgs &a, uint8_t *smem) {
         const int tid = threadIdx.x, lane = tid & 63;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
@@ -565,24 +537,7 @@ struct Gemm {
 #pragma unroll
             for (int i = 0; i < SW::PIECES; ++i) { Side s; w_side(k0, i, s); load_dma<SW, LW>(s, k0, buf + SX::BYTES, tid, i); }
         };
-        i32x4 rx[ALIGNED ? 1 : SX::PIECES], rw[ALIGNED ? 1 : SW::PIECES];
-        auto fetch = [&](int64_t t) {
-            const int64_t k0 = t * KPS;
-#pragma unroll
-            for (int i = 0; i < SX::PIECES; ++i) rx[ALIGNED ? 0 : i] = load_reg<SX, LX>(sx, k0, tid, i);
-#pragma unroll
-            for (int i = 0; i < SW::PIECES; ++i) { Side s; w_side(k0, i, s); rw[ALIGNED ? 0 : i] = load_reg<SW, LW>(s, k0, tid, i); }
-        };
-        auto put = [&](uint8_t *buf) {
-#pragma unroll
-            for (int i = 0; i < SX::PIECES; ++i) *reinterpret_cast<i32x4 *>(buf + (i * NT + tid) * 16) = rx[ALIGNED ? 0 : i];
-#pragma unroll
-            for (int i = 0; i < SW::PIECES; ++i) *reinterpret_cast<i32x4 *>(buf + SX::BYTES + (i * NT + tid) * 16) = rw[ALIGNED ? 0 : i];
-        };
-        if (s_begin < s_end) {
-            if (ALIGNED) dma(s_begin, smem);
-            else { fetch(s_begin); put(smem); }
-        }
+        if (s_begin < s_end) dma(s_begin, smem);
         int cur = 0;
         for (int64_t t = s_begin; t < s_end; ++t, cur ^= 1) {
             __syncthreads();                             // slab t has landed (every wave drains its own LDS-DMA), and nobody reads the other buffer any more
@@ -592,28 +547,23 @@ struct Gemm {
             for (int j = 0; j < FN; ++j) frag<SW, LW>(bw, O::w_row(wn, j, lane), wn * FN + j, lane, wf[j]);
 #pragma unroll
             for (int i = 0; i < FM; ++i) frag<SX, LX>(bx, O::x_row(wm, i, lane), wm * FM + i, lane, xf[i]);
-            const bool more = t + 1 < s_end;
-            if (more) {
-                if (ALIGNED) dma(t + 1, smem + (cur ^ 1) * BUF);
-                else fetch(t + 1);
-            }
+            if (t + 1 < s_end) dma(t + 1, smem + (cur ^ 1) * BUF);
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int i = 0; i < FM; ++i)
 #pragma unroll
                     for (int j = 0; j < FN; ++j) acc[i][j] = mfma_step<DT>(wf[j], xf[i], s, acc[i][j]);
-            if (!ALIGNED && more) put(smem + (cur ^ 1) * BUF);
         }
         __syncthreads();                                 // the slabs' LDS becomes the waves' patches
         O::epilogue(a, acc, m0, n0, slice, tm, wm, wn, lane, z1, smem + wave * O::PATCH);
     }
 };
 
-template <int DT, int LX, int LW, int EPI, int BM, int BN, int WM, int WN, bool ALIGNED>
+template <int DT, int LX, int LW, int EPI, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 1) void gemm_kernel(GemmArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    Gemm<DT, LX, LW, EPI, BM, BN, WM, WN, ALIGNED>::run(a, smem);
+    Gemm<DT, LX, LW, EPI, BM, BN, WM, WN>::run(a, smem);
 }
 
 }  // namespace

@@ -22,10 +22,10 @@ constexpr int SKINNY_ROWS = 64;
 }  // namespace
 
 // launches of one operand type's kernels
-int w3d_lin_tiles_f32(const GemmArgs &a, int prod, int tile, bool aligned, int z, hipStream_t st);
-int w3d_lin_tiles_bf16(const GemmArgs &a, int prod, int tile, bool aligned, int z, hipStream_t st);
-int w3d_lin_tiles_f16(const GemmArgs &a, int prod, int tile, bool aligned, int z, hipStream_t st);
-int w3d_lin_tiles_fp8(const GemmArgs &a, int prod, int tile, bool aligned, int z, hipStream_t st);
+int w3d_lin_tiles_f32(const GemmArgs &a, int prod, int tile, int z, hipStream_t st);
+int w3d_lin_tiles_bf16(const GemmArgs &a, int prod, int tile, int z, hipStream_t st);
+int w3d_lin_tiles_f16(const GemmArgs &a, int prod, int tile, int z, hipStream_t st);
+int w3d_lin_tiles_fp8(const GemmArgs &a, int prod, int tile, int z, hipStream_t st);
 int w3d_lin_skinny_f32(const GemmArgs &a, int prod, hipStream_t st);
 int w3d_lin_skinny_bf16(const GemmArgs &a, int prod, hipStream_t st);
 int w3d_lin_skinny_f16(const GemmArgs &a, int prod, hipStream_t st);
@@ -42,36 +42,34 @@ int launch_kernel(void (*kernel)(GemmArgs), int threads, int lds, const GemmArgs
     W3D_CHECK_LAUNCH();
     return W3D_OK;
 }
-template <int LX, int LW, int EPI, int BM, int BN, int WM, int WN, bool ALIGNED>
+template <int LX, int LW, int EPI, int BM, int BN, int WM, int WN>
 int launch_tile(const GemmArgs &a, int z, hipStream_t st) {
-    typedef Gemm<W3D_LIN_DT, LX, LW, EPI, BM, BN, WM, WN, ALIGNED> G;
-    return launch_kernel(gemm_kernel<W3D_LIN_DT, LX, LW, EPI, BM, BN, WM, WN, ALIGNED>, G::NT, G::LDS_BYTES, a, z, st);
+    typedef Gemm<W3D_LIN_DT, LX, LW, EPI, BM, BN, WM, WN> G;
+    return launch_kernel(gemm_kernel<W3D_LIN_DT, LX, LW, EPI, BM, BN, WM, WN>, G::NT, G::LDS_BYTES, a, z, st);
 }
 template <int LX, int LW, int EPI>
-int launch_shape(const GemmArgs &a, int tile, bool aligned, int z, hipStream_t st) {
+int launch_shape(const GemmArgs &a, int tile, int z, hipStream_t st) {
     if constexpr (W3D_LIN_DT != W3D_DTYPE_F32) {
         if (tile == 256) {
             typedef Pipe<W3D_LIN_DT, LX, LW, EPI> P;
             return launch_kernel(gemm_pipe_kernel<W3D_LIN_DT, LX, LW, EPI>, P::NT, P::LDS_BYTES, a, z, st);
         }
     }
-    if (tile == 128 && aligned) return launch_tile<LX, LW, EPI, 128, 128, 2, 2, true>(a, z, st);
-    if (tile == 128) return launch_tile<LX, LW, EPI, 128, 128, 2, 2, false>(a, z, st);
-    if (aligned) return launch_tile<LX, LW, EPI, 64, 64, 4, 1, true>(a, z, st);
-    return launch_tile<LX, LW, EPI, 64, 64, 4, 1, false>(a, z, st);
+    if (tile == 128) return launch_tile<LX, LW, EPI, 128, 128, 2, 2>(a, z, st);
+    return launch_tile<LX, LW, EPI, 64, 64, 4, 1>(a, z, st);
 }
-int launch_prod(const GemmArgs &a, int prod, int tile, bool aligned, int z, hipStream_t st) {
+int launch_prod(const GemmArgs &a, int prod, int tile, int z, hipStream_t st) {
     switch (prod) {
-        case PROD_LINEAR: return launch_shape<K_ROWS, K_ROWS, EPI_LINEAR>(a, tile, aligned, z, st);
-        case PROD_GATED: return launch_shape<K_ROWS, K_ROWS, EPI_GATED>(a, tile, aligned, z, st);
+        case PROD_LINEAR: return launch_shape<K_ROWS, K_ROWS, EPI_LINEAR>(a, tile, z, st);
+        case PROD_GATED: return launch_shape<K_ROWS, K_ROWS, EPI_GATED>(a, tile, z, st);
         default: break;
     }
     if constexpr (W3D_LIN_DT != W3D_DTYPE_FP8_E4M3) {
         switch (prod) {
-            case PROD_LINEAR_BWD: return launch_shape<K_ROWS, K_ROWS, EPI_LINEAR_BWD>(a, tile, aligned, z, st);
-            case PROD_GATED_BWD: return launch_shape<K_ROWS, K_ROWS, EPI_GATED_BWD>(a, tile, aligned, z, st);
-            case PROD_DX: return launch_shape<K_ROWS, M_ROWS, EPI_STORE>(a, tile, aligned, z, st);
-            case PROD_DW: return launch_shape<M_ROWS, M_ROWS, EPI_STORE>(a, tile, aligned, z, st);
+            case PROD_LINEAR_BWD: return launch_shape<K_ROWS, K_ROWS, EPI_LINEAR_BWD>(a, tile, z, st);
+            case PROD_GATED_BWD: return launch_shape<K_ROWS, K_ROWS, EPI_GATED_BWD>(a, tile, z, st);
+            case PROD_DX: return launch_shape<K_ROWS, M_ROWS, EPI_STORE>(a, tile, z, st);
+            case PROD_DW: return launch_shape<M_ROWS, M_ROWS, EPI_STORE>(a, tile, z, st);
             default: break;
         }
     }
@@ -204,7 +202,7 @@ int launch_skinny(const GemmArgs &a, hipStream_t st) {
 #else
 #define W3D_LIN_NAME(f) f##_fp8
 #endif
-int W3D_LIN_NAME(w3d_lin_tiles)(const GemmArgs &a, int prod, int tile, bool aligned, int z, hipStream_t st) { return launch_prod(a, prod, tile, aligned, z, st); }
+int W3D_LIN_NAME(w3d_lin_tiles)(const GemmArgs &a, int prod, int tile, int z, hipStream_t st) { return launch_prod(a, prod, tile, z, st); }
 int W3D_LIN_NAME(w3d_lin_skinny)(const GemmArgs &a, int prod, hipStream_t st) {
     return prod == PROD_GATED ? launch_skinny<EPI_GATED>(a, st) : launch_skinny<EPI_LINEAR>(a, st);
 }
@@ -303,7 +301,7 @@ bool aligned16(const void *p, int64_t ld) { return !(((uintptr_t)p) & 15) && ld 
 // Slices write and read their f32 tiles (2.5 TB/s with the second launch's start).
 struct TileCost { double lone[3], busy[3], round[3]; };      // of 64, 128, 256
 constexpr TileCost COST_16 = {{0.35, 0.6, 1.2}, {0.22, 0.6, 1.3}, {4, 5, 10}}, COST_FP8 = {{0.35, 0.6, 0.9}, {0.22, 0.6, 0.9}, {4, 5, 10}},
-                   COST_UNALIGNED = {{2.0, 3.5, 0}, {0.5, 1.2, 0}, {4, 5, 0}}, COST_F32 = {{0.72, 2.25, 0}, {0.62, 2.25, 0}, {4, 5, 0}};
+                   COST_F32 = {{0.72, 2.25, 0}, {0.62, 2.25, 0}, {4, 5, 0}};
 #ifndef W3D_FORCE_TILE
 #define W3D_FORCE_TILE 0
 #endif
@@ -311,19 +309,19 @@ constexpr TileCost COST_16 = {{0.35, 0.6, 1.2}, {0.22, 0.6, 1.3}, {4, 5, 10}}, C
 #define W3D_FORCE_SLICES 0
 #endif
 struct Cut { int tile, slices; int64_t tiles_m, tiles_n; };
-// align: 0 none, 1 operands, 2 operands and everything the epilogue touches
-Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool gated, int align, int batch) {
+// vec: rows of everything the epilogue touches are aligned, too (the 256 x 256 tile needs it)
+Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool gated, bool vec, int batch) {
     const int parts = gated ? 2 : 1;
     const int64_t slabs = (K * eb_of(dtype) + SLAB - 1) / SLAB;
     Cut best = {};
     double best_t = 0;
     for (int tile = 64; tile <= 256; tile *= 2) {
-        if (tile == 256 && (align < 2 || dtype == W3D_DTYPE_F32)) break;
+        if (tile == 256 && (!vec || dtype == W3D_DTYPE_F32)) break;
         if (W3D_FORCE_TILE && tile != W3D_FORCE_TILE) continue;
         const int bn = tile / parts;
         const int64_t tm = (M + tile - 1) / tile, tn = (N + bn - 1) / bn, tiles = tm * tn * batch;
         const int k = tile == 64 ? 0 : tile == 128 ? 1 : 2;
-        const TileCost &c = dtype == W3D_DTYPE_F32 ? COST_F32 : !align ? COST_UNALIGNED : dtype == W3D_DTYPE_FP8_E4M3 ? COST_FP8 : COST_16;
+        const TileCost &c = dtype == W3D_DTYPE_F32 ? COST_F32 : dtype == W3D_DTYPE_FP8_E4M3 ? COST_FP8 : COST_16;
         const int per_cu = tile == 256 ? 1 : tile == 128 ? 2 : 4;
         for (int s = 1; s <= 32 && (s == 1 || slabs / s >= 4); ++s) {
             if (W3D_FORCE_SLICES && s != W3D_FORCE_SLICES) continue;
@@ -340,18 +338,17 @@ size_t part_bytes(const Cut &c, int64_t M, int64_t N, bool gated, int batch) {
     return c.slices > 1 ? (size_t)batch * c.slices * M * ceil_to(N, 16) * (gated ? 2 : 1) * 4 : 0;
 }
 
-int run_product(GemmArgs &a, int prod, int dtype, const Cut &c, int align, int z, hipStream_t st) {
-    const bool aligned = align > 0;
+int run_product(GemmArgs &a, int prod, int dtype, const Cut &c, int z, hipStream_t st) {
     a.slices = c.slices;
     if (c.tiles_m > 0x7fffffff || c.tiles_n > 0x7fffffff) return W3D_ERR_UNSUPPORTED;
     a.tiles_m = (int)c.tiles_m; a.tiles_n = (int)c.tiles_n;
     a.part_ld = ceil_to(a.N, 16) * (prod == PROD_GATED || prod == PROD_GATED_BWD ? 2 : 1);
     int rc;
     switch (dtype) {
-        case W3D_DTYPE_F32: rc = w3d_lin_tiles_f32(a, prod, c.tile, aligned, z, st); break;
-        case W3D_DTYPE_BF16: rc = w3d_lin_tiles_bf16(a, prod, c.tile, aligned, z, st); break;
-        case W3D_DTYPE_F16: rc = w3d_lin_tiles_f16(a, prod, c.tile, aligned, z, st); break;
-        default: rc = w3d_lin_tiles_fp8(a, prod, c.tile, aligned, z, st); break;
+        case W3D_DTYPE_F32: rc = w3d_lin_tiles_f32(a, prod, c.tile, z, st); break;
+        case W3D_DTYPE_BF16: rc = w3d_lin_tiles_bf16(a, prod, c.tile, z, st); break;
+        case W3D_DTYPE_F16: rc = w3d_lin_tiles_f16(a, prod, c.tile, z, st); break;
+        default: rc = w3d_lin_tiles_fp8(a, prod, c.tile, z, st); break;
     }
     if (rc != W3D_OK || c.slices == 1) return rc;
     switch (a.out_dt) {
@@ -362,7 +359,66 @@ int run_product(GemmArgs &a, int prod, int dtype, const Cut &c, int align, int z
 }
 
 // 32-bit offsets inside a tile: rows of less than 8 MB
-static bool row_ok(int64_t ld) { return ld < (8 << 20); }
+bool row_ok(int64_t ld) { return ld < (8 << 20); }
+
+// ---- operands whose rows are not aligned (an odd width, a view that starts anywhere) are copied once per call into rows padded with zeros to 16 bytes; the few-row form reads them in place.
+// One wave per row, 16 bytes a lane; one launch for all of a call's operands.  (Staging such rows through registers instead: 4999 x 999 -> 515 f16 in training 162 us.)
+struct Copy { const uint8_t *src; uint8_t *dst; int64_t rows, cols, ld; };      // cols: elements, ld: bytes
+struct Copies { Copy c[4]; int n; };
+template <int EB>
+__global__ __launch_bounds__(256) void align_rows_kernel(Copies a) {
+    const int lane = threadIdx.x & 63;
+    int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t waves = (int64_t)gridDim.x * 4;
+    for (int j = 0; j < a.n; ++j) {
+        const Copy &c = a.c[j];
+        for (; w < c.rows; w += waves) {
+            const uint8_t *src = c.src + w * c.cols * EB;
+            uint8_t *dst = c.dst + w * c.ld;
+            for (int64_t k = lane * 16; k < c.ld; k += 1024) {
+                const int64_t left = c.cols * EB - k;
+                uint32_t v[4] = {0, 0, 0, 0};
+                if (left >= 16) __builtin_memcpy(v, src + k, 16);
+                else
+#pragma unroll
+                    for (int e = 0; e < 16; e += EB)
+                        if (e < left) {
+                            uint32_t b = 0;
+                            __builtin_memcpy(&b, src + k + e, EB);
+                            v[e / 4] |= b << (8 * (e & 3));
+                        }
+                *reinterpret_cast<uint4 *>(dst + k) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+        }
+        w -= c.rows;                                                     // the rows of the copies are one sequence
+    }
+}
+int64_t copy_bytes(int64_t rows, int64_t cols, int eb) { return ceil_to(rows * ceil_to(cols * eb, 16), 256); }
+bool unaligned(const void *p, int64_t ld) { return p && !aligned16(p, ld); }
+struct Aligner {
+    uint8_t *at;
+    Copies todo;
+    int eb;
+    // where the operand's copy will be
+    const uint8_t *copy(const void *p, int64_t rows, int64_t cols, int64_t &ld) {
+        ld = ceil_to(cols * eb, 16);
+        uint8_t *dst = at;
+        at += copy_bytes(rows, cols, eb);
+        todo.c[todo.n++] = {(const uint8_t *)p, dst, rows, cols, ld};
+        return dst;
+    }
+    int run(hipStream_t st) const {
+        if (!todo.n) return W3D_OK;
+        int64_t rows = 0;
+        for (int i = 0; i < todo.n; ++i) rows += todo.c[i].rows;
+        const dim3 grid(w3d_grid(rows, 4, 4096)), block(256);
+        if (eb == 4) hipLaunchKernelGGL(align_rows_kernel<4>, grid, block, 0, st, todo);
+        else if (eb == 2) hipLaunchKernelGGL(align_rows_kernel<2>, grid, block, 0, st, todo);
+        else hipLaunchKernelGGL(align_rows_kernel<1>, grid, block, 0, st, todo);
+        W3D_CHECK_LAUNCH();
+        return W3D_OK;
+    }
+};
 
 int forward(const void *x, const int32_t *xs, const void *w, const int32_t *ws, const void *w2, const int32_t *ws2, const void *bias, const void *bias2, int bias_dtype,
             const void *residual, int64_t R, int64_t K, int64_t N, int dtype, int out_dtype, int act, bool gated, void *y, void *workspace, size_t workspace_bytes, hipStream_t st) {
@@ -370,11 +426,11 @@ int forward(const void *x, const int32_t *xs, const void *w, const int32_t *ws, 
     if ((bias || bias2) && bias_dtype != out_dtype && bias_dtype != W3D_DTYPE_F32) return W3D_ERR_ARG;
     if (R == 0) return W3D_OK;
     if (!x || !w || !y || (gated && !w2)) return W3D_ERR_ARG;
-    const int64_t ld = K * eb_of(dtype);
-    if (!row_ok(ld) || !row_ok(N * eb_of(out_dtype))) return W3D_ERR_UNSUPPORTED;
+    const int eb = eb_of(dtype);
+    if (!row_ok(K * eb) || !row_ok(N * eb_of(out_dtype))) return W3D_ERR_UNSUPPORTED;
     GemmArgs a = {};
     a.x = (const uint8_t *)x; a.w = (const uint8_t *)w; a.w2 = (const uint8_t *)w2;
-    a.ldx = a.ldw = ld; a.M = R; a.N = N; a.K = K;
+    a.ldx = a.ldw = K * eb; a.M = R; a.N = N; a.K = K;
     a.bias = (const uint8_t *)bias; a.bias2 = (const uint8_t *)bias2; a.bias_f32 = bias_dtype == W3D_DTYPE_F32 && out_dtype != W3D_DTYPE_F32;
     a.res = (const uint8_t *)residual; a.xs = xs; a.ws = ws; a.ws2 = ws2;
     a.out = (uint8_t *)y; a.ld_out = N * eb_of(out_dtype); a.act = act; a.out_dt = out_dtype;
@@ -388,43 +444,56 @@ int forward(const void *x, const int32_t *xs, const void *w, const int32_t *ws, 
             default: return w3d_lin_skinny_fp8(a, prod, st);
         }
     }
-    const int align = aligned16(x, ld) && aligned16(w, ld) && aligned16(w2, ld) ? 1 + a.vec_io : 0;
-    const Cut c = cut_of(R, N, K, dtype, gated, align, 1);
-    if (c.slices > 1 && (!workspace || (((uintptr_t)workspace) & 15) || workspace_bytes < part_bytes(c, R, N, gated, 1))) return W3D_ERR_WORKSPACE;
-    a.part = (float *)workspace;
-    return run_product(a, prod, dtype, c, align, 1, st);
+    const Cut c = cut_of(R, N, K, dtype, gated, a.vec_io, 1);
+    Aligner al = {(uint8_t *)workspace, {}, eb};
+    // (all operands of one side have one row length: an unaligned second weight matrix takes the first along)
+    const bool ux = unaligned(x, K * eb), uw = unaligned(w, K * eb) || unaligned(w2, K * eb);
+    const int64_t copies = (ux ? copy_bytes(R, K, eb) : 0) + (uw ? (gated ? 2 : 1) * copy_bytes(N, K, eb) : 0);
+    const size_t need = (size_t)copies + part_bytes(c, R, N, gated, 1);
+    if (need && (!workspace || (((uintptr_t)workspace) & 15) || workspace_bytes < need)) return W3D_ERR_WORKSPACE;
+    if (copies) {
+        if (ux) a.x = al.copy(x, R, K, a.ldx);
+        if (uw) { a.w = al.copy(w, N, K, a.ldw); if (gated) a.w2 = al.copy(w2, N, K, a.ldw); }
+        const int rc = al.run(st);
+        if (rc != W3D_OK) return rc;
+    }
+    a.part = (float *)((uint8_t *)workspace + copies);
+    return run_product(a, prod, dtype, c, 1, st);
 }
 
-// the largest of the cuts a call may take (its alignment is not known to the workspace query)
-size_t forward_bytes(int64_t R, int64_t K, int64_t N, int dtype, bool gated) {
+// what a call may need: by its sizes, and for tensors that may start at any element (views) the copies on top
+size_t forward_bytes(int64_t R, int64_t K, int64_t N, int dtype, bool gated, bool views) {
     if (R <= SKINNY_ROWS || K < 1 || N < 1) return 0;
+    const int eb = eb_of(dtype);
     size_t most = 0;
-    for (int align = 0; align < 3; ++align) {
-        const size_t b = part_bytes(cut_of(R, N, K, dtype, gated, align, 1), R, N, gated, 1);
+    for (int vec = 0; vec < 2; ++vec) {
+        const size_t b = part_bytes(cut_of(R, N, K, dtype, gated, vec, 1), R, N, gated, 1);
         most = b > most ? b : most;
     }
-    return most;
+    return most + (views || K * eb % 16 ? (size_t)(copy_bytes(R, K, eb) + (gated ? 2 : 1) * copy_bytes(N, K, eb)) : 0);
 }
 
-// ---- backward.  Workspace: dz | column sums | partial tiles (of one product at a time)
+// ---- backward.  Workspace: aligned copies | dz | column sums | partial tiles (of one product at a time)
 struct Bwd {
     int64_t pad, ld_dz;          // columns of one half of dz, bytes of a row of dz
-    int64_t dz_bytes, strips, colsum_ld, colsum_bytes, part;
+    int64_t copies, dz_bytes, strips, colsum_ld, colsum_bytes, part;
 };
 int64_t max64(int64_t a, int64_t b) { return a > b ? a : b; }
 // strips of partial column sums that the product forming dz writes: one per tile row and row of waves, or the joining launch's
 int64_t strips_of(const Cut &c, int64_t R) { return c.slices > 1 ? (R + JOIN_ROWS - 1) / JOIN_ROWS : c.tiles_m * (c.tile == 64 ? 4 : 2); }
-Bwd bwd_plan(int64_t R, int64_t K, int64_t N, int dtype, bool gated, bool no_act) {
+// cx, cw, cdy: the rows of x, of the weights, of dy (as an operand) are copied
+Bwd bwd_plan(int64_t R, int64_t K, int64_t N, int dtype, bool gated, bool no_act, bool cx, bool cw, bool cdy) {
     Bwd b;
     const int eb = eb_of(dtype), parts = gated ? 2 : 1;
+    b.copies = (cx ? copy_bytes(R, K, eb) : 0) + (cw ? parts * copy_bytes(N, K, eb) : 0) + (cdy ? copy_bytes(R, N, eb) : 0);
     b.pad = ceil_to(N, gated ? 64 : 16 / eb);
     b.ld_dz = b.pad * parts * eb;
     b.dz_bytes = no_act ? 0 : ceil_to(R * b.ld_dz, 256);
     b.colsum_ld = ceil_to(N, 16) * parts;
     b.part = 0;
     b.strips = no_act ? w3d_column_strips(R, N) : 0;
-    for (int al = 0; al < 3; ++al) {
-        const Cut z = cut_of(R, gated ? b.pad : N, K, dtype, gated, al, 1), dx = cut_of(R, K, gated ? 2 * b.pad : N, dtype, false, al, 1), dw = cut_of(N, K, R, dtype, false, al, parts);
+    for (int vec = 0; vec < 2; ++vec) {
+        const Cut z = cut_of(R, gated ? b.pad : N, K, dtype, gated, vec, 1), dx = cut_of(R, K, gated ? 2 * b.pad : N, dtype, false, vec, 1), dw = cut_of(N, K, R, dtype, false, vec, parts);
         if (!no_act) {
             b.strips = max64(b.strips, strips_of(z, R));
             b.part = max64(b.part, (int64_t)part_bytes(z, R, N, gated, 1));
@@ -444,74 +513,80 @@ int backward(const void *x, const void *w, const void *w2, const void *bias, con
     if (!row_ok(K * eb) || !row_ok((N + 64) * eb * parts)) return W3D_ERR_UNSUPPORTED;
     if (R > 0 && (!x || !w || !dy || (gated && !w2))) return W3D_ERR_ARG;
     const bool no_act = !gated && act == ACT_NONE;
-    const Bwd b = bwd_plan(R, K, N, dtype, gated, no_act);
+    const bool cx = R > 0 && (!no_act || dw) && unaligned(x, K * eb), cw = R > 0 && (!no_act || dx) && (unaligned(w, K * eb) || unaligned(w2, K * eb)),
+               cdy = R > 0 && no_act && (dx || dw) && unaligned(dy, N * eb);
+    const Bwd b = bwd_plan(R, K, N, dtype, gated, no_act, cx, cw, cdy);
     uint8_t *ws = (uint8_t *)workspace;
     if (R > 0) {
-        if (b.dz_bytes + b.colsum_bytes + b.part > 0 && (!ws || (((uintptr_t)ws) & 15) || workspace_bytes < (size_t)(b.dz_bytes + b.colsum_bytes + b.part))) return W3D_ERR_WORKSPACE;
+        const size_t need = (size_t)(b.copies + b.dz_bytes + b.colsum_bytes + b.part);
+        if (need && (!ws || (((uintptr_t)ws) & 15) || workspace_bytes < need)) return W3D_ERR_WORKSPACE;
     }
-    float *colsum = (float *)(ws + b.dz_bytes), *part = (float *)(ws + b.dz_bytes + b.colsum_bytes);
-    const uint8_t *dz = (const uint8_t *)dy;
-    int64_t ld_dz = N * eb, strips = 0;
+    uint8_t *dz_buf = ws + b.copies;
+    float *colsum = (float *)(dz_buf + b.dz_bytes), *part = (float *)(dz_buf + b.dz_bytes + b.colsum_bytes);
+    const uint8_t *X = (const uint8_t *)x, *W = (const uint8_t *)w, *W2 = (const uint8_t *)w2, *dz = (const uint8_t *)dy;
+    int64_t ldx = K * eb, ldw = K * eb, ld_dz = N * eb, strips = 0;
+    Aligner al = {ws, {}, eb};
+    if (cx) X = al.copy(x, R, K, ldx);
+    if (cw) { W = al.copy(w, N, K, ldw); if (gated) W2 = al.copy(w2, N, K, ldw); }
+    if (cdy) dz = al.copy(dy, R, N, ld_dz);
+    int rc = al.run(st);
+    if (rc != W3D_OK) return rc;
     if (R > 0 && !no_act) {
         GemmArgs a = {};
-        a.x = (const uint8_t *)x; a.w = (const uint8_t *)w; a.w2 = (const uint8_t *)w2;
-        a.ldx = a.ldw = K * eb; a.M = R; a.N = N; a.K = K;
+        a.x = X; a.w = W; a.w2 = W2; a.ldx = ldx; a.ldw = ldw; a.M = R; a.N = N; a.K = K;
         a.bias = (const uint8_t *)bias; a.bias2 = (const uint8_t *)bias2; a.bias_f32 = bias_dtype == W3D_DTYPE_F32 && dtype != W3D_DTYPE_F32;
-        a.dy = (const uint8_t *)dy; a.out = ws; a.ld_out = b.ld_dz; a.half_out = b.pad * eb; a.act = act; a.out_dt = dtype;
-        a.vec_io = aligned16(dy, N * eb);
+        a.dy = (const uint8_t *)dy; a.out = dz_buf; a.ld_out = b.ld_dz; a.half_out = b.pad * eb; a.act = act; a.out_dt = dtype;
+        a.vec_io = aligned16(dy, N * eb) ? 1 : 0;
         a.colsum = db || db2 ? colsum : nullptr; a.colsum_ld = b.colsum_ld; a.part = part;
-        const int al = aligned16(x, K * eb) && aligned16(w, K * eb) && aligned16(w2, K * eb) ? 1 + a.vec_io : 0;
-        const Cut c = cut_of(R, gated ? b.pad : N, K, dtype, gated, al, 1);                   // (the tiles write the padding columns too)
-        const int rc = run_product(a, gated ? PROD_GATED_BWD : PROD_LINEAR_BWD, dtype, c, al, 1, st);
+        const Cut c = cut_of(R, gated ? b.pad : N, K, dtype, gated, a.vec_io, 1);              // (the tiles write the padding columns too)
+        rc = run_product(a, gated ? PROD_GATED_BWD : PROD_LINEAR_BWD, dtype, c, 1, st);
         if (rc != W3D_OK) return rc;
         strips = strips_of(c, R);
-        dz = ws; ld_dz = b.ld_dz;
+        dz = dz_buf; ld_dz = b.ld_dz;
     } else if (R > 0 && db) {
-        const int rc = w3d_column_sums(dy, R, N, dtype, colsum, b.colsum_ld, st);
+        rc = w3d_column_sums(dy, R, N, dtype, colsum, b.colsum_ld, st);
         if (rc != W3D_OK) return rc;
         strips = b.strips;
     }
-    if (db) { const int rc = w3d_fold_columns(colsum, (int)strips, b.colsum_ld, N, db, bias_dtype, st); if (rc != W3D_OK) return rc; }
-    if (db2) { const int rc = w3d_fold_columns(colsum + b.colsum_ld / 2, (int)strips, b.colsum_ld, N, db2, bias_dtype, st); if (rc != W3D_OK) return rc; }
+    if (db) { rc = w3d_fold_columns(colsum, (int)strips, b.colsum_ld, N, db, bias_dtype, st); if (rc != W3D_OK) return rc; }
+    if (db2) { rc = w3d_fold_columns(colsum + b.colsum_ld / 2, (int)strips, b.colsum_ld, N, db2, bias_dtype, st); if (rc != W3D_OK) return rc; }
     if (dx && R > 0) {
         GemmArgs a = {};
-        a.x = dz; a.ldx = ld_dz; a.w = (const uint8_t *)w; a.w2 = (const uint8_t *)w2; a.ldw = K * eb;
+        a.x = dz; a.ldx = ld_dz; a.w = W; a.w2 = W2; a.ldw = ldw;
         a.M = R; a.N = K; a.K = gated ? 2 * b.pad : N; a.k_split = gated ? b.pad : 0; a.w_rows = N;
         a.out = (uint8_t *)dx; a.ld_out = K * eb; a.out_dt = dtype; a.part = part;
-        a.vec_io = aligned16(dx, K * eb);
-        const int al = aligned16(dz, ld_dz) && aligned16(w, K * eb) && aligned16(w2, K * eb) ? 1 + a.vec_io : 0;
-        const int rc = run_product(a, PROD_DX, dtype, cut_of(R, K, a.K, dtype, false, al, 1), al, 1, st);
+        a.vec_io = aligned16(dx, K * eb) ? 1 : 0;
+        rc = run_product(a, PROD_DX, dtype, cut_of(R, K, a.K, dtype, false, a.vec_io, 1), 1, st);
         if (rc != W3D_OK) return rc;
     }
     // weight gradients: the two halves of a gated layer are one launch (blockIdx.z) when both are wanted
     const bool both = dw && dw2;
     for (int h = 0; h < 2; ++h) {
         void *o = h ? dw2 : dw;
-        if (!o || (both && h)) continue;
+        if (!o || (both && h && R > 0)) continue;
         if (R == 0) {
-            const int z = w3d_fold_columns(nullptr, 0, 0, N * K, o, dtype, st);
-            if (z != W3D_OK) return z;
-            if (both) { const int z2 = w3d_fold_columns(nullptr, 0, 0, N * K, dw2, dtype, st); if (z2 != W3D_OK) return z2; }
+            rc = w3d_fold_columns(nullptr, 0, 0, N * K, o, dtype, st);
+            if (rc != W3D_OK) return rc;
             continue;
         }
         GemmArgs a = {};
-        a.x = dz + (h ? b.pad * eb : 0); a.ldx = ld_dz; a.w = (const uint8_t *)x; a.ldw = K * eb;
+        a.x = dz + (h ? b.pad * eb : 0); a.ldx = ld_dz; a.w = X; a.ldw = ldx;
         a.M = N; a.N = K; a.K = R; a.w_rows = R; a.z_x = b.pad * eb;
         a.out = (uint8_t *)o; a.out2 = (uint8_t *)dw2; a.ld_out = K * eb; a.out_dt = dtype; a.part = part;
-        a.vec_io = aligned16(o, K * eb) && aligned16(both ? dw2 : nullptr, 0);
-        const int al = aligned16(a.x, ld_dz) && aligned16(x, K * eb) ? 1 + a.vec_io : 0;
-        const int rc = run_product(a, PROD_DW, dtype, cut_of(N, K, R, dtype, false, al, parts), al, both ? 2 : 1, st);
+        a.vec_io = aligned16(o, K * eb) && aligned16(both ? dw2 : nullptr, 0) ? 1 : 0;
+        rc = run_product(a, PROD_DW, dtype, cut_of(N, K, R, dtype, false, a.vec_io, parts), both ? 2 : 1, st);
         if (rc != W3D_OK) return rc;
     }
     return W3D_OK;
 }
 }  // namespace
 
-extern "C" size_t w3d_linear_workspace_bytes(int64_t R, int64_t K, int64_t N, int dtype, int gated) { return R < 1 ? 0 : forward_bytes(R, K, N, dtype, gated != 0); }
-extern "C" size_t w3d_linear_bwd_workspace_bytes(int64_t R, int64_t K, int64_t N, int dtype, int act, int gated) {
+extern "C" size_t w3d_linear_workspace_bytes(int64_t R, int64_t K, int64_t N, int dtype, int gated, int views) { return R < 1 ? 0 : forward_bytes(R, K, N, dtype, gated != 0, views != 0); }
+extern "C" size_t w3d_linear_bwd_workspace_bytes(int64_t R, int64_t K, int64_t N, int dtype, int act, int gated, int views) {
     if (R < 1 || K < 1 || N < 1) return 0;
-    const Bwd b = bwd_plan(R, K, N, dtype, gated != 0, !gated && act == ACT_NONE);
-    return (size_t)(b.dz_bytes + b.colsum_bytes + b.part);
+    const bool no_act = !gated && act == ACT_NONE, ck = views || K * eb_of(dtype) % 16, cn = views || N * eb_of(dtype) % 16;
+    const Bwd b = bwd_plan(R, K, N, dtype, gated != 0, no_act, ck, ck, no_act && cn);
+    return (size_t)(b.copies + b.dz_bytes + b.colsum_bytes + b.part);
 }
 extern "C" int w3d_linear_fwd(const void *x, const void *w, const void *bias, int bias_dtype, const void *residual, int64_t R, int64_t K, int64_t N, int dtype, int act, void *y,
                               void *workspace, size_t workspace_bytes, w3d_stream_t stream) {

@@ -1461,6 +1461,14 @@ def _scratch(nbytes: int, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
+def _views(*tensors) -> int:
+    """Does one of the tensors start off a 16-byte boundary (a slice of something)?  The library then copies it."""
+    for t in tensors:
+        if t.data_ptr() & 15:
+            return 1
+    return 0
+
+
 def _wants_grad(*tensors) -> bool:
     if torch.is_grad_enabled():
         for t in tensors:
@@ -1558,7 +1566,7 @@ def raw_linear(x, w, bias, residual, act: int, y):
     """y [..., N] = act(x [..., K] w [N,K]^T + bias) + residual, contiguous."""
     N, K = w.shape
     R, dt = x.numel() // K, _code(x)
-    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, dt, 0)
+    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, dt, 0, _views(x, w))
     _launch("w3d_linear_fwd", x.device, lib().w3d_linear_fwd, x, w, bias, _code(bias), residual, R, K, N, dt, act, y, _scratch(nbytes, x.device), nbytes)
 
 
@@ -1566,7 +1574,7 @@ def raw_gated_linear(x, wg, wu, bg, bu, act: int, y):
     """y [..., N] = act(x wg^T + bg) * (x wu^T + bu), contiguous."""
     N, K = wg.shape
     R, dt = x.numel() // K, _code(x)
-    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, dt, 1)
+    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, dt, 1, _views(x, wg, wu))
     _launch("w3d_gated_linear_fwd", x.device, lib().w3d_gated_linear_fwd, x, wg, wu, bg, bu, _code(bg if bg is not None else bu), R, K, N, dt, act, y, _scratch(nbytes, x.device), nbytes)
 
 
@@ -1592,9 +1600,9 @@ class _Linear(torch.autograd.Function):
         if R == 0:
             dw, db = (t.zero_() if t is not None else None for t in (dw, db))
         elif want_x or want_w or want_b:
-            dt = _code(x)
-            nbytes = lib().w3d_linear_bwd_workspace_bytes(R, K, N, dt, ctx.act, 0)
-            _launch("w3d_linear_bwd", x.device, lib().w3d_linear_bwd, x, w, bias, _code(bias), gy.contiguous(), R, K, N, dt, ctx.act, dx, dw, db, _scratch(nbytes, x.device), nbytes)
+            dt, gyc = _code(x), gy.contiguous()
+            nbytes = lib().w3d_linear_bwd_workspace_bytes(R, K, N, dt, ctx.act, 0, _views(x, w, gyc))
+            _launch("w3d_linear_bwd", x.device, lib().w3d_linear_bwd, x, w, bias, _code(bias), gyc, R, K, N, dt, ctx.act, dx, dw, db, _scratch(nbytes, x.device), nbytes)
         return dx, dw, db, gy if want_r else None, None
 
 
@@ -1643,7 +1651,7 @@ class _GatedLinear(torch.autograd.Function):
             grads = [t.zero_() if t is not None else None for t in grads]
         else:
             dt = _code(x)
-            nbytes = lib().w3d_linear_bwd_workspace_bytes(R, K, N, dt, ctx.act, 1)
+            nbytes = lib().w3d_linear_bwd_workspace_bytes(R, K, N, dt, ctx.act, 1, _views(x, wg, wu))
             _launch("w3d_gated_linear_bwd", x.device, lib().w3d_gated_linear_bwd, x, wg, wu, bg, bu, _code(bg if bg is not None else bu), gy.contiguous(), R, K, N, dt, ctx.act, *grads,
                     _scratch(nbytes, x.device), nbytes)
         return (*grads, None)
@@ -1704,7 +1712,7 @@ def linear_fp8(q, scale, weight_q, weight_scale, bias=None, activation=None, res
     if residual is not None:
         residual = _head_arg("linear_fp8", "residual", residual, (R, N), out_dtype, dev)
     y = torch.empty(R, N, dtype=out_dtype, device=dev)
-    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, FP8, 0)
+    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, FP8, 0, _views(q, weight_q))
     _launch("w3d_linear_fp8_fwd", dev, lib().w3d_linear_fp8_fwd, q, scale, weight_q, weight_scale, bias, _code(bias), residual, R, K, N, code, act, y, _scratch(nbytes, dev), nbytes)
     return y
 
@@ -1719,7 +1727,7 @@ def gated_linear_fp8(q, scale, gate_q, gate_scale, up_q, up_scale, b_gate=None, 
     N, gate_q, up_q, b_gate, b_up = _gated_args("gated_linear_fp8", q, gate_q, up_q, b_gate, b_up, torch.uint8, out_dtype)
     R, K = q.shape
     y = torch.empty(R, N, dtype=out_dtype, device=dev)
-    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, FP8, 1)
+    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, FP8, 1, _views(q, gate_q, up_q))
     _launch("w3d_gated_linear_fp8_fwd", dev, lib().w3d_gated_linear_fp8_fwd, q, scale, gate_q, gate_scale, up_q, up_scale, b_gate, b_up, _code(b_gate if b_gate is not None else b_up), R, K, N,
             code, act, y, _scratch(nbytes, dev), nbytes)
     return y
