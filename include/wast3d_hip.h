@@ -644,8 +644,9 @@ int w3d_rms_norm_bwd(const void *x, const void *residual, const void *weight, in
  * Gated linear layer: y = act(x Wg^T + bg) * (x Wu^T + bu), one launch for both products.
  * act: W3D_ACT_*; gelu is z * Phi(z).  Rows of x, w and y shorter than 8 MB (W3D_ERR_UNSUPPORTED otherwise).
  * The _fp8 forms take e4m3 rows with one E8M0 exponent (1..254) each for x AND the weights, and write bf16 or f16 (residual and biases of out_dtype, biases also f32).
- * The _bwd forms need the forward's inputs (they form z again) and dy [R,N]: dx [R,K], dw [N,K], dbias [N] (of bias_dtype), each optional; the residual's gradient is dy itself.
- * workspace: w3d_linear_workspace_bytes (dtype W3D_DTYPE_FP8_E4M3 for the _fp8 forms) / w3d_linear_bwd_workspace_bytes; views: 1 if x, a weight matrix or dy may start at an address that
+ * W3D_DTYPE_F32 forward calls can keep the values before the activation: z, f32 [R][w3d_linear_z_stride(N, gated)], 16-byte aligned, or NULL (always, for 16-bit rows).
+ * The _bwd forms need the forward's inputs and dy [R,N]; 16-bit ones form z again (z NULL), f32 ones take the z that was kept (unless act is W3D_ACT_NONE in a linear layer): dx [R,K], dw [N,K], dbias [N] (of bias_dtype), each optional; the residual's gradient is dy itself.
+ * workspace: w3d_linear_workspace_bytes (dtype W3D_DTYPE_FP8_E4M3 for the _fp8 forms) / w3d_linear_bwd_workspace_bytes (kept: 1 if z is passed); views: 1 if x, a weight matrix or dy may start at an address that
  * is no multiple of 16 (room for aligned copies; widths that are no multiple of 16 bytes get theirs without it). */
 #define W3D_ACT_NONE 0
 #define W3D_ACT_RELU 1
@@ -653,20 +654,21 @@ int w3d_rms_norm_bwd(const void *x, const void *residual, const void *weight, in
 #define W3D_ACT_SILU 3
 #define W3D_ACT_SIGMOID 4
 size_t w3d_linear_workspace_bytes(int64_t R, int64_t K, int64_t N, int dtype, int gated, int views);
-size_t w3d_linear_bwd_workspace_bytes(int64_t R, int64_t K, int64_t N, int dtype, int act, int gated, int views);
+size_t w3d_linear_bwd_workspace_bytes(int64_t R, int64_t K, int64_t N, int dtype, int act, int gated, int kept, int views);
+int64_t w3d_linear_z_stride(int64_t N, int gated);
 int w3d_linear_fwd(const void *x, const void *w, const void *bias, int bias_dtype, const void *residual, int64_t R, int64_t K, int64_t N, int dtype, int act, void *y,
-                   void *workspace, size_t workspace_bytes, w3d_stream_t stream);
+                   float *z, void *workspace, size_t workspace_bytes, w3d_stream_t stream);
 int w3d_linear_fp8_fwd(const void *x, const int32_t *x_scale, const void *w, const int32_t *w_scale, const void *bias, int bias_dtype, const void *residual, int64_t R, int64_t K,
                        int64_t N, int out_dtype, int act, void *y, void *workspace, size_t workspace_bytes, w3d_stream_t stream);
-int w3d_linear_bwd(const void *x, const void *w, const void *bias, int bias_dtype, const void *dy, int64_t R, int64_t K, int64_t N, int dtype, int act, void *dx, void *dw,
-                   void *dbias, void *workspace, size_t workspace_bytes, w3d_stream_t stream);
+int w3d_linear_bwd(const void *x, const void *w, const void *bias, int bias_dtype, const void *dy, const float *z, int64_t R, int64_t K, int64_t N, int dtype, int act, void *dx,
+                   void *dw, void *dbias, void *workspace, size_t workspace_bytes, w3d_stream_t stream);
 int w3d_gated_linear_fwd(const void *x, const void *w_gate, const void *w_up, const void *b_gate, const void *b_up, int bias_dtype, int64_t R, int64_t K, int64_t N, int dtype,
-                         int act, void *y, void *workspace, size_t workspace_bytes, w3d_stream_t stream);
+                         int act, void *y, float *z, void *workspace, size_t workspace_bytes, w3d_stream_t stream);
 int w3d_gated_linear_fp8_fwd(const void *x, const int32_t *x_scale, const void *w_gate, const int32_t *gate_scale, const void *w_up, const int32_t *up_scale, const void *b_gate,
                              const void *b_up, int bias_dtype, int64_t R, int64_t K, int64_t N, int out_dtype, int act, void *y, void *workspace, size_t workspace_bytes,
                              w3d_stream_t stream);
-int w3d_gated_linear_bwd(const void *x, const void *w_gate, const void *w_up, const void *b_gate, const void *b_up, int bias_dtype, const void *dy, int64_t R, int64_t K, int64_t N,
-                         int dtype, int act, void *dx, void *dw_gate, void *dw_up, void *db_gate, void *db_up, void *workspace, size_t workspace_bytes, w3d_stream_t stream);
+int w3d_gated_linear_bwd(const void *x, const void *w_gate, const void *w_up, const void *b_gate, const void *b_up, int bias_dtype, const void *dy, const float *z, int64_t R, int64_t K,
+                         int64_t N, int dtype, int act, void *dx, void *dw_gate, void *dw_up, void *db_gate, void *db_up, void *workspace, size_t workspace_bytes, w3d_stream_t stream);
 
 /* GaussianRasterizer.markVisible (RAST/diff_gaussian_rasterization/__init__.py:192-201) */
 int w3d_mark_visible(const float *means3D, const float *viewmatrix, const float *projmatrix, int P,

@@ -152,13 +152,14 @@ SIGNATURES = {
     "w3d_rms_norm_bwd_workspace_bytes": (sz, [i64, i32]),
     "w3d_rms_norm_bwd": (i32, [vp, vp, vp, i32, vp, vp, vp, i64, i32, i32, vp, vp, vp, sz, vp]),
     "w3d_linear_workspace_bytes": (sz, [i64, i64, i64, i32, i32, i32]),
-    "w3d_linear_bwd_workspace_bytes": (sz, [i64, i64, i64, i32, i32, i32, i32]),
-    "w3d_linear_fwd": (i32, [vp, vp, vp, i32, vp, i64, i64, i64, i32, i32, vp, vp, sz, vp]),
+    "w3d_linear_bwd_workspace_bytes": (sz, [i64, i64, i64, i32, i32, i32, i32, i32]),
+    "w3d_linear_z_stride": (i64, [i64, i32]),
+    "w3d_linear_fwd": (i32, [vp, vp, vp, i32, vp, i64, i64, i64, i32, i32, vp, vp, vp, sz, vp]),
     "w3d_linear_fp8_fwd": (i32, [vp, vp, vp, vp, vp, i32, vp, i64, i64, i64, i32, i32, vp, vp, sz, vp]),
-    "w3d_linear_bwd": (i32, [vp, vp, vp, i32, vp, i64, i64, i64, i32, i32, vp, vp, vp, vp, sz, vp]),
-    "w3d_gated_linear_fwd": (i32, [vp, vp, vp, vp, vp, i32, i64, i64, i64, i32, i32, vp, vp, sz, vp]),
+    "w3d_linear_bwd": (i32, [vp, vp, vp, i32, vp, vp, i64, i64, i64, i32, i32, vp, vp, vp, vp, sz, vp]),
+    "w3d_gated_linear_fwd": (i32, [vp, vp, vp, vp, vp, i32, i64, i64, i64, i32, i32, vp, vp, vp, sz, vp]),
     "w3d_gated_linear_fp8_fwd": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, i64, i64, i64, i32, i32, vp, vp, sz, vp]),
-    "w3d_gated_linear_bwd": (i32, [vp, vp, vp, vp, vp, i32, vp, i64, i64, i64, i32, i32, vp, vp, vp, vp, vp, vp, sz, vp]),
+    "w3d_gated_linear_bwd": (i32, [vp, vp, vp, vp, vp, i32, vp, vp, i64, i64, i64, i32, i32, vp, vp, vp, vp, vp, vp, sz, vp]),
     "w3d_mark_visible": (i32, [vp, vp, vp, i32, vp, vp]),
     "w3d_activations_fwd": (i32, [vp, vp, vp, i32, vp, vp, vp, vp]),
     "w3d_activations_bwd": (i32, [vp, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp]),

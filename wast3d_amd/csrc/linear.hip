@@ -5,9 +5,9 @@
 //   * tiles of 256 x 256 (gemm_pipe.h), 128 x 128 or 64 x 64 (gemm_tile.h) through LDS
 //   * when the tiles are few for 256 CUs the contraction is cut into slices; partial tiles are added in slice order, and the epilogue applied, by a second launch
 //
-// Backward keeps nothing of the forward pass but its inputs: z is formed again and turned into dz in the epilogue, where the column sums for the bias
+// Backward keeps nothing of a 16-bit forward pass but its inputs: z is formed again and turned into dz in the epilogue, where the column sums for the bias
 // gradient are taken too — storing z in 16 bits would put its rounding into every gradient, storing it in 32 costs more traffic than forming it again
-// (R x N x 12 bytes written and read, against 2 R N K operations).  dz is rounded once to the operands' type (it is an operand of two products); sums are f32.
+// (R x N x 12 bytes written and read, against 2 R N K operations).  An f32 forward pass keeps z (at a tenth of the 16-bit rate forming it again is the dearer way).  dz is rounded once to the operands' type (it is an operand of two products); sums are f32.
 //
 // One translation unit per operand type (W3D_LIN_DT: the tiles), one for the entry points.
 #include "gemm_pipe.h"
@@ -66,10 +66,15 @@ int launch_prod(const GemmArgs &a, int prod, int tile, int z, hipStream_t st) {
     }
     if constexpr (W3D_LIN_DT != W3D_DTYPE_FP8_E4M3) {
         switch (prod) {
-            case PROD_LINEAR_BWD: return launch_shape<K_ROWS, K_ROWS, EPI_LINEAR_BWD>(a, tile, z, st);
-            case PROD_GATED_BWD: return launch_shape<K_ROWS, K_ROWS, EPI_GATED_BWD>(a, tile, z, st);
             case PROD_DX: return launch_shape<K_ROWS, M_ROWS, EPI_STORE>(a, tile, z, st);
             case PROD_DW: return launch_shape<M_ROWS, M_ROWS, EPI_STORE>(a, tile, z, st);
+            default: break;
+        }
+    }
+    if constexpr (W3D_LIN_DT == W3D_DTYPE_BF16 || W3D_LIN_DT == W3D_DTYPE_F16) {
+        switch (prod) {
+            case PROD_LINEAR_BWD: return launch_shape<K_ROWS, K_ROWS, EPI_LINEAR_BWD>(a, tile, z, st);
+            case PROD_GATED_BWD: return launch_shape<K_ROWS, K_ROWS, EPI_GATED_BWD>(a, tile, z, st);
             default: break;
         }
     }
@@ -169,8 +174,10 @@ __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
                     v[e] = __builtin_ldexpf(v[e], a.xs[m] + a.ws[c + e] - 254);
                     if (GATED) u[e] = __builtin_ldexpf(u[e], a.xs[m] + a.ws2[c + e] - 254);
                 }
-                float y = act_fwd<ACT>(v[e] + bias_at<OT>(a.bias, a.bias_f32, c + e, a.N));
-                if (GATED) y *= u[e] + bias_at<OT>(a.bias2, a.bias_f32, c + e, a.N);
+                const float z = v[e] + bias_at<OT>(a.bias, a.bias_f32, c + e, a.N), z2 = GATED ? u[e] + bias_at<OT>(a.bias2, a.bias_f32, c + e, a.N) : 0.f;
+                if (DT == W3D_DTYPE_F32 && a.z) { a.z[m * a.part_ld + c + e] = z; if (GATED) a.z[m * a.part_ld + a.part_ld / 2 + c + e] = z2; }
+                float y = act_fwd<ACT>(z);
+                if (GATED) y *= z2;
                 else if (a.res) y += load1<OT>(a.res + (m * a.N + c + e) * OB);
                 store1<OT>(a.out + m * a.ld_out + (c + e) * OB, y);
             }
@@ -211,8 +218,8 @@ int W3D_LIN_NAME(w3d_lin_skinny)(const GemmArgs &a, int prod, hipStream_t st) {
 
 namespace {
 
-// Partial sums of a sliced product: part[slice][m][ld] -> the epilogue of the product.  A block takes 64 columns of a strip of JOIN_ROWS rows, four rows at a time (one per wave), so that
-// the column sums of dz are complete per strip; the slices' loads are independent.
+// Partial sums of a sliced product: part[slice][m][ld] -> the epilogue of the product (one slice: the values before the activation that an f32 forward pass kept, for the gradient's).  A block
+// takes 64 columns of a strip of rows (a multiple of JOIN_ROWS), four rows at a time (one per wave), so that the column sums of dz are complete per strip; the slices' loads are independent.
 constexpr int JOIN_ROWS = 16;
 template <int OT, int EPI>
 __global__ __launch_bounds__(256) void join_slices_kernel(GemmArgs a) {
@@ -220,18 +227,20 @@ __global__ __launch_bounds__(256) void join_slices_kernel(GemmArgs a) {
     constexpr bool GATED = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
     __shared__ float sums[2][4][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t n = (int64_t)blockIdx.x * 64 + lane, r0 = (int64_t)blockIdx.y * JOIN_ROWS;
+    const int64_t n = (int64_t)blockIdx.x * 64 + lane, r_end = min(a.M, ((int64_t)blockIdx.y + 1) * a.strip);
     const int64_t pad = EPI == EPI_LINEAR_BWD ? a.ld_out / OB : EPI == EPI_GATED_BWD ? a.half_out / OB : a.N;
     const bool in = n < a.N, store = n < pad;
     const float b0 = bias_at<OT>(a.bias, a.bias_f32, n, a.N), b1 = GATED ? bias_at<OT>(a.bias2, a.bias_f32, n, a.N) : 0.f;
     const int s0 = a.ws && in ? a.ws[n] - 254 : 0, s1 = GATED && a.ws2 && in ? a.ws2[n] - 254 : 0;
     const int64_t z = blockIdx.z, slice = a.M * a.part_ld;
+    float c0 = 0.f, c1 = 0.f;
+    for (int64_t r0 = (int64_t)blockIdx.y * a.strip; r0 < r_end; r0 += JOIN_ROWS) {
     float v[JOIN_ROWS / 4], u[JOIN_ROWS / 4];
 #pragma unroll
     for (int i = 0; i < JOIN_ROWS / 4; ++i) {
         v[i] = u[i] = 0.f;
         const int64_t m = r0 + 4 * i + wave;
-        if (!in || m >= a.M) continue;
+        if (!in || m >= r_end) continue;
         const float *p = a.part + (z * a.slices * a.M + m) * a.part_ld + n;
         for (int s = 0; s < a.slices; ++s) {
             v[i] += p[s * slice];
@@ -240,14 +249,14 @@ __global__ __launch_bounds__(256) void join_slices_kernel(GemmArgs a) {
     }
     with_act(a.act, [&](auto act_c) {
         constexpr int ACT = decltype(act_c)::value;
-        float c0 = 0.f, c1 = 0.f;
 #pragma unroll
         for (int i = 0; i < JOIN_ROWS / 4; ++i) {
             const int64_t m = r0 + 4 * i + wave;
-            if (!store || m >= a.M) continue;
+            if (!store || m >= r_end) continue;
             float x = v[i], y = u[i];
             if (a.xs) { x = __builtin_ldexpf(x, a.xs[m] + s0); if (GATED) y = __builtin_ldexpf(y, a.xs[m] + s1); }
             x += b0; y += b1;
+            if (OT == W3D_DTYPE_F32 && (EPI == EPI_LINEAR || EPI == EPI_GATED) && a.z && in) { a.z[m * a.part_ld + n] = x; if (GATED) a.z[m * a.part_ld + a.part_ld / 2 + n] = y; }
             uint8_t *o = (EPI == EPI_STORE && z ? a.out2 : a.out) + m * a.ld_out + n * OB;
             if (EPI == EPI_STORE) store1<OT>(o, x);
             else if (EPI == EPI_LINEAR) {
@@ -265,20 +274,23 @@ __global__ __launch_bounds__(256) void join_slices_kernel(GemmArgs a) {
                 c0 += x;
             }
         }
-        if ((EPI == EPI_LINEAR_BWD || EPI == EPI_GATED_BWD) && a.colsum) {
-            sums[0][wave][lane] = c0;
-            if (GATED) sums[1][wave][lane] = c1;
-            __syncthreads();
-            if (wave < (GATED ? 2 : 1) && in)
-                a.colsum[(int64_t)blockIdx.y * a.colsum_ld + wave * (a.colsum_ld / 2) + n] = (sums[wave][0][lane] + sums[wave][1][lane]) + (sums[wave][2][lane] + sums[wave][3][lane]);
-        }
     });
+    }
+    if ((EPI == EPI_LINEAR_BWD || EPI == EPI_GATED_BWD) && a.colsum) {
+        sums[0][wave][lane] = c0;
+        if (GATED) sums[1][wave][lane] = c1;
+        __syncthreads();
+        if (wave < (GATED ? 2 : 1) && in)
+            a.colsum[(int64_t)blockIdx.y * a.colsum_ld + wave * (a.colsum_ld / 2) + n] = (sums[wave][0][lane] + sums[wave][1][lane]) + (sums[wave][2][lane] + sums[wave][3][lane]);
+    }
 }
+// rows of a strip: JOIN_ROWS, more where the strips would be over 1 024
+int64_t strip_rows(int64_t M) { return (M / 1024 + JOIN_ROWS) / JOIN_ROWS * JOIN_ROWS; }
 template <int OT>
-int join_as(const GemmArgs &a, int prod, int z, hipStream_t st) {
+int join_as(GemmArgs a, int prod, int z, hipStream_t st) {
     const int64_t cols = prod == PROD_LINEAR_BWD ? a.ld_out / Elem<OT>::B : prod == PROD_GATED_BWD ? a.half_out / Elem<OT>::B : a.N;
-    const int64_t strips = (a.M + JOIN_ROWS - 1) / JOIN_ROWS;
-    if (strips > 65535) return W3D_ERR_UNSUPPORTED;                      // (sliced products have few tiles: see cut_of)
+    a.strip = strip_rows(a.M);
+    const int64_t strips = (a.M + a.strip - 1) / a.strip;
     const dim3 grid((unsigned)((cols + 63) / 64), (unsigned)strips, z), block(256);
     switch (prod) {
         case PROD_LINEAR: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_LINEAR>), grid, block, 0, st, a); break;
@@ -338,11 +350,21 @@ size_t part_bytes(const Cut &c, int64_t M, int64_t N, bool gated, int batch) {
     return c.slices > 1 ? (size_t)batch * c.slices * M * ceil_to(N, 16) * (gated ? 2 : 1) * 4 : 0;
 }
 
+// floats of a row of partial sums, or of kept values before the activation
+int64_t z_stride(int64_t N, bool gated) { return ceil_to(N, 16) * (gated ? 2 : 1); }
+// the second launch of a sliced product, or of a gradient whose z was kept
+int join(const GemmArgs &a, int prod, int z, hipStream_t st) {
+    switch (a.out_dt) {
+        case W3D_DTYPE_F32: return join_as<W3D_DTYPE_F32>(a, prod, z, st);
+        case W3D_DTYPE_BF16: return join_as<W3D_DTYPE_BF16>(a, prod, z, st);
+        default: return join_as<W3D_DTYPE_F16>(a, prod, z, st);
+    }
+}
 int run_product(GemmArgs &a, int prod, int dtype, const Cut &c, int z, hipStream_t st) {
     a.slices = c.slices;
     if (c.tiles_m > 0x7fffffff || c.tiles_n > 0x7fffffff) return W3D_ERR_UNSUPPORTED;
     a.tiles_m = (int)c.tiles_m; a.tiles_n = (int)c.tiles_n;
-    a.part_ld = ceil_to(a.N, 16) * (prod == PROD_GATED || prod == PROD_GATED_BWD ? 2 : 1);
+    a.part_ld = z_stride(a.N, prod == PROD_GATED || prod == PROD_GATED_BWD);
     int rc;
     switch (dtype) {
         case W3D_DTYPE_F32: rc = w3d_lin_tiles_f32(a, prod, c.tile, z, st); break;
@@ -350,12 +372,7 @@ int run_product(GemmArgs &a, int prod, int dtype, const Cut &c, int z, hipStream
         case W3D_DTYPE_F16: rc = w3d_lin_tiles_f16(a, prod, c.tile, z, st); break;
         default: rc = w3d_lin_tiles_fp8(a, prod, c.tile, z, st); break;
     }
-    if (rc != W3D_OK || c.slices == 1) return rc;
-    switch (a.out_dt) {
-        case W3D_DTYPE_F32: return join_as<W3D_DTYPE_F32>(a, prod, z, st);
-        case W3D_DTYPE_BF16: return join_as<W3D_DTYPE_BF16>(a, prod, z, st);
-        default: return join_as<W3D_DTYPE_F16>(a, prod, z, st);
-    }
+    return rc != W3D_OK || c.slices == 1 ? rc : join(a, prod, z, st);
 }
 
 // 32-bit offsets inside a tile: rows of less than 8 MB
@@ -421,11 +438,11 @@ struct Aligner {
 };
 
 int forward(const void *x, const int32_t *xs, const void *w, const int32_t *ws, const void *w2, const int32_t *ws2, const void *bias, const void *bias2, int bias_dtype,
-            const void *residual, int64_t R, int64_t K, int64_t N, int dtype, int out_dtype, int act, bool gated, void *y, void *workspace, size_t workspace_bytes, hipStream_t st) {
+            const void *residual, int64_t R, int64_t K, int64_t N, int dtype, int out_dtype, int act, bool gated, void *y, float *z, void *workspace, size_t workspace_bytes, hipStream_t st) {
     if (R < 0 || K < 1 || N < 1 || act < 0 || act > ACT_SIGMOID || !float_dtype(out_dtype)) return W3D_ERR_ARG;
     if ((bias || bias2) && bias_dtype != out_dtype && bias_dtype != W3D_DTYPE_F32) return W3D_ERR_ARG;
     if (R == 0) return W3D_OK;
-    if (!x || !w || !y || (gated && !w2)) return W3D_ERR_ARG;
+    if (!x || !w || !y || (gated && !w2) || (z && (dtype != W3D_DTYPE_F32 || ((uintptr_t)z & 15)))) return W3D_ERR_ARG;
     const int eb = eb_of(dtype);
     if (!row_ok(K * eb) || !row_ok(N * eb_of(out_dtype))) return W3D_ERR_UNSUPPORTED;
     GemmArgs a = {};
@@ -433,7 +450,7 @@ int forward(const void *x, const int32_t *xs, const void *w, const int32_t *ws, 
     a.ldx = a.ldw = K * eb; a.M = R; a.N = N; a.K = K;
     a.bias = (const uint8_t *)bias; a.bias2 = (const uint8_t *)bias2; a.bias_f32 = bias_dtype == W3D_DTYPE_F32 && out_dtype != W3D_DTYPE_F32;
     a.res = (const uint8_t *)residual; a.xs = xs; a.ws = ws; a.ws2 = ws2;
-    a.out = (uint8_t *)y; a.ld_out = N * eb_of(out_dtype); a.act = act; a.out_dt = out_dtype;
+    a.out = (uint8_t *)y; a.ld_out = N * eb_of(out_dtype); a.act = act; a.out_dt = out_dtype; a.z = z; a.part_ld = z_stride(N, gated);
     a.vec_io = aligned16(y, a.ld_out) && aligned16(residual, 0) ? 1 : 0;
     const int prod = gated ? PROD_GATED : PROD_LINEAR;
     if (R <= SKINNY_ROWS) {
@@ -480,9 +497,10 @@ struct Bwd {
 };
 int64_t max64(int64_t a, int64_t b) { return a > b ? a : b; }
 // strips of partial column sums that the product forming dz writes: one per tile row and row of waves, or the joining launch's
-int64_t strips_of(const Cut &c, int64_t R) { return c.slices > 1 ? (R + JOIN_ROWS - 1) / JOIN_ROWS : c.tiles_m * (c.tile == 64 ? 4 : 2); }
-// cx, cw, cdy: the rows of x, of the weights, of dy (as an operand) are copied
-Bwd bwd_plan(int64_t R, int64_t K, int64_t N, int dtype, bool gated, bool no_act, bool cx, bool cw, bool cdy) {
+int64_t join_strips(int64_t R) { return (R + strip_rows(R) - 1) / strip_rows(R); }
+int64_t strips_of(const Cut &c, int64_t R) { return c.slices > 1 ? join_strips(R) : c.tiles_m * (c.tile == 64 ? 4 : 2); }
+// kept: z is there; cx, cw, cdy: the rows of x, of the weights, of dy (as an operand) are copied
+Bwd bwd_plan(int64_t R, int64_t K, int64_t N, int dtype, bool gated, bool no_act, bool kept, bool cx, bool cw, bool cdy) {
     Bwd b;
     const int eb = eb_of(dtype), parts = gated ? 2 : 1;
     b.copies = (cx ? copy_bytes(R, K, eb) : 0) + (cw ? parts * copy_bytes(N, K, eb) : 0) + (cdy ? copy_bytes(R, N, eb) : 0);
@@ -491,10 +509,10 @@ Bwd bwd_plan(int64_t R, int64_t K, int64_t N, int dtype, bool gated, bool no_act
     b.dz_bytes = no_act ? 0 : ceil_to(R * b.ld_dz, 256);
     b.colsum_ld = ceil_to(N, 16) * parts;
     b.part = 0;
-    b.strips = no_act ? w3d_column_strips(R, N) : 0;
+    b.strips = no_act ? w3d_column_strips(R, N) : kept ? join_strips(R) : 0;
     for (int vec = 0; vec < 2; ++vec) {
         const Cut z = cut_of(R, gated ? b.pad : N, K, dtype, gated, vec, 1), dx = cut_of(R, K, gated ? 2 * b.pad : N, dtype, false, vec, 1), dw = cut_of(N, K, R, dtype, false, vec, parts);
-        if (!no_act) {
+        if (!no_act && !kept) {
             b.strips = max64(b.strips, strips_of(z, R));
             b.part = max64(b.part, (int64_t)part_bytes(z, R, N, gated, 1));
         }
@@ -504,18 +522,20 @@ Bwd bwd_plan(int64_t R, int64_t K, int64_t N, int dtype, bool gated, bool no_act
     return b;
 }
 
-int backward(const void *x, const void *w, const void *w2, const void *bias, const void *bias2, int bias_dtype, const void *dy, int64_t R, int64_t K, int64_t N, int dtype, int act,
-             bool gated, void *dx, void *dw, void *dw2, void *db, void *db2, void *workspace, size_t workspace_bytes, hipStream_t st) {
+int backward(const void *x, const void *w, const void *w2, const void *bias, const void *bias2, int bias_dtype, const void *dy, const float *z, int64_t R, int64_t K, int64_t N, int dtype,
+             int act, bool gated, void *dx, void *dw, void *dw2, void *db, void *db2, void *workspace, size_t workspace_bytes, hipStream_t st) {
     if (R < 0 || K < 1 || N < 1 || act < 0 || act > ACT_SIGMOID || !float_dtype(dtype)) return W3D_ERR_ARG;
     if ((bias || bias2 || db || db2) && bias_dtype != dtype && bias_dtype != W3D_DTYPE_F32) return W3D_ERR_ARG;
     if (!dx && !dw && !dw2 && !db && !db2) return W3D_ERR_ARG;
     const int eb = eb_of(dtype), parts = gated ? 2 : 1;
     if (!row_ok(K * eb) || !row_ok((N + 64) * eb * parts)) return W3D_ERR_UNSUPPORTED;
-    if (R > 0 && (!x || !w || !dy || (gated && !w2))) return W3D_ERR_ARG;
+    if (R > 0 && (!x || !w || !dy || (gated && !w2) || ((uintptr_t)z & 15))) return W3D_ERR_ARG;
     const bool no_act = !gated && act == ACT_NONE;
-    const bool cx = R > 0 && (!no_act || dw) && unaligned(x, K * eb), cw = R > 0 && (!no_act || dx) && (unaligned(w, K * eb) || unaligned(w2, K * eb)),
+    if (R > 0 && (dtype == W3D_DTYPE_F32 ? !no_act && !z : z != nullptr)) return W3D_ERR_ARG;
+    const bool again = !no_act && !z;                                                         // z is formed again
+    const bool cx = R > 0 && (again || dw || dw2) && unaligned(x, K * eb), cw = R > 0 && (again || dx) && (unaligned(w, K * eb) || unaligned(w2, K * eb)),
                cdy = R > 0 && no_act && (dx || dw) && unaligned(dy, N * eb);
-    const Bwd b = bwd_plan(R, K, N, dtype, gated, no_act, cx, cw, cdy);
+    const Bwd b = bwd_plan(R, K, N, dtype, gated, no_act, z != nullptr, cx, cw, cdy);
     uint8_t *ws = (uint8_t *)workspace;
     if (R > 0) {
         const size_t need = (size_t)(b.copies + b.dz_bytes + b.colsum_bytes + b.part);
@@ -538,10 +558,18 @@ int backward(const void *x, const void *w, const void *w2, const void *bias, con
         a.dy = (const uint8_t *)dy; a.out = dz_buf; a.ld_out = b.ld_dz; a.half_out = b.pad * eb; a.act = act; a.out_dt = dtype;
         a.vec_io = aligned16(dy, N * eb) ? 1 : 0;
         a.colsum = db || db2 ? colsum : nullptr; a.colsum_ld = b.colsum_ld; a.part = part;
-        const Cut c = cut_of(R, gated ? b.pad : N, K, dtype, gated, a.vec_io, 1);              // (the tiles write the padding columns too)
-        rc = run_product(a, gated ? PROD_GATED_BWD : PROD_LINEAR_BWD, dtype, c, 1, st);
+        const int prod = gated ? PROD_GATED_BWD : PROD_LINEAR_BWD;
+        if (z) {
+            a.part = const_cast<float *>(z); a.part_ld = z_stride(N, gated); a.slices = 1;
+            a.bias = a.bias2 = nullptr;
+            rc = join(a, prod, 1, st);
+            strips = join_strips(R);
+        } else {
+            const Cut c = cut_of(R, gated ? b.pad : N, K, dtype, gated, a.vec_io, 1);          // (the tiles write the padding columns too)
+            rc = run_product(a, prod, dtype, c, 1, st);
+            strips = strips_of(c, R);
+        }
         if (rc != W3D_OK) return rc;
-        strips = strips_of(c, R);
         dz = dz_buf; ld_dz = b.ld_dz;
     } else if (R > 0 && db) {
         rc = w3d_column_sums(dy, R, N, dtype, colsum, b.colsum_ld, st);
@@ -582,42 +610,43 @@ int backward(const void *x, const void *w, const void *w2, const void *bias, con
 }  // namespace
 
 extern "C" size_t w3d_linear_workspace_bytes(int64_t R, int64_t K, int64_t N, int dtype, int gated, int views) { return R < 1 ? 0 : forward_bytes(R, K, N, dtype, gated != 0, views != 0); }
-extern "C" size_t w3d_linear_bwd_workspace_bytes(int64_t R, int64_t K, int64_t N, int dtype, int act, int gated, int views) {
+extern "C" size_t w3d_linear_bwd_workspace_bytes(int64_t R, int64_t K, int64_t N, int dtype, int act, int gated, int kept, int views) {
     if (R < 1 || K < 1 || N < 1) return 0;
     const bool no_act = !gated && act == ACT_NONE, ck = views || K * eb_of(dtype) % 16, cn = views || N * eb_of(dtype) % 16;
-    const Bwd b = bwd_plan(R, K, N, dtype, gated != 0, no_act, ck, ck, no_act && cn);
+    const Bwd b = bwd_plan(R, K, N, dtype, gated != 0, no_act, kept != 0, ck, ck, no_act && cn);
     return (size_t)(b.copies + b.dz_bytes + b.colsum_bytes + b.part);
 }
+extern "C" int64_t w3d_linear_z_stride(int64_t N, int gated) { return N < 1 ? 0 : z_stride(N, gated != 0); }
 extern "C" int w3d_linear_fwd(const void *x, const void *w, const void *bias, int bias_dtype, const void *residual, int64_t R, int64_t K, int64_t N, int dtype, int act, void *y,
-                              void *workspace, size_t workspace_bytes, w3d_stream_t stream) {
+                              float *z, void *workspace, size_t workspace_bytes, w3d_stream_t stream) {
     if (!float_dtype(dtype)) return W3D_ERR_ARG;
-    return forward(x, nullptr, w, nullptr, nullptr, nullptr, bias, nullptr, bias_dtype, residual, R, K, N, dtype, dtype, act, false, y, workspace, workspace_bytes, w3d_s(stream));
+    return forward(x, nullptr, w, nullptr, nullptr, nullptr, bias, nullptr, bias_dtype, residual, R, K, N, dtype, dtype, act, false, y, z, workspace, workspace_bytes, w3d_s(stream));
 }
 extern "C" int w3d_linear_fp8_fwd(const void *x, const int32_t *x_scale, const void *w, const int32_t *w_scale, const void *bias, int bias_dtype, const void *residual, int64_t R,
                                   int64_t K, int64_t N, int out_dtype, int act, void *y, void *workspace, size_t workspace_bytes, w3d_stream_t stream) {
     if ((out_dtype != W3D_DTYPE_BF16 && out_dtype != W3D_DTYPE_F16) || (R > 0 && (!x_scale || !w_scale))) return W3D_ERR_ARG;
-    return forward(x, x_scale, w, w_scale, nullptr, nullptr, bias, nullptr, bias_dtype, residual, R, K, N, W3D_DTYPE_FP8_E4M3, out_dtype, act, false, y, workspace, workspace_bytes,
+    return forward(x, x_scale, w, w_scale, nullptr, nullptr, bias, nullptr, bias_dtype, residual, R, K, N, W3D_DTYPE_FP8_E4M3, out_dtype, act, false, y, nullptr, workspace, workspace_bytes,
                    w3d_s(stream));
 }
 extern "C" int w3d_gated_linear_fwd(const void *x, const void *w_gate, const void *w_up, const void *b_gate, const void *b_up, int bias_dtype, int64_t R, int64_t K, int64_t N, int dtype,
-                                    int act, void *y, void *workspace, size_t workspace_bytes, w3d_stream_t stream) {
+                                    int act, void *y, float *z, void *workspace, size_t workspace_bytes, w3d_stream_t stream) {
     if (!float_dtype(dtype)) return W3D_ERR_ARG;
-    return forward(x, nullptr, w_gate, nullptr, w_up, nullptr, b_gate, b_up, bias_dtype, nullptr, R, K, N, dtype, dtype, act, true, y, workspace, workspace_bytes, w3d_s(stream));
+    return forward(x, nullptr, w_gate, nullptr, w_up, nullptr, b_gate, b_up, bias_dtype, nullptr, R, K, N, dtype, dtype, act, true, y, z, workspace, workspace_bytes, w3d_s(stream));
 }
 extern "C" int w3d_gated_linear_fp8_fwd(const void *x, const int32_t *x_scale, const void *w_gate, const int32_t *gate_scale, const void *w_up, const int32_t *up_scale,
                                         const void *b_gate, const void *b_up, int bias_dtype, int64_t R, int64_t K, int64_t N, int out_dtype, int act, void *y, void *workspace,
                                         size_t workspace_bytes, w3d_stream_t stream) {
     if ((out_dtype != W3D_DTYPE_BF16 && out_dtype != W3D_DTYPE_F16) || (R > 0 && (!x_scale || !gate_scale || !up_scale))) return W3D_ERR_ARG;
-    return forward(x, x_scale, w_gate, gate_scale, w_up, up_scale, b_gate, b_up, bias_dtype, nullptr, R, K, N, W3D_DTYPE_FP8_E4M3, out_dtype, act, true, y, workspace, workspace_bytes,
+    return forward(x, x_scale, w_gate, gate_scale, w_up, up_scale, b_gate, b_up, bias_dtype, nullptr, R, K, N, W3D_DTYPE_FP8_E4M3, out_dtype, act, true, y, nullptr, workspace, workspace_bytes,
                    w3d_s(stream));
 }
-extern "C" int w3d_linear_bwd(const void *x, const void *w, const void *bias, int bias_dtype, const void *dy, int64_t R, int64_t K, int64_t N, int dtype, int act, void *dx, void *dw,
-                              void *dbias, void *workspace, size_t workspace_bytes, w3d_stream_t stream) {
-    return backward(x, w, nullptr, bias, nullptr, bias_dtype, dy, R, K, N, dtype, act, false, dx, dw, nullptr, dbias, nullptr, workspace, workspace_bytes, w3d_s(stream));
+extern "C" int w3d_linear_bwd(const void *x, const void *w, const void *bias, int bias_dtype, const void *dy, const float *z, int64_t R, int64_t K, int64_t N, int dtype, int act, void *dx,
+                              void *dw, void *dbias, void *workspace, size_t workspace_bytes, w3d_stream_t stream) {
+    return backward(x, w, nullptr, bias, nullptr, bias_dtype, dy, z, R, K, N, dtype, act, false, dx, dw, nullptr, dbias, nullptr, workspace, workspace_bytes, w3d_s(stream));
 }
-extern "C" int w3d_gated_linear_bwd(const void *x, const void *w_gate, const void *w_up, const void *b_gate, const void *b_up, int bias_dtype, const void *dy, int64_t R, int64_t K,
-                                    int64_t N, int dtype, int act, void *dx, void *dw_gate, void *dw_up, void *db_gate, void *db_up, void *workspace, size_t workspace_bytes,
+extern "C" int w3d_gated_linear_bwd(const void *x, const void *w_gate, const void *w_up, const void *b_gate, const void *b_up, int bias_dtype, const void *dy, const float *z, int64_t R,
+                                    int64_t K, int64_t N, int dtype, int act, void *dx, void *dw_gate, void *dw_up, void *db_gate, void *db_up, void *workspace, size_t workspace_bytes,
                                     w3d_stream_t stream) {
-    return backward(x, w_gate, w_up, b_gate, b_up, bias_dtype, dy, R, K, N, dtype, act, true, dx, dw_gate, dw_up, db_gate, db_up, workspace, workspace_bytes, w3d_s(stream));
+    return backward(x, w_gate, w_up, b_gate, b_up, bias_dtype, dy, z, R, K, N, dtype, act, true, dx, dw_gate, dw_up, db_gate, db_up, workspace, workspace_bytes, w3d_s(stream));
 }
 #endif

@@ -1562,35 +1562,41 @@ def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-6):
     return (q, scale) if s is None else (q, scale, s)
 
 
-def raw_linear(x, w, bias, residual, act: int, y):
+def raw_linear(x, w, bias, residual, act: int, y, z=None):
     """y [..., N] = act(x [..., K] w [N,K]^T + bias) + residual, contiguous."""
     N, K = w.shape
     R, dt = x.numel() // K, _code(x)
     nbytes = lib().w3d_linear_workspace_bytes(R, K, N, dt, 0, _views(x, w))
-    _launch("w3d_linear_fwd", x.device, lib().w3d_linear_fwd, x, w, bias, _code(bias), residual, R, K, N, dt, act, y, _scratch(nbytes, x.device), nbytes)
+    _launch("w3d_linear_fwd", x.device, lib().w3d_linear_fwd, x, w, bias, _code(bias), residual, R, K, N, dt, act, y, z, _scratch(nbytes, x.device), nbytes)
 
 
-def raw_gated_linear(x, wg, wu, bg, bu, act: int, y):
+def raw_gated_linear(x, wg, wu, bg, bu, act: int, y, z=None):
     """y [..., N] = act(x wg^T + bg) * (x wu^T + bu), contiguous."""
     N, K = wg.shape
     R, dt = x.numel() // K, _code(x)
     nbytes = lib().w3d_linear_workspace_bytes(R, K, N, dt, 1, _views(x, wg, wu))
-    _launch("w3d_gated_linear_fwd", x.device, lib().w3d_gated_linear_fwd, x, wg, wu, bg, bu, _code(bg if bg is not None else bu), R, K, N, dt, act, y, _scratch(nbytes, x.device), nbytes)
+    _launch("w3d_gated_linear_fwd", x.device, lib().w3d_gated_linear_fwd, x, wg, wu, bg, bu, _code(bg if bg is not None else bu), R, K, N, dt, act, y, z, _scratch(nbytes, x.device), nbytes)
+
+
+def _kept(x, N: int, gated: int):
+    """Room for the values before the activation: kept for the gradient by 32-bit calls (16-bit ones form them again)."""
+    return x.new_empty(x.numel() // x.shape[-1], lib().w3d_linear_z_stride(N, gated)) if x.dtype == torch.float32 else None
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, residual, act):
         y = x.new_empty(x.shape[:-1] + w.shape[:1])
-        raw_linear(x, w, bias, residual, act, y)
-        ctx.save_for_backward(x, w, bias)
+        z = _kept(x, w.shape[0], 0) if act else None
+        raw_linear(x, w, bias, residual, act, y, z)
+        ctx.save_for_backward(x, w, bias, z)
         ctx.act = act
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
-        x, w, bias = ctx.saved_tensors
+        x, w, bias, z = ctx.saved_tensors
         want_x, want_w, want_b, want_r, _ = ctx.needs_input_grad
         N, K = w.shape
         dx = torch.empty_like(x) if want_x else None
@@ -1601,8 +1607,8 @@ class _Linear(torch.autograd.Function):
             dw, db = (t.zero_() if t is not None else None for t in (dw, db))
         elif want_x or want_w or want_b:
             dt, gyc = _code(x), gy.contiguous()
-            nbytes = lib().w3d_linear_bwd_workspace_bytes(R, K, N, dt, ctx.act, 0, _views(x, w, gyc))
-            _launch("w3d_linear_bwd", x.device, lib().w3d_linear_bwd, x, w, bias, _code(bias), gyc, R, K, N, dt, ctx.act, dx, dw, db, _scratch(nbytes, x.device), nbytes)
+            nbytes = lib().w3d_linear_bwd_workspace_bytes(R, K, N, dt, ctx.act, 0, z is not None, _views(x, w, gyc))
+            _launch("w3d_linear_bwd", x.device, lib().w3d_linear_bwd, x, w, bias, _code(bias), gyc, z, R, K, N, dt, ctx.act, dx, dw, db, _scratch(nbytes, x.device), nbytes)
         return dx, dw, db, gy if want_r else None, None
 
 
@@ -1614,7 +1620,7 @@ def _head_weight(what: str, name: str, w):
 
 def linear(x, weight, bias=None, activation=None, residual=None):
     """y = act(x weight^T + bias) + residual in one launch.  x [..., K] f32 / bf16 / f16, weight [N,K] and residual [..., N] of x's type, bias [N] of x's type or f32;
-    activation None, 'relu', 'gelu' (z Phi(z)), 'silu' or 'sigmoid'.  Sums in f32, one rounding at the end.  Differentiable in everything; nothing but the inputs is kept for it."""
+    activation None, 'relu', 'gelu' (z Phi(z)), 'silu' or 'sigmoid'.  Sums in f32, one rounding at the end.  Differentiable in everything; for it 16-bit calls keep nothing but the inputs, f32 calls the values before the activation."""
     _head_rows("linear", x)
     act = _head_act(activation)
     N, _ = _head_weight("linear", "weight", weight)
@@ -1635,15 +1641,16 @@ class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wg, wu, bg, bu, act):
         y = x.new_empty(x.shape[:-1] + wg.shape[:1])
-        raw_gated_linear(x, wg, wu, bg, bu, act, y)
-        ctx.save_for_backward(x, wg, wu, bg, bu)
+        z = _kept(x, wg.shape[0], 1)
+        raw_gated_linear(x, wg, wu, bg, bu, act, y, z)
+        ctx.save_for_backward(x, wg, wu, bg, bu, z)
         ctx.act = act
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
-        x, wg, wu, bg, bu = ctx.saved_tensors
+        x, wg, wu, bg, bu, z = ctx.saved_tensors
         N, K = wg.shape
         grads = [torch.empty_like(t) if need else None for t, need in zip((x, wg, wu, bg, bu), ctx.needs_input_grad)]
         R = x.numel() // K
@@ -1651,8 +1658,8 @@ class _GatedLinear(torch.autograd.Function):
             grads = [t.zero_() if t is not None else None for t in grads]
         else:
             dt = _code(x)
-            nbytes = lib().w3d_linear_bwd_workspace_bytes(R, K, N, dt, ctx.act, 1, _views(x, wg, wu))
-            _launch("w3d_gated_linear_bwd", x.device, lib().w3d_gated_linear_bwd, x, wg, wu, bg, bu, _code(bg if bg is not None else bu), gy.contiguous(), R, K, N, dt, ctx.act, *grads,
+            nbytes = lib().w3d_linear_bwd_workspace_bytes(R, K, N, dt, ctx.act, 1, z is not None, _views(x, wg, wu))
+            _launch("w3d_gated_linear_bwd", x.device, lib().w3d_gated_linear_bwd, x, wg, wu, bg, bu, _code(bg if bg is not None else bu), gy.contiguous(), z, R, K, N, dt, ctx.act, *grads,
                     _scratch(nbytes, x.device), nbytes)
         return (*grads, None)
 
@@ -1668,7 +1675,7 @@ def _gated_args(what, x, wg, wu, bg, bu, dtype, bias_dtype):
 
 def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     """y = act(x w_gate^T + b_gate) * (x w_up^T + b_up): both products, the activation and the product in one launch.  x [..., K] f32 / bf16 / f16, weights [N,K] of x's type, biases
-    [N] of x's type or f32 (both alike); activation as in linear.  Sums in f32, one rounding at the end.  Differentiable in everything; nothing but the inputs is kept for it."""
+    [N] of x's type or f32 (both alike); activation as in linear.  Sums in f32, one rounding at the end.  Differentiable in everything; for it 16-bit calls keep nothing but the inputs, f32 calls the values before the activation."""
     _head_rows("gated_linear", x)
     act = _head_act(activation)
     N, w_gate, w_up, b_gate, b_up = _gated_args("gated_linear", x, w_gate, w_up, b_gate, b_up, x.dtype, x.dtype)
