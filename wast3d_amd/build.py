@@ -17,15 +17,14 @@ LIB = os.path.join(HERE, "libwast3d_hip.so")
 OBJ = os.path.join(HERE, "_obj")
 ARCH = "gfx950"
 FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wno-unused-result", "-ffp-contract=on",
-         "-I/opt/rocm/include", "-DROCPRIM_NO_DEPRECATED_WARNINGS"]
+         "-I/opt/rocm/include", "-DROCPRIM_NO_DEPRECATED_WARNINGS",
+         # no packed f32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on this hardware (the host pass warns that it does not know the feature)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
-
-# no packed f32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on this hardware
-NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 # per-file additions.  knn_mfma.hip: scores are compared with fmaxf trees; without "no NaNs" every fmaxf input gets a canonicalising
 # v_max_f32 x, x (15 instead of 9 VALU per 32x32 block in the selection pretest).  Infinities stay honoured (they are the sentinels).
-EXTRA_FLAGS = {"knn_mfma.hip": ["-fno-honor-nans"], "rms_norm.hip": NO_PACKED_F32, "columns.hip": NO_PACKED_F32, "linear.hip": NO_PACKED_F32}
+EXTRA_FLAGS = {"knn_mfma.hip": ["-fno-honor-nans"]}
 
 
 # knn_mfma.hip is compiled into a main object (entry points, dispatch) and one leaf object per (operand format, feature width): the leaves hold the kernel
