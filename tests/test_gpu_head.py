@@ -209,6 +209,37 @@ def gated_gradients(R, K, N, dt, acts):
                 within(grads[name], ref, tol + h * (ref.abs() + tol) + tiny(dt), f"d{name} {act}")
 
 
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("R", [40, 700])
+def test_any_subset_of_gradients(R, dt):
+    """A call that wants only some of its gradients gets the same bits for them as one that wants all."""
+    x, w, b, r = linear_case(R, 99, 70, dt, "silu", True, True, seed=170)
+    v, c = rnd(70, 99, seed=171, dtype=dt, scale=0.1), rnd(70, seed=172, dtype=dt)
+    dy = rnd(R, 70, seed=173, dtype=dt)
+    calls = [(lambda x, w, b, r: ops.linear(x, w, b, activation="silu", residual=r), (x, w, b, r)), (lambda x, w, b: ops.linear(x, w, b), (x, w, b)),
+             (lambda x, w, v, b, c: ops.gated_linear(x, w, v, b, c, activation="gelu"), (x, w, v, b, c)), (lambda x, w, r: sum(ops.rms_norm(x, w, residual=r)), (r, b, r * 0.5))]
+    for f, args in calls:
+        full = [a.clone().requires_grad_(True) for a in args]
+        want = torch.autograd.grad(f(*full), full, dy)
+        for mask in range(1, 2 ** len(args)):
+            some = [a.clone().requires_grad_(bool(mask >> i & 1)) for i, a in enumerate(args)]
+            live = [i for i in range(len(args)) if mask >> i & 1]
+            got = torch.autograd.grad(f(*some), [some[i] for i in live], dy)
+            assert all(torch.equal(g, want[i]) for g, i in zip(got, live)), (mask, live)
+
+
+def test_gradients_accumulate_and_second_derivatives_are_refused():
+    x, w = rnd(70, 64, seed=180).requires_grad_(True), rnd(48, 64, seed=181).requires_grad_(True)
+    y = ops.linear(ops.rms_norm(x) + ops.rms_norm(x), w, activation="gelu")
+    y.sum().backward()
+    first = x.grad.clone(), w.grad.clone()
+    ops.linear(ops.rms_norm(x) + ops.rms_norm(x), w, activation="gelu").sum().backward()
+    assert torch.equal(x.grad, 2 * first[0]) and torch.equal(w.grad, 2 * first[1])
+    g, = torch.autograd.grad(ops.linear(x, w, activation="gelu").sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), x)
+
+
 # ------------------------------------------------------------------------------------------------ 8-bit rows
 def dequant(q, e):
     return torch.ldexp(q.view(torch.float8_e4m3fn).double(), (e - 127)[:, None].double())

@@ -31,6 +31,7 @@ def test_rms_norm_arguments(L):
     assert f(P, None, None, 0, 4, 8, 0, 1e-6, P, P, None, None) == ARG                          # a sum without a residual
     assert f(None, None, None, 0, 0, 8, 0, 1e-6, None, None, None, None) == 0                   # no rows
     assert L.w3d_rms_norm_fp8(P, None, None, 0, 4, 8, 0, 1e-6, P, None, None, None) == ARG
+    assert f(P, None, None, 0, 4, (1 << 30) + 1, 0, 1e-6, P, None, None, None) == UNSUP
     b = L.w3d_rms_norm_bwd
     assert b(P, None, P, 0, P, P, None, 4, 8, 0, None, None, P, 4096, None) == ARG                    # nothing wanted
     assert b(P, None, P, 0, P, None, None, 4, 8, 0, P, P, P, 4096, None) == ARG

@@ -312,7 +312,7 @@ bool aligned16(const void *p, int64_t ld) { return !(((uintptr_t)p) & 15) && ld 
 // widths 100 .. 4 096: `lone`, a 128-byte slab of a block that has its CU for itself; `busy`, the same of a block among others, per block on the CU; `round`, start and epilogue of a block.
 // Slices write and read their f32 tiles (2.5 TB/s with the second launch's start).
 struct TileCost { double lone[3], busy[3], round[3]; };      // of 64, 128, 256
-constexpr TileCost COST_16 = {{0.35, 0.6, 1.2}, {0.22, 0.6, 1.3}, {4, 5, 10}}, COST_FP8 = {{0.35, 0.6, 0.9}, {0.22, 0.6, 0.9}, {4, 5, 10}},
+constexpr TileCost COST_16 = {{0.35, 0.6, 1.2}, {0.22, 0.6, 1.3}, {4, 5, 10}}, COST_DW = {{0.57, 0.77, 1.35}, {0.24, 0.85, 1.35}, {4, 5, 10}}, COST_FP8 = {{0.35, 0.6, 0.9}, {0.22, 0.6, 0.9}, {4, 5, 10}},
                    COST_F32 = {{0.72, 2.25, 0}, {0.62, 2.25, 0}, {4, 5, 0}};
 #ifndef W3D_FORCE_TILE
 #define W3D_FORCE_TILE 0
@@ -322,7 +322,8 @@ constexpr TileCost COST_16 = {{0.35, 0.6, 1.2}, {0.22, 0.6, 1.3}, {4, 5, 10}}, C
 #endif
 struct Cut { int tile, slices; int64_t tiles_m, tiles_n; };
 // vec: rows of everything the epilogue touches are aligned, too (the 256 x 256 tile needs it)
-Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool gated, bool vec, int batch) {
+// dw: both operands M_ROWS
+Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool gated, bool vec, int batch, bool dw = false) {
     const int parts = gated ? 2 : 1;
     const int64_t slabs = (K * eb_of(dtype) + SLAB - 1) / SLAB;
     Cut best = {};
@@ -333,7 +334,7 @@ Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool gated, bool vec, int
         const int bn = tile / parts;
         const int64_t tm = (M + tile - 1) / tile, tn = (N + bn - 1) / bn, tiles = tm * tn * batch;
         const int k = tile == 64 ? 0 : tile == 128 ? 1 : 2;
-        const TileCost &c = dtype == W3D_DTYPE_F32 ? COST_F32 : dtype == W3D_DTYPE_FP8_E4M3 ? COST_FP8 : COST_16;
+        const TileCost &c = dtype == W3D_DTYPE_F32 ? COST_F32 : dtype == W3D_DTYPE_FP8_E4M3 ? COST_FP8 : dw ? COST_DW : COST_16;
         const int per_cu = tile == 256 ? 1 : tile == 128 ? 2 : 4;
         for (int s = 1; s <= 32 && (s == 1 || slabs / s >= 4); ++s) {
             if (W3D_FORCE_SLICES && s != W3D_FORCE_SLICES) continue;
@@ -511,7 +512,7 @@ Bwd bwd_plan(int64_t R, int64_t K, int64_t N, int dtype, bool gated, bool no_act
     b.part = 0;
     b.strips = no_act ? w3d_column_strips(R, N) : kept ? join_strips(R) : 0;
     for (int vec = 0; vec < 2; ++vec) {
-        const Cut z = cut_of(R, gated ? b.pad : N, K, dtype, gated, vec, 1), dx = cut_of(R, K, gated ? 2 * b.pad : N, dtype, false, vec, 1), dw = cut_of(N, K, R, dtype, false, vec, parts);
+        const Cut z = cut_of(R, gated ? b.pad : N, K, dtype, gated, vec, 1), dx = cut_of(R, K, gated ? 2 * b.pad : N, dtype, false, vec, 1), dw = cut_of(N, K, R, dtype, false, vec, parts, true);
         if (!no_act && !kept) {
             b.strips = max64(b.strips, strips_of(z, R));
             b.part = max64(b.part, (int64_t)part_bytes(z, R, N, gated, 1));
@@ -602,7 +603,7 @@ int backward(const void *x, const void *w, const void *w2, const void *bias, con
         a.M = N; a.N = K; a.K = R; a.w_rows = R; a.z_x = b.pad * eb;
         a.out = (uint8_t *)o; a.out2 = (uint8_t *)dw2; a.ld_out = K * eb; a.out_dt = dtype; a.part = part;
         a.vec_io = aligned16(o, K * eb) && aligned16(both ? dw2 : nullptr, 0) ? 1 : 0;
-        rc = run_product(a, PROD_DW, dtype, cut_of(N, K, R, dtype, false, a.vec_io, parts), both ? 2 : 1, st);
+        rc = run_product(a, PROD_DW, dtype, cut_of(N, K, R, dtype, false, a.vec_io, parts, true), both ? 2 : 1, st);
         if (rc != W3D_OK) return rc;
     }
     return W3D_OK;

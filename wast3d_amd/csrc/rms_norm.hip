@@ -12,7 +12,7 @@
 
 namespace {
 
-constexpr int NORM_BLOCK = 256;
+constexpr int NORM_BLOCK = 256, MAX_WIDTH = 1 << 30;      // (columns are 32-bit)
 
 struct NormArgs {
     const char *x, *res, *w;
@@ -374,6 +374,7 @@ static int rms_norm_any(const void *x, const void *residual, const void *weight,
                         void *q, int32_t *scale, w3d_stream_t stream) {
     if (R < 0 || d < 1 || !dtype_ok(dtype) || !(eps >= 0.f)) return W3D_ERR_ARG;
     if (weight && weight_dtype != dtype && weight_dtype != W3D_DTYPE_F32) return W3D_ERR_ARG;
+    if (d > MAX_WIDTH) return W3D_ERR_UNSUPPORTED;
     if (R == 0) return W3D_OK;
     if (!x || (s && !residual)) return W3D_ERR_ARG;
     NormArgs a = {(const char *)x, (const char *)residual, (const char *)weight, (char *)y, (char *)s, rstd, (uint8_t *)q, scale, R, d,
@@ -406,6 +407,7 @@ extern "C" int w3d_rms_norm_bwd(const void *x, const void *residual, const void 
     if (R < 0 || d < 1 || !dtype_ok(dtype) || (!dx && !dweight)) return W3D_ERR_ARG;
     if ((weight || dweight) && weight_dtype != dtype && weight_dtype != W3D_DTYPE_F32) return W3D_ERR_ARG;
     if (R > 0 && (!x || !rstd || !dy)) return W3D_ERR_ARG;
+    if (d > MAX_WIDTH) return W3D_ERR_UNSUPPORTED;
     hipStream_t st = w3d_s(stream);
     const int blocks = R > 0 ? blocks_for(R, d) : 0;
     if (R > 0) {

@@ -1414,25 +1414,25 @@ _DTYPE_CODES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 
 def _head_rows(what: str, x):
     """Type code of the rows; the rest of a call's tensors is checked against them (_head_arg)."""
-    if not x.is_cuda:
-        require_cuda(x)
     code = _DTYPE_CODES.get(x.dtype)
-    if code is None:
-        raise W3dError(f"{what}: unsupported dtype {x.dtype} (float32, bfloat16 or float16)")
-    if x.dim() < 1 or x.shape[-1] < 1:
+    if code is None or not x.is_cuda or x.dim() < 1 or x.shape[-1] < 1:
+        if not x.is_cuda:
+            require_cuda(x)
+        if code is None:
+            raise W3dError(f"{what}: unsupported dtype {x.dtype} (float32, bfloat16 or float16)")
         raise W3dError(f"{what}: rows of at least one element expected, got a tensor of shape {tuple(x.shape)}")
     return code
 
 
 def _head_arg(what: str, name: str, t, shape, dtype, device, wide: bool = False):
     """Shape, type and device of one tensor of a call (wide: f32 is taken next to 16-bit rows) -> the contiguous tensor."""
+    if t.shape == shape and t.device == device and (t.dtype == dtype or (wide and t.dtype == torch.float32)):
+        return t.contiguous()
     if t.shape != shape:
         raise W3dError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.dtype != dtype and not (wide and t.dtype == torch.float32):
-        raise W3dError(f"{what}: {name} is {t.dtype}, expected {dtype}" + (" or torch.float32" if wide else ""))
     if t.device != device:
         raise W3dError(f"{what}: {name} is on {t.device}, the rows are on {device}")
-    return t.contiguous()
+    raise W3dError(f"{what}: {name} is {t.dtype}, expected {dtype}" + (" or torch.float32" if wide else ""))
 
 
 def _head_eps(eps) -> float:
@@ -1442,19 +1442,27 @@ def _head_eps(eps) -> float:
     return eps
 
 
-def _launch(what: str, device, fn, *args):
-    """One call of the library on the current stream of the tensors' own device (tensors travel as their addresses; the stream is the last argument)."""
-    index = device.index
-    args = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _launch(what: str, index: int, fn, *args):
+    """One call of the library on the current stream of the tensors' own device (the stream is the last argument; tensors travel as addresses, None as NULL)."""
     if index == torch.cuda.current_device():
         clear_stale_hip_error()
-        code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        code = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
             clear_stale_hip_error()
-            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+            code = fn(*args, _raw_stream(index))
     if code:
         check(code, what)
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+_FEW_ROWS = 64                                                     # the few-row form takes no workspace (w3d_linear_workspace_bytes)
 
 
 def _scratch(nbytes: int, device):
@@ -1484,7 +1492,8 @@ def _code(t) -> int:
 def raw_rms_norm(x, weight, residual, eps: float, y, s=None, rstd=None):
     """y (and s = x + residual, and rstd f32 [R]) of contiguous rows x [..., d]."""
     d = x.shape[-1]
-    _launch("w3d_rms_norm_fwd", x.device, lib().w3d_rms_norm_fwd, x, residual, weight, _code(weight), x.numel() // d, d, _code(x), eps, y, s, rstd)
+    _launch("w3d_rms_norm_fwd", x.get_device(), lib().w3d_rms_norm_fwd, x.data_ptr(), _at(residual), _at(weight), _code(weight), x.numel() // d, d, _DTYPE_CODES[x.dtype], eps, y.data_ptr(),
+            _at(s), _at(rstd))
 
 
 def raw_rms_norm_bwd(x, residual, weight, rstd, dy, ds, dx=None, dweight=None):
@@ -1492,7 +1501,9 @@ def raw_rms_norm_bwd(x, residual, weight, rstd, dy, ds, dx=None, dweight=None):
     d = x.shape[-1]
     R = x.numel() // d
     nbytes = lib().w3d_rms_norm_bwd_workspace_bytes(R, d) if dweight is not None else 0
-    _launch("w3d_rms_norm_bwd", x.device, lib().w3d_rms_norm_bwd, x, residual, weight, _code(weight), rstd, dy, ds, R, d, _code(x), dx, dweight, _scratch(nbytes, x.device), nbytes)
+    ws = _scratch(nbytes, x.device)
+    _launch("w3d_rms_norm_bwd", x.get_device(), lib().w3d_rms_norm_bwd, x.data_ptr(), _at(residual), _at(weight), _code(weight), rstd.data_ptr(), dy.data_ptr(), _at(ds), R, d,
+            _DTYPE_CODES[x.dtype], _at(dx), _at(dweight), _at(ws), nbytes)
 
 
 class _RmsNorm(torch.autograd.Function):
@@ -1558,24 +1569,27 @@ def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-6):
     q = torch.empty(R, d, dtype=torch.uint8, device=x.device)
     scale = torch.empty(R, dtype=torch.int32, device=x.device)
     s = torch.empty_like(xc) if residual is not None else None
-    _launch("w3d_rms_norm_fp8", x.device, lib().w3d_rms_norm_fp8, xc, residual, weight, _code(weight), R, d, code, eps, q, scale, s)
+    _launch("w3d_rms_norm_fp8", x.get_device(), lib().w3d_rms_norm_fp8, xc.data_ptr(), _at(residual), _at(weight), _code(weight), R, d, code, eps, q.data_ptr(), scale.data_ptr(), _at(s))
     return (q, scale) if s is None else (q, scale, s)
 
 
 def raw_linear(x, w, bias, residual, act: int, y, z=None):
     """y [..., N] = act(x [..., K] w [N,K]^T + bias) + residual, contiguous."""
     N, K = w.shape
-    R, dt = x.numel() // K, _code(x)
-    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, dt, 0, _views(x, w))
-    _launch("w3d_linear_fwd", x.device, lib().w3d_linear_fwd, x, w, bias, _code(bias), residual, R, K, N, dt, act, y, z, _scratch(nbytes, x.device), nbytes)
+    R, dt = x.numel() // K, _DTYPE_CODES[x.dtype]
+    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, dt, 0, _views(x, w)) if R > _FEW_ROWS else 0
+    ws = _scratch(nbytes, x.device) if nbytes else None
+    _launch("w3d_linear_fwd", x.get_device(), lib().w3d_linear_fwd, x.data_ptr(), w.data_ptr(), _at(bias), _code(bias), _at(residual), R, K, N, dt, act, y.data_ptr(), _at(z), _at(ws), nbytes)
 
 
 def raw_gated_linear(x, wg, wu, bg, bu, act: int, y, z=None):
     """y [..., N] = act(x wg^T + bg) * (x wu^T + bu), contiguous."""
     N, K = wg.shape
-    R, dt = x.numel() // K, _code(x)
-    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, dt, 1, _views(x, wg, wu))
-    _launch("w3d_gated_linear_fwd", x.device, lib().w3d_gated_linear_fwd, x, wg, wu, bg, bu, _code(bg if bg is not None else bu), R, K, N, dt, act, y, z, _scratch(nbytes, x.device), nbytes)
+    R, dt = x.numel() // K, _DTYPE_CODES[x.dtype]
+    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, dt, 1, _views(x, wg, wu)) if R > _FEW_ROWS else 0
+    ws = _scratch(nbytes, x.device) if nbytes else None
+    _launch("w3d_gated_linear_fwd", x.get_device(), lib().w3d_gated_linear_fwd, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), _at(bg), _at(bu), _code(bg if bg is not None else bu), R, K, N,
+            dt, act, y.data_ptr(), _at(z), _at(ws), nbytes)
 
 
 def _kept(x, N: int, gated: int):
@@ -1608,7 +1622,9 @@ class _Linear(torch.autograd.Function):
         elif want_x or want_w or want_b:
             dt, gyc = _code(x), gy.contiguous()
             nbytes = lib().w3d_linear_bwd_workspace_bytes(R, K, N, dt, ctx.act, 0, z is not None, _views(x, w, gyc))
-            _launch("w3d_linear_bwd", x.device, lib().w3d_linear_bwd, x, w, bias, _code(bias), gyc, z, R, K, N, dt, ctx.act, dx, dw, db, _scratch(nbytes, x.device), nbytes)
+            ws = _scratch(nbytes, x.device)
+            _launch("w3d_linear_bwd", x.get_device(), lib().w3d_linear_bwd, x.data_ptr(), w.data_ptr(), _at(bias), _code(bias), gyc.data_ptr(), _at(z), R, K, N, dt, ctx.act, _at(dx), _at(dw),
+                    _at(db), _at(ws), nbytes)
         return dx, dw, db, gy if want_r else None, None
 
 
@@ -1659,8 +1675,9 @@ class _GatedLinear(torch.autograd.Function):
         else:
             dt = _code(x)
             nbytes = lib().w3d_linear_bwd_workspace_bytes(R, K, N, dt, ctx.act, 1, z is not None, _views(x, wg, wu))
-            _launch("w3d_gated_linear_bwd", x.device, lib().w3d_gated_linear_bwd, x, wg, wu, bg, bu, _code(bg if bg is not None else bu), gy.contiguous(), z, R, K, N, dt, ctx.act, *grads,
-                    _scratch(nbytes, x.device), nbytes)
+            ws, gyc = _scratch(nbytes, x.device), gy.contiguous()
+            _launch("w3d_gated_linear_bwd", x.get_device(), lib().w3d_gated_linear_bwd, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), _at(bg), _at(bu), _code(bg if bg is not None else bu),
+                    gyc.data_ptr(), _at(z), R, K, N, dt, ctx.act, *(_at(g) for g in grads), _at(ws), nbytes)
         return (*grads, None)
 
 
@@ -1719,8 +1736,10 @@ def linear_fp8(q, scale, weight_q, weight_scale, bias=None, activation=None, res
     if residual is not None:
         residual = _head_arg("linear_fp8", "residual", residual, (R, N), out_dtype, dev)
     y = torch.empty(R, N, dtype=out_dtype, device=dev)
-    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, FP8, 0, _views(q, weight_q))
-    _launch("w3d_linear_fp8_fwd", dev, lib().w3d_linear_fp8_fwd, q, scale, weight_q, weight_scale, bias, _code(bias), residual, R, K, N, code, act, y, _scratch(nbytes, dev), nbytes)
+    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, FP8, 0, _views(q, weight_q)) if R > _FEW_ROWS else 0
+    ws = _scratch(nbytes, dev)
+    _launch("w3d_linear_fp8_fwd", dev.index, lib().w3d_linear_fp8_fwd, q.data_ptr(), scale.data_ptr(), weight_q.data_ptr(), weight_scale.data_ptr(), _at(bias), _code(bias), _at(residual),
+            R, K, N, code, act, y.data_ptr(), _at(ws), nbytes)
     return y
 
 
@@ -1734,7 +1753,8 @@ def gated_linear_fp8(q, scale, gate_q, gate_scale, up_q, up_scale, b_gate=None, 
     N, gate_q, up_q, b_gate, b_up = _gated_args("gated_linear_fp8", q, gate_q, up_q, b_gate, b_up, torch.uint8, out_dtype)
     R, K = q.shape
     y = torch.empty(R, N, dtype=out_dtype, device=dev)
-    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, FP8, 1, _views(q, gate_q, up_q))
-    _launch("w3d_gated_linear_fp8_fwd", dev, lib().w3d_gated_linear_fp8_fwd, q, scale, gate_q, gate_scale, up_q, up_scale, b_gate, b_up, _code(b_gate if b_gate is not None else b_up), R, K, N,
-            code, act, y, _scratch(nbytes, dev), nbytes)
+    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, FP8, 1, _views(q, gate_q, up_q)) if R > _FEW_ROWS else 0
+    ws = _scratch(nbytes, dev)
+    _launch("w3d_gated_linear_fp8_fwd", dev.index, lib().w3d_gated_linear_fp8_fwd, q.data_ptr(), scale.data_ptr(), gate_q.data_ptr(), gate_scale.data_ptr(), up_q.data_ptr(),
+            up_scale.data_ptr(), _at(b_gate), _at(b_up), _code(b_gate if b_gate is not None else b_up), R, K, N, code, act, y.data_ptr(), _at(ws), nbytes)
     return y
