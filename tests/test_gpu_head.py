@@ -453,6 +453,37 @@ def test_bad_gradient_rows_stay_alone():
         assert a.isfinite().all() and torch.equal(a[:149], c[:149]) and c[149].isnan().all()
 
 
+def test_more_than_2_to_the_31_elements():
+    """Rows whose elements are past 2^31 (and bytes past 2^32) from the first: the last rows of every output against the definition on those rows alone."""
+    R, K, N, tail = 2_200_001, 1024, 128, 300
+    x = torch.empty(R, K, dtype=BF16, device="cuda")
+    x[: 1 << 16] = rnd(1 << 16, K, seed=190, dtype=BF16)
+    for a in range(1 << 16, R, 1 << 16):
+        x[a: a + (1 << 16)] = x[: min(1 << 16, R - a)]
+    x[-tail:] = rnd(tail, K, seed=191, dtype=BF16)
+    w, b = rnd(N, K, seed=192, dtype=BF16, scale=K ** -0.5), rnd(N, seed=193, dtype=BF16)
+    y = ops.linear(x, w, b, activation="gelu")
+    check_linear(x[-tail:], w, b, None, "gelu", y[-tail:])
+    check_linear(x[:tail], w, b, None, "gelu", y[:tail])
+    assert torch.equal(ops.rms_norm(x)[-tail:], ops.rms_norm(x[-tail:].clone()))
+    q, e = ops.rms_norm_fp8(x)
+    q1, e1 = ops.rms_norm_fp8(x[-tail:].clone())
+    assert torch.equal(q[-tail:], q1) and torch.equal(e[-tail:], e1)
+    check_linear(dequant(q[-tail:], e[-tail:]), dequant(*ops.quantize_rows_fp8(w)), None, None, None, ops.linear_fp8(q, e, *ops.quantize_rows_fp8(w))[-tail:])
+    del q, e, y
+    dy = torch.zeros(R, N, dtype=BF16, device="cuda")
+    dy[-tail:] = rnd(tail, N, seed=194, dtype=BF16)
+    w.requires_grad_(True)
+    xg = x.requires_grad_(True)
+    dx, dw = torch.autograd.grad(ops.linear(xg, w, b, activation="gelu"), (xg, w), dy)
+    xt, wt = x.detach()[-tail:].clone().requires_grad_(True), w.detach().clone().requires_grad_(True)
+    dxt, dwt = torch.autograd.grad(ops.linear(xt, wt, b, activation="gelu"), (xt, wt), dy[-tail:])
+    # (the same products in another cut: two f32 sums of the same terms, rounded once)
+    assert not dx[:-tail].any()
+    for a, c in ((dx[-tail:], dxt), (dw, dwt)):
+        within(a, c, 2 ** -7 * c.double().abs() + 1e-3 * float(c.double().abs().mean()))
+
+
 # ------------------------------------------------------------------------------------------------ no rows, repeatability, streams, graphs
 def test_no_rows():
     for dt in (BF16, F32):
