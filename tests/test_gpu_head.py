@@ -453,6 +453,64 @@ def test_bad_gradient_rows_stay_alone():
         assert a.isfinite().all() and torch.equal(a[:149], c[:149]) and c[149].isnan().all()
 
 
+@pytest.mark.parametrize("N", [64, 70])
+@pytest.mark.parametrize("act", ["relu", "sigmoid"])
+def test_an_infinite_row_keeps_its_finite_gradient(act, N):
+    """z = +-inf: the derivatives are 0 or 1 and dx finite; columns that only pad dz to whole chunks (70) must not add inf * 0."""
+    x, w, _, _ = linear_case(150, 96, N, BF16, act, False, False, seed=97)
+    x[149, 5] = float("inf")
+    dy = rnd(150, N, seed=98, dtype=BF16)
+    dx, = torch.autograd.grad(ops.linear(x.requires_grad_(True), w, activation=act), x, dy)
+    d = (w[:, 5] > 0).double() if act == "relu" else torch.zeros(N, dtype=torch.float64, device="cuda")
+    dz = dy[149].double() * d
+    ref, mag = dz @ w.double(), dz.abs() @ w.double().abs()
+    within(dx[149], ref, (N + 8) * W * mag + half_step(BF16) * ref.abs() + tiny(BF16))
+    assert dx[:149].isfinite().all()
+
+
+def test_rows_just_short_of_8_megabytes():
+    """The longest rows there are (32-bit offsets inside a tile): the last columns hold everything, so that the definition is a small product."""
+    K, used = (8 << 20) // 2 - 8, 512
+    for R, N in ((100, 9), (1030, 264)):
+        x, w = torch.zeros(R, K, dtype=BF16, device="cuda"), torch.zeros(N, K, dtype=BF16, device="cuda")
+        xs, ws, b, _ = linear_case(R, used, N, BF16, None, True, False, seed=185)
+        x[:, -used:], w[:, -used:] = xs, ws
+        y = ops.linear(x.requires_grad_(True), w.requires_grad_(True), b)
+        check_linear(xs, ws, b, None, None, y)
+        dy = rnd(R, N, seed=186, dtype=BF16)
+        dx, dw = torch.autograd.grad(y, (x, w), dy)
+        for got, p, q, n in ((dx, dy, ws, N), (dw, dy.t(), xs, R)):
+            ref, mag = p.double() @ q.double(), p.double().abs() @ q.double().abs()
+            within(got[:, -used:], ref, (n + 8) * W * mag + half_step(BF16) * ref.abs() + tiny(BF16))
+            assert not got[:, :-used].any()
+        del x, w, y, dx, dw, got
+    with pytest.raises(_lib.W3dError):
+        ops.linear(torch.zeros(1, K + 8, dtype=BF16, device="cuda"), torch.zeros(1, K + 8, dtype=BF16, device="cuda"))
+
+
+def test_rms_norm_widths_past_32_bits_are_refused():
+    one = torch.ones(1, 1, dtype=BF16, device="cuda")
+    for d in ((1 << 30) + 1, (1 << 31) + 5, (1 << 32) + 5):
+        for f in (ops.rms_norm, ops.rms_norm_fp8):
+            with pytest.raises(_lib.W3dError):
+                f(one.expand(1, d))
+
+
+def test_rms_norm_fp8_of_infinities():
+    """An infinity behind the norm saturates, by the rule of quantize_rows_fp8; the other rows do not see it."""
+    x, w = rnd(5, 64, seed=187), torch.ones(64, device="cuda")
+    q0, e0 = ops.rms_norm_fp8(x, w)
+    w[7] = float("inf")
+    q, e = ops.rms_norm_fp8(x, w)
+    q2, e2 = ops.quantize_rows_fp8(ops.rms_norm(x, w))
+    assert torch.equal(q, q2) and torch.equal(e, e2)
+    x[3] *= 3.0e38
+    x[3, 9] = float("inf")
+    q, e = ops.rms_norm_fp8(x)
+    keep = torch.arange(5, device="cuda") != 3
+    assert torch.equal(q[keep], q0[keep]) and torch.equal(e[keep], e0[keep])
+
+
 def test_more_than_2_to_the_31_elements():
     """Rows whose elements are past 2^31 (and bytes past 2^32) from the first: the last rows of every output against the definition on those rows alone."""
     R, K, N, tail = 2_200_001, 1024, 128, 300

@@ -198,7 +198,7 @@ struct Pipe {
     template <int LAY, int N>
     static __device__ __forceinline__ void read_side(const uint32_t (&a)[4], uint32_t at, i32x4 (&v)[N]) {
         if constexpr (LAY == K_ROWS && MS == 16 && N == 8) {
-            asm volatile("ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:1024\n\tds_read_b128 %2, %8 offset:2048\n\tds_read_b128 %3, %8 offset:3072\n\t"
+            asm volatile("ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:1024\n\tds_read_b128 %2, %8 offset:2048\n\tds_read_b128 %3, %8 offset:0xc00\n\t"
                          "ds_read_b128 %4, %8 offset:4096\n\tds_read_b128 %5, %8 offset:5120\n\tds_read_b128 %6, %8 offset:6144\n\tds_read_b128 %7, %8 offset:7168\n\ts_waitcnt lgkmcnt(0)"
                          : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7]) : "v"(a[0] + at) : "memory");
         } else if constexpr (LAY == K_ROWS && MS == 16) {

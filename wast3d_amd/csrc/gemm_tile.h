@@ -391,10 +391,17 @@ struct Out {
             };
             if constexpr (BWD) with_act(a.act, apply);                                         // (per row: five copies of the whole would spill)
             else apply(act_c);
+            // the padding columns of dz are part of the contraction of dx: zeros, also where the row's z or dy is not finite (VEC: a run is inside or outside as a whole, and linear rows have none)
+            if constexpr (BWD && (GATED || !VEC))
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const bool in = n + (VEC ? 0 : e) < a.N;
+                    v[e] = in ? v[e] : 0.f;
+                    if (GATED) u[e] = in ? u[e] : 0.f;
+                }
             if (BWD)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) { c0[e] += live ? v[e] : 0.f; if (GATED) c1[e] += live ? u[e] : 0.f; }      // column sums in f32, before the rounding
-            // BWD writes dz; zeros in the padding columns (dy is read as zero there and z is finite: W has no such rows, the bias no such elements), which are part of the contraction of dx
             if (live && (BWD ? pad > 0 : n < a.N)) {
                 store_run<OT, 8>(out + off, VEC ? 8 : BWD ? pad : a.N - n, VEC || BWD || vec, v);
                 if (EPI == EPI_GATED_BWD) store_run<OT, 8>(out + off + a.half_out, VEC ? 8 : pad, true, u);

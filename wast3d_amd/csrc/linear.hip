@@ -314,12 +314,6 @@ bool aligned16(const void *p, int64_t ld) { return !(((uintptr_t)p) & 15) && ld 
 struct TileCost { double lone[3], busy[3], round[3]; };      // of 64, 128, 256
 constexpr TileCost COST_16 = {{0.35, 0.6, 1.2}, {0.22, 0.6, 1.3}, {4, 5, 10}}, COST_DW = {{0.57, 0.77, 1.35}, {0.24, 0.85, 1.35}, {4, 5, 10}}, COST_FP8 = {{0.35, 0.6, 0.9}, {0.22, 0.6, 0.9}, {4, 5, 10}},
                    COST_F32 = {{0.72, 2.25, 0}, {0.62, 2.25, 0}, {4, 5, 0}};
-#ifndef W3D_FORCE_TILE
-#define W3D_FORCE_TILE 0
-#endif
-#ifndef W3D_FORCE_SLICES
-#define W3D_FORCE_SLICES 0
-#endif
 struct Cut { int tile, slices; int64_t tiles_m, tiles_n; };
 // vec: rows of everything the epilogue touches are aligned, too (the 256 x 256 tile needs it)
 // dw: both operands M_ROWS
@@ -330,14 +324,12 @@ Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool gated, bool vec, int
     double best_t = 0;
     for (int tile = 64; tile <= 256; tile *= 2) {
         if (tile == 256 && (!vec || dtype == W3D_DTYPE_F32)) break;
-        if (W3D_FORCE_TILE && tile != W3D_FORCE_TILE) continue;
         const int bn = tile / parts;
         const int64_t tm = (M + tile - 1) / tile, tn = (N + bn - 1) / bn, tiles = tm * tn * batch;
         const int k = tile == 64 ? 0 : tile == 128 ? 1 : 2;
         const TileCost &c = dtype == W3D_DTYPE_F32 ? COST_F32 : dtype == W3D_DTYPE_FP8_E4M3 ? COST_FP8 : dw ? COST_DW : COST_16;
         const int per_cu = tile == 256 ? 1 : tile == 128 ? 2 : 4;
         for (int s = 1; s <= 32 && (s == 1 || slabs / s >= 4); ++s) {
-            if (W3D_FORCE_SLICES && s != W3D_FORCE_SLICES) continue;
             const double cu = (double)((tiles * s + 255) / 256), rounds = (double)((tiles * s + 256 * per_cu - 1) / (256 * per_cu)), n = (double)((slabs + s - 1) / s);
             const double a = n * c.busy[k] * cu, b = n * c.lone[k] * rounds;
             double t = (a > b ? a : b) + c.round[k] * rounds;

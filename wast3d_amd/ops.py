@@ -1489,6 +1489,14 @@ def _code(t) -> int:
     return 0 if t is None else _DTYPE_CODES[t.dtype]
 
 
+_MAX_WIDTH = 1 << 30                                               # columns of a normalised row (the library counts them in 32 bits)
+
+
+def _norm_width(what: str, x):
+    if x.shape[-1] > _MAX_WIDTH:
+        raise W3dError(f"{what}: rows of {x.shape[-1]} elements (at most {_MAX_WIDTH})")
+
+
 def raw_rms_norm(x, weight, residual, eps: float, y, s=None, rstd=None):
     """y (and s = x + residual, and rstd f32 [R]) of contiguous rows x [..., d]."""
     d = x.shape[-1]
@@ -1537,6 +1545,7 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-6):
     Returns y, or (y, s) with a residual (s rounded to x's type: what the next block adds to).  The norm is taken of the unrounded sum; sums are f32.
     Differentiable in x, weight and residual."""
     _head_rows("rms_norm", x)
+    _norm_width("rms_norm", x)
     eps = _head_eps(eps)
     xc = x.contiguous()
     if weight is not None:
@@ -1555,6 +1564,7 @@ def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-6):
     """rms_norm with its rows in 8 bits: (q uint8 [R,d] = OCP e4m3 bytes, scale int32 [R] = E8M0 exponents) as of quantize_rows_fp8, and s [R,d] behind them with a residual.
     x [R,d].  The rows are quantised from the f32 values, by quantize_rows_fp8's rule; they go straight into raw_knn_match_fp8 (d = 128, 256) or the _fp8 layers.  No gradient."""
     code = _head_rows("rms_norm_fp8", x)
+    _norm_width("rms_norm_fp8", x)
     if x.dim() != 2:
         raise W3dError(f"rms_norm_fp8: rows [R,d] expected, got a tensor of shape {tuple(x.shape)}")
     eps = _head_eps(eps)
