@@ -110,6 +110,20 @@ def test_large_forward(R, K, N):
         check_gated(*c, "silu", ops.gated_linear(*c, activation="silu"))
 
 
+# few rows that take tiles over a sliced contraction (long rows, many columns), next to ones that do not
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+@pytest.mark.parametrize("R,K,N", [(1, 65536, 16), (3, 65544, 20), (16, 8192, 96), (33, 2048, 16400), (48, 4096, 520), (64, 8200, 64), (64, 16384, 33)])
+def test_few_long_rows(R, K, N, dt):
+    x, w, b, r = linear_case(R, K, N, dt, "gelu", True, True, seed=40)
+    check_linear(x, w, b, r, "gelu", ops.linear(x, w, b, activation="gelu", residual=r))
+    shift = torch.cat([w.new_zeros(1), w.reshape(-1)])[1:].view(N, K)                          # weights off the 16-byte grid: read in place
+    check_linear(x, shift, b, r, "silu", ops.linear(x, shift, b, activation="silu", residual=r))
+    c = gated_case(R, K, N, dt, bias=True, seed=41)
+    check_gated(*c, "silu", ops.gated_linear(*c, activation="silu"))
+    if dt != F32:
+        fp8_layers(R, K, N, dt, [(1, "gelu")])
+
+
 @pytest.mark.parametrize("R,K,N", LARGE)
 def test_large_gradients(R, K, N):
     linear_gradients(R, K, N, BF16, [(2, "gelu")])

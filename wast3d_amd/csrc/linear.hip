@@ -1,7 +1,7 @@
 // Linear and gated linear layers on feature rows: z = x W^T + b;  y = act(z) + residual  /  y = act(x Wg^T + bg) * (x Wu^T + bu), and their gradients.
 //
 // Three kernels do the products (gemm_tile.h has the tile):
-//   * few rows (<= SKINNY_ROWS): the weights are read once, straight into MFMA fragments, by as many waves as there are; the rows are the other operand
+//   * few rows: the weights are read once, straight into MFMA fragments, by as many waves as there are; the rows are the other operand
 //   * tiles of 256 x 256 (gemm_pipe.h), 128 x 128 or 64 x 64 (gemm_tile.h) through LDS
 //   * when the tiles are few for 256 CUs the contraction is cut into slices; partial tiles are added in slice order, and the epilogue applied, by a second launch
 //
@@ -235,18 +235,35 @@ __global__ __launch_bounds__(256) void join_slices_kernel(GemmArgs a) {
     const int64_t z = blockIdx.z, slice = a.M * a.part_ld;
     float c0 = 0.f, c1 = 0.f;
     for (int64_t r0 = (int64_t)blockIdx.y * a.strip; r0 < r_end; r0 += JOIN_ROWS) {
-    float v[JOIN_ROWS / 4], u[JOIN_ROWS / 4];
+    float v[JOIN_ROWS / 4] = {}, u[JOIN_ROWS / 4] = {};
+    const float *p[JOIN_ROWS / 4];                                                             // (rows and columns past the end load the last ones; never stored)
 #pragma unroll
-    for (int i = 0; i < JOIN_ROWS / 4; ++i) {
-        v[i] = u[i] = 0.f;
-        const int64_t m = r0 + 4 * i + wave;
-        if (!in || m >= r_end) continue;
-        const float *p = a.part + (z * a.slices * a.M + m) * a.part_ld + n;
-        for (int s = 0; s < a.slices; ++s) {
-            v[i] += p[s * slice];
-            if (GATED) u[i] += p[s * slice + a.part_ld / 2];
+    for (int i = 0; i < JOIN_ROWS / 4; ++i) p[i] = a.part + (z * a.slices * a.M + min(r0 + 4 * i + wave, r_end - 1)) * a.part_ld + min(n, a.N - 1);
+    auto add = [&](auto run) {                                                                 // RUN slices of every row: all loads first, then the sums in slice order
+        constexpr int RUN = decltype(run)::value;
+        float l[JOIN_ROWS / 4][RUN], h[JOIN_ROWS / 4][RUN];
+#pragma unroll
+        for (int i = 0; i < JOIN_ROWS / 4; ++i) {
+#pragma unroll
+            for (int k = 0; k < RUN; ++k) {
+                l[i][k] = p[i][k * slice];
+                if (GATED) h[i][k] = p[i][k * slice + a.part_ld / 2];
+            }
+            p[i] += RUN * slice;
         }
-    }
+#pragma unroll
+        for (int i = 0; i < JOIN_ROWS / 4; ++i)
+#pragma unroll
+            for (int k = 0; k < RUN; ++k) {
+                v[i] += l[i][k];
+                if (GATED) u[i] += h[i][k];
+            }
+    };
+    int left = a.slices;
+    for (; left >= 8; left -= 8) add(std::integral_constant<int, 8>());
+    if (left & 4) add(std::integral_constant<int, 4>());
+    if (left & 2) add(std::integral_constant<int, 2>());
+    if (left & 1) add(std::integral_constant<int, 1>());
     with_act(a.act, [&](auto act_c) {
         constexpr int ACT = decltype(act_c)::value;
 #pragma unroll
@@ -310,35 +327,45 @@ bool aligned16(const void *p, int64_t ld) { return !(((uintptr_t)p) & 15) && ld 
 
 // How a product is cut: tile size and slices of the contraction, by the time they would take.  Microseconds, fitted to every tile with 1, 2 and 4 slices on 12 sizes of rows 100 .. 65 536 and
 // widths 100 .. 4 096: `lone`, a 128-byte slab of a block that has its CU for itself; `busy`, the same of a block among others, per block on the CU; `round`, start and epilogue of a block.
-// Slices write and read their f32 tiles (2.5 TB/s with the second launch's start).
+// Slices write and read their f32 tiles (2.5 TB/s, and the second launch).  The choices take 4 % longer than the best of all 13 over 18 such sizes, forward, dx and dW.
 struct TileCost { double lone[3], busy[3], round[3]; };      // of 64, 128, 256
-constexpr TileCost COST_16 = {{0.35, 0.6, 1.2}, {0.22, 0.6, 1.3}, {4, 5, 10}}, COST_DW = {{0.57, 0.77, 1.35}, {0.24, 0.85, 1.35}, {4, 5, 10}}, COST_FP8 = {{0.35, 0.6, 0.9}, {0.22, 0.6, 0.9}, {4, 5, 10}},
-                   COST_F32 = {{0.72, 2.25, 0}, {0.62, 2.25, 0}, {4, 5, 0}};
-struct Cut { int tile, slices; int64_t tiles_m, tiles_n; };
+constexpr TileCost COST_16 = {{0.35, 0.6, 1.2}, {0.22, 0.6, 1.3}, {4, 5, 10}}, COST_DW = {{0.57, 0.77, 1.35}, {0.24, 0.5, 1.35}, {4, 5, 10}}, COST_FP8 = {{0.35, 0.6, 0.9}, {0.22, 0.6, 0.9}, {4, 5, 10}},
+                   COST_F32 = {{0.72, 2.25, 0}, {0.62, 2.25, 0}, {4, 5, 0}}, COST_FEW = {{0.8, 0, 0}, {0.4, 0, 0}, {4, 0, 0}};
+enum Products { PLAIN, DW, FEW };      // DW: both operands M_ROWS; FEW: at most SKINNY_ROWS rows (one row of 64-wide tiles; the weights come from HBM, a slab waits for them)
+struct Cut { int tile, slices; int64_t tiles_m, tiles_n; double us; };
 // vec: rows of everything the epilogue touches are aligned, too (the 256 x 256 tile needs it)
-// dw: both operands M_ROWS
-Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool gated, bool vec, int batch, bool dw = false) {
+Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool gated, bool vec, int batch, Products kind = PLAIN) {
     const int parts = gated ? 2 : 1;
     const int64_t slabs = (K * eb_of(dtype) + SLAB - 1) / SLAB;
     Cut best = {};
     double best_t = 0;
     for (int tile = 64; tile <= 256; tile *= 2) {
-        if (tile == 256 && (!vec || dtype == W3D_DTYPE_F32)) break;
+        if ((tile == 256 && (!vec || dtype == W3D_DTYPE_F32)) || (tile > 64 && kind == FEW)) break;
         const int bn = tile / parts;
         const int64_t tm = (M + tile - 1) / tile, tn = (N + bn - 1) / bn, tiles = tm * tn * batch;
         const int k = tile == 64 ? 0 : tile == 128 ? 1 : 2;
-        const TileCost &c = dtype == W3D_DTYPE_F32 ? COST_F32 : dtype == W3D_DTYPE_FP8_E4M3 ? COST_FP8 : dw ? COST_DW : COST_16;
+        const TileCost &c = dtype == W3D_DTYPE_F32 ? COST_F32 : kind == FEW ? COST_FEW : dtype == W3D_DTYPE_FP8_E4M3 ? COST_FP8 : kind == DW ? COST_DW : COST_16;
         const int per_cu = tile == 256 ? 1 : tile == 128 ? 2 : 4;
         for (int s = 1; s <= 32 && (s == 1 || slabs / s >= 4); ++s) {
             const double cu = (double)((tiles * s + 255) / 256), rounds = (double)((tiles * s + 256 * per_cu - 1) / (256 * per_cu)), n = (double)((slabs + s - 1) / s);
             const double a = n * c.busy[k] * cu, b = n * c.lone[k] * rounds;
             double t = (a > b ? a : b) + c.round[k] * rounds;
-            if (s > 1) t += 5.0 + 8.0 * (double)s * (double)batch * (double)M * (double)N * parts / 2.5e6;
-            if (best_t == 0 || t < best_t) { best_t = t; best = {tile, s, tm, tn}; }
+            if (s > 1) t += 3.0 + 8.0 * (double)s * (double)batch * (double)M * (double)N * parts / 2.5e6;
+            if (best_t == 0 || t < best_t) { best_t = t; best = {tile, s, tm, tn, t}; }
         }
     }
     return best;
 }
+// Few rows: do they take skinny_kernel or 64-wide tiles over a sliced contraction?  A skinny block reads its 16 weight rows and ALL of the rows, 27 bytes a nanosecond (measured at 64 .. 16 384
+// columns); long rows onto few columns leave it short of blocks, and many long rows are read once per 16 columns.  us, skinny | tiles, weights from HBM: bf16 4096 -> 4096 1 row 10.3 | 14.2,
+// 16 rows 12.1 | 15.1, 32 rows 17.1 | 15.5, 64 rows 24.7 | 20.7; 1024 -> 4096 64 rows 8.2 | 12.1; 8192 -> 64 1 row 11.3 | 8.0, 64 rows 37.8 | 9.2; 2048 -> 16384 16 rows 23.4 | 32.0, 64 rows
+// 46.3 | 31.8; f32 512 -> 512 64 rows 8.4 | 8.5; f32 4096 -> 4096 16 rows 21.4 | 29.3, 64 rows 55.3 | 36.3.  Unaligned operands are read in place, which beats copying the weights.
+bool few_rows(int64_t R, int64_t K, int64_t N, int dtype, bool gated, bool unaligned, const Cut &tiles) {
+    if (R > SKINNY_ROWS || unaligned) return R <= SKINNY_ROWS;
+    const double blocks = (double)((N + 15) / 16), cu = blocks > 256 ? blocks / 256 : 1;
+    return 2.5 + cu * 16.0 * ((gated ? 2 : 1) + (double)R / 16) * (double)K * eb_of(dtype) / 27e3 <= tiles.us;
+}
+Cut forward_cut(int64_t R, int64_t K, int64_t N, int dtype, bool gated, bool vec) { return cut_of(R, N, K, dtype, gated, vec, 1, R <= SKINNY_ROWS ? FEW : PLAIN); }
 size_t part_bytes(const Cut &c, int64_t M, int64_t N, bool gated, int batch) {
     return c.slices > 1 ? (size_t)batch * c.slices * M * ceil_to(N, 16) * (gated ? 2 : 1) * 4 : 0;
 }
@@ -446,7 +473,10 @@ int forward(const void *x, const int32_t *xs, const void *w, const int32_t *ws, 
     a.out = (uint8_t *)y; a.ld_out = N * eb_of(out_dtype); a.act = act; a.out_dt = out_dtype; a.z = z; a.part_ld = z_stride(N, gated);
     a.vec_io = aligned16(y, a.ld_out) && aligned16(residual, 0) ? 1 : 0;
     const int prod = gated ? PROD_GATED : PROD_LINEAR;
-    if (R <= SKINNY_ROWS) {
+    // (all operands of one side have one row length: an unaligned second weight matrix takes the first along)
+    const bool ux = unaligned(x, K * eb), uw = unaligned(w, K * eb) || unaligned(w2, K * eb);
+    const Cut c = forward_cut(R, K, N, dtype, gated, a.vec_io);
+    if (few_rows(R, K, N, dtype, gated, ux || uw, c)) {
         switch (dtype) {
             case W3D_DTYPE_F32: return w3d_lin_skinny_f32(a, prod, st);
             case W3D_DTYPE_BF16: return w3d_lin_skinny_bf16(a, prod, st);
@@ -454,10 +484,7 @@ int forward(const void *x, const int32_t *xs, const void *w, const int32_t *ws, 
             default: return w3d_lin_skinny_fp8(a, prod, st);
         }
     }
-    const Cut c = cut_of(R, N, K, dtype, gated, a.vec_io, 1);
     Aligner al = {(uint8_t *)workspace, {}, eb};
-    // (all operands of one side have one row length: an unaligned second weight matrix takes the first along)
-    const bool ux = unaligned(x, K * eb), uw = unaligned(w, K * eb) || unaligned(w2, K * eb);
     const int64_t copies = (ux ? copy_bytes(R, K, eb) : 0) + (uw ? (gated ? 2 : 1) * copy_bytes(N, K, eb) : 0);
     const size_t need = (size_t)copies + part_bytes(c, R, N, gated, 1);
     if (need && (!workspace || (((uintptr_t)workspace) & 15) || workspace_bytes < need)) return W3D_ERR_WORKSPACE;
@@ -473,13 +500,16 @@ int forward(const void *x, const int32_t *xs, const void *w, const int32_t *ws, 
 
 // what a call may need: by its sizes, and for tensors that may start at any element (views) the copies on top
 size_t forward_bytes(int64_t R, int64_t K, int64_t N, int dtype, bool gated, bool views) {
-    if (R <= SKINNY_ROWS || K < 1 || N < 1) return 0;
+    if (K < 1 || N < 1) return 0;
     const int eb = eb_of(dtype);
     size_t most = 0;
     for (int vec = 0; vec < 2; ++vec) {
-        const size_t b = part_bytes(cut_of(R, N, K, dtype, gated, vec, 1), R, N, gated, 1);
+        const Cut c = forward_cut(R, K, N, dtype, gated, vec);
+        if (few_rows(R, K, N, dtype, gated, K * eb % 16 != 0, c)) continue;
+        const size_t b = part_bytes(c, R, N, gated, 1);
         most = b > most ? b : most;
     }
+    if (R <= SKINNY_ROWS) return most;                                                        // (no copies)
     return most + (views || K * eb % 16 ? (size_t)(copy_bytes(R, K, eb) + (gated ? 2 : 1) * copy_bytes(N, K, eb)) : 0);
 }
 
@@ -504,7 +534,7 @@ Bwd bwd_plan(int64_t R, int64_t K, int64_t N, int dtype, bool gated, bool no_act
     b.part = 0;
     b.strips = no_act ? w3d_column_strips(R, N) : kept ? join_strips(R) : 0;
     for (int vec = 0; vec < 2; ++vec) {
-        const Cut z = cut_of(R, gated ? b.pad : N, K, dtype, gated, vec, 1), dx = cut_of(R, K, gated ? 2 * b.pad : N, dtype, false, vec, 1), dw = cut_of(N, K, R, dtype, false, vec, parts, true);
+        const Cut z = cut_of(R, gated ? b.pad : N, K, dtype, gated, vec, 1), dx = cut_of(R, K, gated ? 2 * b.pad : N, dtype, false, vec, 1), dw = cut_of(N, K, R, dtype, false, vec, parts, DW);
         if (!no_act && !kept) {
             b.strips = max64(b.strips, strips_of(z, R));
             b.part = max64(b.part, (int64_t)part_bytes(z, R, N, gated, 1));
@@ -595,7 +625,7 @@ int backward(const void *x, const void *w, const void *w2, const void *bias, con
         a.M = N; a.N = K; a.K = R; a.w_rows = R; a.z_x = b.pad * eb;
         a.out = (uint8_t *)o; a.out2 = (uint8_t *)dw2; a.ld_out = K * eb; a.out_dt = dtype; a.part = part;
         a.vec_io = aligned16(o, K * eb) && aligned16(both ? dw2 : nullptr, 0) ? 1 : 0;
-        rc = run_product(a, PROD_DW, dtype, cut_of(N, K, R, dtype, false, a.vec_io, parts, true), both ? 2 : 1, st);
+        rc = run_product(a, PROD_DW, dtype, cut_of(N, K, R, dtype, false, a.vec_io, parts, DW), both ? 2 : 1, st);
         if (rc != W3D_OK) return rc;
     }
     return W3D_OK;

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 
 import torch
 
@@ -1462,7 +1463,15 @@ def _at(t):
     return None if t is None else t.data_ptr()
 
 
-_FEW_ROWS = 64                                                     # the few-row form takes no workspace (w3d_linear_workspace_bytes)
+@functools.lru_cache(4096)
+def _forward_bytes(R: int, K: int, N: int, dtype: int, gated: int, views: int) -> int:
+    """Workspace of a forward call (a function of its sizes alone: asked once)."""
+    return lib().w3d_linear_workspace_bytes(R, K, N, dtype, gated, views)
+
+
+@functools.lru_cache(4096)
+def _backward_bytes(R: int, K: int, N: int, dtype: int, act: int, gated: int, kept: bool, views: int) -> int:
+    return lib().w3d_linear_bwd_workspace_bytes(R, K, N, dtype, act, gated, kept, views)
 
 
 def _scratch(nbytes: int, device):
@@ -1587,7 +1596,7 @@ def raw_linear(x, w, bias, residual, act: int, y, z=None):
     """y [..., N] = act(x [..., K] w [N,K]^T + bias) + residual, contiguous."""
     N, K = w.shape
     R, dt = x.numel() // K, _DTYPE_CODES[x.dtype]
-    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, dt, 0, _views(x, w)) if R > _FEW_ROWS else 0
+    nbytes = _forward_bytes(R, K, N, dt, 0, _views(x, w))
     ws = _scratch(nbytes, x.device) if nbytes else None
     _launch("w3d_linear_fwd", x.get_device(), lib().w3d_linear_fwd, x.data_ptr(), w.data_ptr(), _at(bias), _code(bias), _at(residual), R, K, N, dt, act, y.data_ptr(), _at(z), _at(ws), nbytes)
 
@@ -1596,7 +1605,7 @@ def raw_gated_linear(x, wg, wu, bg, bu, act: int, y, z=None):
     """y [..., N] = act(x wg^T + bg) * (x wu^T + bu), contiguous."""
     N, K = wg.shape
     R, dt = x.numel() // K, _DTYPE_CODES[x.dtype]
-    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, dt, 1, _views(x, wg, wu)) if R > _FEW_ROWS else 0
+    nbytes = _forward_bytes(R, K, N, dt, 1, _views(x, wg, wu))
     ws = _scratch(nbytes, x.device) if nbytes else None
     _launch("w3d_gated_linear_fwd", x.get_device(), lib().w3d_gated_linear_fwd, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), _at(bg), _at(bu), _code(bg if bg is not None else bu), R, K, N,
             dt, act, y.data_ptr(), _at(z), _at(ws), nbytes)
@@ -1631,7 +1640,7 @@ class _Linear(torch.autograd.Function):
             dw, db = (t.zero_() if t is not None else None for t in (dw, db))
         elif want_x or want_w or want_b:
             dt, gyc = _code(x), gy.contiguous()
-            nbytes = lib().w3d_linear_bwd_workspace_bytes(R, K, N, dt, ctx.act, 0, z is not None, _views(x, w, gyc))
+            nbytes = _backward_bytes(R, K, N, dt, ctx.act, 0, z is not None, _views(x, w, gyc))
             ws = _scratch(nbytes, x.device)
             _launch("w3d_linear_bwd", x.get_device(), lib().w3d_linear_bwd, x.data_ptr(), w.data_ptr(), _at(bias), _code(bias), gyc.data_ptr(), _at(z), R, K, N, dt, ctx.act, _at(dx), _at(dw),
                     _at(db), _at(ws), nbytes)
@@ -1684,7 +1693,7 @@ class _GatedLinear(torch.autograd.Function):
             grads = [t.zero_() if t is not None else None for t in grads]
         else:
             dt = _code(x)
-            nbytes = lib().w3d_linear_bwd_workspace_bytes(R, K, N, dt, ctx.act, 1, z is not None, _views(x, wg, wu))
+            nbytes = _backward_bytes(R, K, N, dt, ctx.act, 1, z is not None, _views(x, wg, wu))
             ws, gyc = _scratch(nbytes, x.device), gy.contiguous()
             _launch("w3d_gated_linear_bwd", x.get_device(), lib().w3d_gated_linear_bwd, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), _at(bg), _at(bu), _code(bg if bg is not None else bu),
                     gyc.data_ptr(), _at(z), R, K, N, dt, ctx.act, *(_at(g) for g in grads), _at(ws), nbytes)
@@ -1746,7 +1755,7 @@ def linear_fp8(q, scale, weight_q, weight_scale, bias=None, activation=None, res
     if residual is not None:
         residual = _head_arg("linear_fp8", "residual", residual, (R, N), out_dtype, dev)
     y = torch.empty(R, N, dtype=out_dtype, device=dev)
-    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, FP8, 0, _views(q, weight_q)) if R > _FEW_ROWS else 0
+    nbytes = _forward_bytes(R, K, N, FP8, 0, _views(q, weight_q))
     ws = _scratch(nbytes, dev)
     _launch("w3d_linear_fp8_fwd", dev.index, lib().w3d_linear_fp8_fwd, q.data_ptr(), scale.data_ptr(), weight_q.data_ptr(), weight_scale.data_ptr(), _at(bias), _code(bias), _at(residual),
             R, K, N, code, act, y.data_ptr(), _at(ws), nbytes)
@@ -1763,7 +1772,7 @@ def gated_linear_fp8(q, scale, gate_q, gate_scale, up_q, up_scale, b_gate=None, 
     N, gate_q, up_q, b_gate, b_up = _gated_args("gated_linear_fp8", q, gate_q, up_q, b_gate, b_up, torch.uint8, out_dtype)
     R, K = q.shape
     y = torch.empty(R, N, dtype=out_dtype, device=dev)
-    nbytes = lib().w3d_linear_workspace_bytes(R, K, N, FP8, 1, _views(q, gate_q, up_q)) if R > _FEW_ROWS else 0
+    nbytes = _forward_bytes(R, K, N, FP8, 1, _views(q, gate_q, up_q))
     ws = _scratch(nbytes, dev)
     _launch("w3d_gated_linear_fp8_fwd", dev.index, lib().w3d_gated_linear_fp8_fwd, q.data_ptr(), scale.data_ptr(), gate_q.data_ptr(), gate_scale.data_ptr(), up_q.data_ptr(),
             up_scale.data_ptr(), _at(b_gate), _at(b_up), _code(b_gate if b_gate is not None else b_up), R, K, N, code, act, y.data_ptr(), _at(ws), nbytes)
