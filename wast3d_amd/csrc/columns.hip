@@ -3,7 +3,8 @@
 
 namespace {
 
-// out[c] = sum over p of part[p][c]: 64 columns per block, its sixteen waves take every sixteenth strip, eight loads in flight each (the strips are few and the launch short: latency)
+// out[c] = sum over p of part[p][c]: 64 columns per block, its sixteen waves take every sixteenth strip, eight loads in flight each (the strips are few and the launch short: latency; 128 strips of
+// 4 096 columns 4.9 us)
 template <int DT>
 __global__ __launch_bounds__(1024) void fold_columns_kernel(const float *__restrict__ part, int parts, int64_t ld, int64_t n, void *__restrict__ out) {
     __shared__ float sm[16][64];

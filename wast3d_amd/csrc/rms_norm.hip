@@ -8,6 +8,9 @@
 // Bound by HBM: every element is read once and written once.  A row stays in registers between its sum and its output, in f32; sums are f32.
 // G lanes share a row (a wave holds 64 / G rows), 8 elements per lane and vector, NV vectors per lane: G x NV is the smallest that covers the row, wide
 // rows take the whole block of 256 lanes.  Rows beyond 8 192 elements are read again instead of kept (second and third reading come from L2).
+//
+// Measured, bf16: 1 000 000 x 256 with a residual into 8 bits 327 us (5.5 TB/s); 65 536 x 256 with a residual 22.8 us, backward 27.2 + 4.4 us (fold of dw); kept rows 4.7 - 6.4 TB/s forward,
+// 3.4 - 5.4 backward (131 072 x 256 .. 16 384 x 8 192), rows read again 3.4 - 3.7 and 2.4 (16 384 wide).
 #include "rows16.h"
 
 namespace {
@@ -308,13 +311,15 @@ static int bwd_blocks(int64_t R, int rows_per_block) {
     return (int)(n < 1 ? 1 : n > 1024 ? 1024 : n);
 }
 struct Shape { int g, nv; };
-// lanes per row and vectors per lane: the smallest power-of-two group whose one vector covers the row; past 512 elements a wave holds two to four vectors a lane, past 2 048 the block does
+// Lanes per row and vectors per lane: the smallest power-of-two group whose one vector covers the row; past 512 elements a wave holds two vectors a lane, past 1 024 the block takes the row.
+// us forward | backward with dw, bf16, this choice against the next one: 131 072 x 64, 8 lanes 10.2 | 19.2, 16 lanes 13.9 | 23.9; x 256, 32 lanes 23.5 | 39.6, 64 lanes 32.9 | 61.1; x 1 024,
+// two vectors 98.6 | 152, the block 117 | 256; 65 536 x 2 048, the block 97.6 | 163, four vectors of a wave 111 | 232; 32 768 x 4 096, the block 99 | 162, eight vectors of a wave 204 | 405.
 static Shape shape_of(int d) {
     const int v = (d + 7) / 8;
     for (int g = 8; g <= 64; g *= 2)
         if (v <= g) return {g, 1};
     if (v <= 128) return {64, 2};
-    if (v <= 256) return {64, 4};
+    if (v <= 256) return {256, 1};
     if (v <= 512) return {256, 2};
     if (v <= 1024) return {256, 4};
     return {0, 0};
@@ -334,7 +339,7 @@ static int launch_fwd(const NormArgs &a, hipStream_t st) {
     else if (sh.g == 32) W3D_NORM(32, 1);
     else if (sh.g == 64 && sh.nv == 1) W3D_NORM(64, 1);
     else if (sh.g == 64 && sh.nv == 2) W3D_NORM(64, 2);
-    else if (sh.g == 64) W3D_NORM(64, 4);
+    else if (sh.nv == 1) W3D_NORM(256, 1);
     else if (sh.nv == 2) W3D_NORM(256, 2);
     else W3D_NORM(256, 4);
 #undef W3D_NORM
@@ -355,7 +360,7 @@ static int launch_bwd(const NormBwdArgs &a, int blocks, hipStream_t st) {
     else if (sh.g == 32) W3D_NORM(32, 1);
     else if (sh.g == 64 && sh.nv == 1) W3D_NORM(64, 1);
     else if (sh.g == 64 && sh.nv == 2) W3D_NORM(64, 2);
-    else if (sh.g == 64) W3D_NORM(64, 4);
+    else if (sh.nv == 1) W3D_NORM(256, 1);
     else if (sh.nv == 2) W3D_NORM(256, 2);
     else W3D_NORM(256, 4);
 #undef W3D_NORM
@@ -363,7 +368,10 @@ static int launch_bwd(const NormBwdArgs &a, int blocks, hipStream_t st) {
 }
 static int blocks_for(int64_t R, int d) {
     const Shape sh = shape_of(d);
-    if (!sh.g) return (int)(R < 64 ? R : 64);
+    if (!sh.g) {                                                          // strips of rows: 2 048 blocks together with those across the columns
+        const int across = (d + NORM_BLOCK * 8 - 1) / (NORM_BLOCK * 8), strips = (2048 + across - 1) / across;
+        return (int)(R < strips ? R : strips);
+    }
     return bwd_blocks(R, NORM_BLOCK / sh.g);
 }
 static bool dtype_ok(int t) { return t == W3D_DTYPE_F32 || t == W3D_DTYPE_BF16 || t == W3D_DTYPE_F16; }
