@@ -42,7 +42,7 @@ struct GemmArgs {
     int64_t part_ld;
     float *z;                           // forward, f32: where the values before the activation go, [M][part_ld] (gated: the second half part_ld / 2 further), or NULL
     int64_t strip;                      // rows of one partial column sum of the joining launch
-    int bias_f32, act, slices, tiles_m, tiles_n, vec_io, out_dt;
+    int bias_f32, act, slices, tiles_m, tiles_n, out_dt;
 };
 }  // namespace w3d_lin
 using w3d_lin::GemmArgs;
@@ -110,16 +110,19 @@ __device__ __forceinline__ void with_act(int act, F f) {
     }
 }
 
-// ---- runs of CNT (4, 8 or 16) consecutive elements of a row, `n` of them inside; vec: the row is 16-byte aligned at 8-element steps
+// ---- runs of CNT (4, 8 or 16) consecutive elements of a row, `n` of them inside, at any alignment (global memory takes vector accesses at any element; element
+// by element the four products of 4 999 x 999 -> 515 f16 in training took 14 us more of 110)
+typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef int i32x2_any __attribute__((ext_vector_type(2), aligned(2)));
 template <int DT, int CNT>
-__device__ __forceinline__ void load_run(const uint8_t *p, int64_t n, bool vec, float (&v)[CNT]) {
+__device__ __forceinline__ void load_run(const uint8_t *p, int64_t n, float (&v)[CNT]) {
     constexpr int EB = Elem<DT>::B;
-    if (vec && n >= CNT) {
+    if (n >= CNT) {
         uint32_t w[CNT * EB / 4];
         if (CNT * EB >= 16) {
 #pragma unroll
-            for (int i = 0; i < CNT * EB / 16; ++i) { const i32x4 t = reinterpret_cast<const i32x4 *>(p)[i]; __builtin_memcpy(&w[4 * i], &t, 16); }
-        } else { const uint2 t = *reinterpret_cast<const uint2 *>(p); w[0] = t.x; w[1] = t.y; }
+            for (int i = 0; i < CNT * EB / 16; ++i) { const i32x4 t = reinterpret_cast<const i32x4_any *>(p)[i]; __builtin_memcpy(&w[4 * i], &t, 16); }
+        } else { const i32x2_any t = *reinterpret_cast<const i32x2_any *>(p); w[0] = t.x; w[1] = t.y; }
 #pragma unroll
         for (int i = 0; i < CNT; ++i) {
             if (DT == W3D_DTYPE_F32) v[i] = __uint_as_float(w[i]);
@@ -153,9 +156,9 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {                   
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
 }
 template <int DT, int CNT>
-__device__ __forceinline__ void store_run(uint8_t *p, int64_t n, bool vec, const float (&v)[CNT]) {
+__device__ __forceinline__ void store_run(uint8_t *p, int64_t n, const float (&v)[CNT]) {
     constexpr int EB = Elem<DT>::B;
-    if (vec && n >= CNT) {
+    if (n >= CNT) {
         uint32_t w[CNT * EB / 4];
 #pragma unroll
         for (int i = 0; i < CNT * EB / 4; ++i) {
@@ -164,8 +167,8 @@ __device__ __forceinline__ void store_run(uint8_t *p, int64_t n, bool vec, const
         }
         if (CNT * EB >= 16) {
 #pragma unroll
-            for (int i = 0; i < CNT * EB / 16; ++i) { i32x4 t; __builtin_memcpy(&t, &w[4 * i], 16); reinterpret_cast<i32x4 *>(p)[i] = t; }
-        } else *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+            for (int i = 0; i < CNT * EB / 16; ++i) { i32x4 t; __builtin_memcpy(&t, &w[4 * i], 16); reinterpret_cast<i32x4_any *>(p)[i] = t; }
+        } else *reinterpret_cast<i32x2_any *>(p) = i32x2_any{(int)w[0], (int)w[1]};
         return;
     }
 #pragma unroll
@@ -275,7 +278,7 @@ struct Out {
         const int64_t mw = m0 + wm * (BM / WM), left64 = a.M - mw - lane / LPR;
         const int left = (int)(left64 < BM ? left64 < -BM ? -BM : left64 : BM);                // rows from the lane's first that exist (<= 0: none)
         const bool any = a.M > mw && a.N > c0;                                                 // the wave's corner is inside C (uniform)
-        const bool fast = VEC || (a.vec_io && n + 8 <= a.N);
+        const bool fast = VEC || n + 8 <= a.N;
         i32x4 ring[AHEAD][RAW];                                                                // src of the next passes (indexed at compile time: a rotation would wait for the loads)
         const uint32_t src_ld = (uint32_t)(a.N * OB);
         const uint8_t *from = src + mw * a.N * OB + c0 * OB;                                   // the wave's corner: uniform, lanes add 32 bits
@@ -285,7 +288,7 @@ struct Out {
             const int r = VEC ? (q * RPP < left ? q * RPP : left - 1) : q * RPP;
             if (VEC ? any : fast && r < left)
 #pragma unroll
-                for (int k = 0; k < RAW; ++k) ring[slot][k] = reinterpret_cast<const i32x4 *>(from + (uint32_t)(lane / LPR + r) * src_ld + col)[k];
+                for (int k = 0; k < RAW; ++k) ring[slot][k] = reinterpret_cast<const i32x4_any *>(from + (uint32_t)(lane / LPR + r) * src_ld + col)[k];
         };
         if (SRC)
 #pragma unroll
@@ -304,7 +307,7 @@ struct Out {
                     float t[8] = {};
                     if (SRC) {
                         if (fast) unpack8<OT>(ring[(c * PASSES + k) % AHEAD], t);
-                        else if (!VEC && row < left) load_run<OT, 8>(from + (uint32_t)(lane / LPR + row) * src_ld + (uint32_t)(n - c0) * OB, a.N - n, false, t);
+                        else if (!VEC && row < left) load_run<OT, 8>(from + (uint32_t)(lane / LPR + row) * src_ld + (uint32_t)(n - c0) * OB, a.N - n, t);
                         if (q + AHEAD < ALL) fetch(q + AHEAD, (c * PASSES + k) % AHEAD);
                     }
                     f(p, row, row < left, t, off);
@@ -324,7 +327,7 @@ struct Out {
                 for (int p = 0; p < PARTS; ++p) {
                     float v[8];
                     get(patch, pass, p, lane, v);
-                    if (live && n < a.N) store_run<W3D_DTYPE_F32, 8>(out + off + p * (ld / 2), VEC ? 8 : a.N - n, true, v);
+                    if (live && n < a.N) store_run<W3D_DTYPE_F32, 8>(out + off + p * (ld / 2), VEC ? 8 : a.N - n, v);
                 }
             });
             return;
@@ -339,14 +342,13 @@ struct Out {
     template <int OT>
     static __device__ __forceinline__ void finish(const GemmArgs &a, const Acc &acc, int64_t m0, int64_t n, int64_t col0, int tm, int wm, int lane, bool z1, uint8_t *patch) {
         constexpr int OB = Elem<OT>::B;
-        const bool vec = a.vec_io != 0;
         const int64_t mw = m0 + wm * (BM / WM);
         uint8_t *out = (EPI == EPI_STORE && z1 ? a.out2 : a.out) + mw * a.ld_out + col0 * OB;
         if constexpr (EPI == EPI_STORE) {
             each_row<OT, OB, false>(a, acc, nullptr, a.ld_out, m0, n, col0, wm, lane, patch, [&](int pass, int, bool live, float (&)[8], uint32_t off) {
                 float v[8];
                 get(patch, pass, 0, lane, v);
-                if (live && n < a.N) store_run<OT, 8>(out + off, VEC ? 8 : a.N - n, VEC || vec, v);
+                if (live && n < a.N) store_run<OT, 8>(out + off, VEC ? 8 : a.N - n, v);
             });
             return;
         }
@@ -374,8 +376,8 @@ struct Out {
             for (int e = 0; e < 8; ++e) { v[e] += b0[e]; if (GATED) u[e] += b1[e]; }
             if (DT == W3D_DTYPE_F32 && !BWD && a.z && live && n < a.N) {
                 float *z = a.z + (mw + lane / LPR + r) * a.part_ld + n;
-                store_run<W3D_DTYPE_F32, 8>((uint8_t *)z, a.N - n, true, v);
-                if (GATED) store_run<W3D_DTYPE_F32, 8>((uint8_t *)(z + a.part_ld / 2), a.N - n, true, u);
+                store_run<W3D_DTYPE_F32, 8>((uint8_t *)z, a.N - n, v);
+                if (GATED) store_run<W3D_DTYPE_F32, 8>((uint8_t *)(z + a.part_ld / 2), a.N - n, u);
             }
             auto apply = [&](auto act) {
                 constexpr int ACT = decltype(act)::value;
@@ -407,8 +409,8 @@ struct Out {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) { c0[e] += live ? v[e] : 0.f; if (GATED) c1[e] += live ? u[e] : 0.f; }      // column sums in f32, before the rounding
             if (live && (BWD ? pad > 0 : n < a.N)) {
-                store_run<OT, 8>(out + off, VEC ? 8 : BWD ? pad : a.N - n, VEC || BWD || vec, v);
-                if (EPI == EPI_GATED_BWD) store_run<OT, 8>(out + off + a.half_out, VEC ? 8 : pad, true, u);
+                store_run<OT, 8>(out + off, VEC ? 8 : BWD ? pad : a.N - n, v);
+                if (EPI == EPI_GATED_BWD) store_run<OT, 8>(out + off + a.half_out, VEC ? 8 : pad, u);
             }
         };
         auto rows = [&](auto act_c, auto src_c) {

@@ -7,7 +7,8 @@
 //
 // Backward keeps nothing of a 16-bit forward pass but its inputs: z is formed again and turned into dz in the epilogue, where the column sums for the bias
 // gradient are taken too — storing z in 16 bits would put its rounding into every gradient, storing it in 32 costs more traffic than forming it again
-// (R x N x 12 bytes written and read, against 2 R N K operations).  An f32 forward pass keeps z (at a tenth of the 16-bit rate forming it again is the dearer way).  dz is rounded once to the operands' type (it is an operand of two products); sums are f32.
+// (R x N x 12 bytes written and read, against 2 R N K operations).  An f32 forward pass keeps z (at a tenth of the 16-bit rate forming it again is the dearer way).  dz is rounded once to the
+// operands' type (it is an operand of two products); sums are f32.
 //
 // One translation unit per operand type (W3D_LIN_DT: the tiles), one for the entry points.
 #include "gemm_pipe.h"
@@ -82,8 +83,8 @@ int launch_prod(const GemmArgs &a, int prod, int tile, int z, hipStream_t st) {
 }
 
 // ---- few rows.  Bound by the weights: every one is read once.  A block owns 16 columns (of each half of a gated layer); its waves share the contraction in turns of STEP_RUN steps of 64
-// bytes, a lane loading 16 bytes of one weight row per step, so that a row's 256 consecutive bytes are in flight together (runs of 8 steps: 9.5 instead of 10.3 us for one row below, but 13.0 instead of 12.1 for 16); rows of any alignment
-// are read in place.  The waves' partial sums meet in LDS.  Measured, weights from HBM: bf16 4096 -> 4096, 1 row 10.3 us (3.2 TB/s with the launch), 16 rows 12.1; fp8 8.1 and 8.5; gated 1024 -> 2816
+// bytes, a lane loading 16 bytes of one weight row per step, so that a row's 256 consecutive bytes are in flight together (runs of 8 steps: 9.5 instead of 10.3 us for one row below, but 13.0 instead of 12.1 for 16); rows of any
+// alignment are read in place.  The waves' partial sums meet in LDS.  Measured, weights from HBM: bf16 4096 -> 4096, 1 row 10.3 us (3.2 TB/s with the launch), 16 rows 12.1; fp8 8.1 and 8.5; gated 1024 -> 2816
 // 5.9 us.
 template <int EPI, int RF>
 __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
@@ -220,8 +221,8 @@ int W3D_LIN_NAME(w3d_lin_skinny)(const GemmArgs &a, int prod, hipStream_t st) {
 namespace {
 
 // Partial sums of a sliced product: part[slice][m][ld] -> the epilogue of the product (one slice: the values before the activation that an f32 forward pass kept, for the gradient's).  A block
-// takes 64 columns of a strip of rows (a multiple of JOIN_ROWS), JOIN_ROWS at a time (a quarter per wave), so that the column sums of dz are complete per strip; up to 8 slices of every row are loaded before the first sum (one after another, 16 slices
-// of 16 rows waited 12 us).  Measured: 4 slices of 1024 x 4096 in f32, 75 MB, 18 us.
+// takes 64 columns of a strip of rows (a multiple of JOIN_ROWS), JOIN_ROWS at a time (a quarter per wave), so that the column sums of dz are complete per strip; up to 8
+// slices of every row are loaded before the first sum (one after another, 16 slices of 16 rows waited 12 us).  Measured: 4 slices of 1024 x 4096 in f32, 75 MB, 18 us.
 constexpr int JOIN_ROWS = 16;
 template <int OT, int EPI>
 __global__ __launch_bounds__(256) void join_slices_kernel(GemmArgs a) {
@@ -473,11 +474,11 @@ int forward(const void *x, const int32_t *xs, const void *w, const int32_t *ws, 
     a.bias = (const uint8_t *)bias; a.bias2 = (const uint8_t *)bias2; a.bias_f32 = bias_dtype == W3D_DTYPE_F32 && out_dtype != W3D_DTYPE_F32;
     a.res = (const uint8_t *)residual; a.xs = xs; a.ws = ws; a.ws2 = ws2;
     a.out = (uint8_t *)y; a.ld_out = N * eb_of(out_dtype); a.act = act; a.out_dt = out_dtype; a.z = z; a.part_ld = z_stride(N, gated);
-    a.vec_io = aligned16(y, a.ld_out) && aligned16(residual, 0) ? 1 : 0;
+    const bool vec = aligned16(y, a.ld_out) && aligned16(residual, 0);
     const int prod = gated ? PROD_GATED : PROD_LINEAR;
     // (all operands of one side have one row length: an unaligned second weight matrix takes the first along)
     const bool ux = unaligned(x, K * eb), uw = unaligned(w, K * eb) || unaligned(w2, K * eb);
-    const Cut c = forward_cut(R, K, N, dtype, gated, a.vec_io);
+    const Cut c = forward_cut(R, K, N, dtype, gated, vec);
     if (few_rows(R, K, N, dtype, gated, ux || uw, c)) {
         switch (dtype) {
             case W3D_DTYPE_F32: return w3d_lin_skinny_f32(a, prod, st);
@@ -581,7 +582,6 @@ int backward(const void *x, const void *w, const void *w2, const void *bias, con
         a.x = X; a.w = W; a.w2 = W2; a.ldx = ldx; a.ldw = ldw; a.M = R; a.N = N; a.K = K;
         a.bias = (const uint8_t *)bias; a.bias2 = (const uint8_t *)bias2; a.bias_f32 = bias_dtype == W3D_DTYPE_F32 && dtype != W3D_DTYPE_F32;
         a.dy = (const uint8_t *)dy; a.out = dz_buf; a.ld_out = b.ld_dz; a.half_out = b.pad * eb; a.act = act; a.out_dt = dtype;
-        a.vec_io = aligned16(dy, N * eb) ? 1 : 0;
         a.colsum = db || db2 ? colsum : nullptr; a.colsum_ld = b.colsum_ld; a.part = part;
         const int prod = gated ? PROD_GATED_BWD : PROD_LINEAR_BWD;
         if (z) {
@@ -590,7 +590,7 @@ int backward(const void *x, const void *w, const void *w2, const void *bias, con
             rc = join(a, prod, 1, st);
             strips = join_strips(R);
         } else {
-            const Cut c = cut_of(R, gated ? b.pad : N, K, dtype, gated, a.vec_io, 1);          // (the tiles write the padding columns too)
+            const Cut c = cut_of(R, gated ? b.pad : N, K, dtype, gated, aligned16(dy, N * eb), 1);          // (the tiles write the padding columns too)
             rc = run_product(a, prod, dtype, c, 1, st);
             strips = strips_of(c, R);
         }
@@ -608,8 +608,7 @@ int backward(const void *x, const void *w, const void *w2, const void *bias, con
         a.x = dz; a.ldx = ld_dz; a.w = W; a.w2 = W2; a.ldw = ldw;
         a.M = R; a.N = K; a.K = gated ? 2 * b.pad : N; a.k_split = gated ? b.pad : 0; a.w_rows = N;
         a.out = (uint8_t *)dx; a.ld_out = K * eb; a.out_dt = dtype; a.part = part;
-        a.vec_io = aligned16(dx, K * eb) ? 1 : 0;
-        rc = run_product(a, PROD_DX, dtype, cut_of(R, K, a.K, dtype, false, a.vec_io, 1), 1, st);
+        rc = run_product(a, PROD_DX, dtype, cut_of(R, K, a.K, dtype, false, aligned16(dx, K * eb), 1), 1, st);
         if (rc != W3D_OK) return rc;
     }
     // weight gradients: the two halves of a gated layer are one launch (blockIdx.z) when both are wanted
@@ -626,8 +625,8 @@ int backward(const void *x, const void *w, const void *w2, const void *bias, con
         a.x = dz + (h ? b.pad * eb : 0); a.ldx = ld_dz; a.w = X; a.ldw = ldx;
         a.M = N; a.N = K; a.K = R; a.w_rows = R; a.z_x = b.pad * eb;
         a.out = (uint8_t *)o; a.out2 = (uint8_t *)dw2; a.ld_out = K * eb; a.out_dt = dtype; a.part = part;
-        a.vec_io = aligned16(o, K * eb) && aligned16(both ? dw2 : nullptr, 0) ? 1 : 0;
-        rc = run_product(a, PROD_DW, dtype, cut_of(N, K, R, dtype, false, a.vec_io, parts, DW), both ? 2 : 1, st);
+        const bool vec = aligned16(o, K * eb) && aligned16(both ? dw2 : nullptr, 0);
+        rc = run_product(a, PROD_DW, dtype, cut_of(N, K, R, dtype, false, vec, parts, DW), both ? 2 : 1, st);
         if (rc != W3D_OK) return rc;
     }
     return W3D_OK;
