@@ -371,6 +371,18 @@ def test_rms_norm_fp8(R, d, dt):
         assert torch.equal(e, e2) and torch.equal(q.view(torch.float8_e4m3fn).float(), q2.view(torch.float8_e4m3fn).float())
 
 
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("R,d", [(200000, 256), (300, 2056), (40, 9000)])
+def test_rms_norm_fp8_is_the_rounded_definition(R, d, dt):
+    """8-bit rows are the 64-bit rows rounded to f32 and then to e4m3: no value falls on the other side of a border (the sums' orders differ by 2^-50)."""
+    x, w = rnd(R, d, seed=51, dtype=dt), (1 + 0.1 * rnd(d, seed=52)).to(dt)
+    q, e = ops.rms_norm_fp8(x, w)
+    y = (x.double() * (1 / torch.sqrt(x.double().square().mean(1, keepdim=True) + float(torch.tensor(1e-6)))) * w.double()).float()
+    m, ex = torch.frexp(y.abs().amax(1))
+    assert torch.equal(e, torch.where(m <= 0.875, ex - 9, ex - 8) + 127)
+    assert torch.equal(dequant(q, e), (y.double() * torch.exp2(127.0 - e.double())[:, None]).float().to(torch.float8_e4m3fn).double() * torch.exp2(e.double() - 127)[:, None])
+
+
 def test_rms_norm_only_the_sum_is_used():
     x, r, w = (rnd(40, 96, seed=i).requires_grad_(True) for i in (1, 2, 3))
     w = rnd(96, seed=3).requires_grad_(True)

@@ -5,12 +5,15 @@
 //   given dy (and ds, what reaches s from elsewhere):  g = dy w;  x^ = s r;  dx = r (g - x^ mean(g x^)) + ds;  dw = sum over rows of dy x^
 // The backward pass forms s again from x and the residual, unrounded: from the rounded s its error would show in dw (1.5 x the error of one rounding).
 //
-// Bound by HBM: every element is read once and written once.  A row stays in registers between its sum and its output, in f32; sums are f32.
+// Bound by HBM: every element is read once and written once.  A row stays in registers between its sum and its output, in f32.  Sums are f32 for 16-bit rows.
+// For 8-bit rows the forward pass is 64-bit between the loads and one rounding to f32: what 32 bits lose (2^-23 or so) moves values over e4m3's borders by whole steps: 100 - 127 of 256 million at
+// 1 000 000 x 256, none this way (360 us; 327 in 32 bits).  f32 rows are formed alike, so that quantising them afterwards gives the same bytes.
 // G lanes share a row (a wave holds 64 / G rows), 8 elements per lane and vector, NV vectors per lane: G x NV is the smallest that covers the row, wide
 // rows take the whole block of 256 lanes.  Rows beyond 8 192 elements are read again instead of kept (second and third reading come from L2).
 //
-// Measured, bf16: 1 000 000 x 256 with a residual into 8 bits 327 us (5.5 TB/s); 65 536 x 256 with a residual 22.8 us, backward 27.2 + 4.4 us (fold of dw); kept rows 4.7 - 6.4 TB/s forward,
+// Measured, bf16: 1 000 000 x 256 with a residual into 8 bits 360 us (5.0 TB/s); 65 536 x 256 with a residual 22.8 us, backward 27.2 + 4.4 us (fold of dw); kept rows 4.7 - 6.4 TB/s forward,
 // 3.4 - 5.4 backward (131 072 x 256 .. 16 384 x 8 192), rows read again 3.4 - 3.7 and 2.4 (16 384 wide).
+#include <type_traits>
 #include "rows16.h"
 
 namespace {
@@ -25,7 +28,8 @@ struct NormArgs {
     int32_t *scale;
     int64_t R;
     int d, w_f32;
-    float eps, inv_d;
+    float eps;
+    double inv_d;
 };
 
 template <int DT>
@@ -50,20 +54,28 @@ __device__ __forceinline__ void sum_row(const A &a, int64_t at, int c, float (&s
 }
 
 // sum / maximum over the G lanes of a row; G = 256: over the block (red: 4 floats of LDS per slot; every lane of the block calls)
-template <int G, bool MAX>
-__device__ __forceinline__ float group_reduce(float v, float *red) {
+template <int G, bool MAX, typename T>
+__device__ __forceinline__ T group_reduce(T v, T *red) {
+    auto op = [](T a, T b) { return MAX ? (T)fmaxf(a, b) : a + b; };
 #pragma unroll
-    for (int o = (G < 64 ? G : 64) / 2; o > 0; o >>= 1) {
-        const float t = __shfl_xor(v, o, 64);
-        v = MAX ? fmaxf(v, t) : v + t;
-    }
+    for (int o = (G < 64 ? G : 64) / 2; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
     if (G == 256) {
         __syncthreads();
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = MAX ? fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])) : (red[0] + red[1]) + (red[2] + red[3]);
+        v = op(op(red[0], red[1]), op(red[2], red[3]));
     }
     return v;
+}
+
+// The forward pass's type: 64 bits for 8-bit rows, and for f32 ones (the same rows, quantised afterwards, are the same bytes)
+template <int DT, bool Q> struct Wide { typedef typename std::conditional<Q || DT == W3D_DTYPE_F32, double, float>::type T; };
+__device__ __forceinline__ float inverse_rms(float sum, const NormArgs &a) { return 1.0f / sqrtf(sum * (float)a.inv_d + a.eps); }
+// 1 / sqrt(mean + eps) of a row's 64-bit sum of squares: the 32-bit value and one Newton step in 64 bits.  Where that step is not a number (a mean of 0, infinity, NaN or past 32 bits) the first
+// value stands.
+__device__ __forceinline__ double inverse_rms(double sum, const NormArgs &a) {
+    const double v = sum * a.inv_d + (double)a.eps, r0 = (double)(1.0f / sqrtf((float)v)), r = r0 * fma(-0.5 * v * r0, r0, 1.5);
+    return r > 0.0 && r < 1e300 ? r : r0;
 }
 
 // the E8M0 exponent of a row: the smallest power of two that takes amax into e4m3's range (448 = 0.875 2^9), 127 for a row of zeros (or one without a finite maximum below 2^127)
@@ -89,10 +101,12 @@ __device__ __forceinline__ void store_fp8(uint8_t *p, int n, const float (&v)[8]
         if (i < n) p[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
 }
 
-template <int DT, int G, int NV>
+template <int DT, int G, int NV, bool Q>
 __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_kernel(NormArgs a) {
+    typedef typename Wide<DT, Q>::T T;
     constexpr int EB = Elem<DT>::B, RPB = NORM_BLOCK / G;
     __shared__ float red[4];
+    __shared__ T red_sum[4];
     const int gl = threadIdx.x & (G - 1), c0 = gl * 8;
     float w[NV][8];
 #pragma unroll
@@ -101,7 +115,8 @@ __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_kernel(NormArgs a) {
         const int64_t r = r0 + threadIdx.x / G;
         const bool live = r < a.R;
         const int64_t at = (live ? r : a.R - 1) * a.d;
-        float s[NV][8], sum = 0.f;
+        float s[NV][8];
+        T sum = 0;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int c = c0 + v * G * 8;
@@ -110,10 +125,9 @@ __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_kernel(NormArgs a) {
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(s[v][i], s[v][i], sum);
-        sum = group_reduce<G, false>(sum, red);
-        const float rs = 1.0f / sqrtf(sum * a.inv_d + a.eps);
-        if (a.rstd && live && gl == 0) a.rstd[r] = rs;
+            for (int i = 0; i < 8; ++i) sum = fma((T)s[v][i], (T)s[v][i], sum);
+        const T rs = inverse_rms(group_reduce<G, false>(sum, red_sum), a);
+        if (a.rstd && live && gl == 0) a.rstd[r] = (float)rs;
         if (a.s && live) {
 #pragma unroll
             for (int v = 0; v < NV; ++v) { const int c = c0 + v * G * 8; store8<DT>(a.s + (at + c) * EB, a.d - c, s[v]); }
@@ -122,12 +136,12 @@ __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_kernel(NormArgs a) {
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) { s[v][i] = s[v][i] * rs * w[v][i]; amax = fmaxf(amax, fabsf(s[v][i])); }
-        if (a.y && live) {
+            for (int i = 0; i < 8; ++i) { s[v][i] = (float)((T)s[v][i] * rs * (T)w[v][i]); amax = fmaxf(amax, fabsf(s[v][i])); }
+        if (!Q && live) {
 #pragma unroll
             for (int v = 0; v < NV; ++v) { const int c = c0 + v * G * 8; store8<DT>(a.y + (at + c) * EB, a.d - c, s[v]); }
         }
-        if (a.q) {
+        if (Q) {
             const int e = e8m0_of(group_reduce<G, true>(amax, red));
             const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
             if (live) {
@@ -140,31 +154,33 @@ __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_kernel(NormArgs a) {
 }
 
 // rows of more than 256 x 8 x 4 elements: one block per row, the row read again for every pass over it
-template <int DT>
+template <int DT, bool Q>
 __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_wide_kernel(NormArgs a) {
+    typedef typename Wide<DT, Q>::T T;
     constexpr int EB = Elem<DT>::B;
     __shared__ float red[4];
+    __shared__ T red_sum[4];
     for (int64_t r = blockIdx.x; r < a.R; r += gridDim.x) {
         const int64_t at = r * a.d;
-        float sum = 0.f, s[8], w[8];
+        float s[8], w[8];
+        T sum = 0;
         for (int c = threadIdx.x * 8; c < a.d; c += NORM_BLOCK * 8) {
             sum_row<DT>(a, at, c, s);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(s[i], s[i], sum);
+            for (int i = 0; i < 8; ++i) sum = fma((T)s[i], (T)s[i], sum);
         }
-        sum = group_reduce<256, false>(sum, red);
-        const float rs = 1.0f / sqrtf(sum * a.inv_d + a.eps);
-        if (a.rstd && threadIdx.x == 0) a.rstd[r] = rs;
+        const T rs = inverse_rms(group_reduce<256, false>(sum, red_sum), a);
+        if (a.rstd && threadIdx.x == 0) a.rstd[r] = (float)rs;
         float amax = 0.f;
         for (int c = threadIdx.x * 8; c < a.d; c += NORM_BLOCK * 8) {
             sum_row<DT>(a, at, c, s);
             load_weight<DT>(a.w, a.w_f32, c, a.d, w);
             if (a.s) store8<DT>(a.s + (at + c) * EB, a.d - c, s);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) { s[i] = s[i] * rs * w[i]; amax = c + i < a.d ? fmaxf(amax, fabsf(s[i])) : amax; }
-            if (a.y) store8<DT>(a.y + (at + c) * EB, a.d - c, s);
+            for (int i = 0; i < 8; ++i) { s[i] = (float)((T)s[i] * rs * (T)w[i]); amax = c + i < a.d ? fmaxf(amax, fabsf(s[i])) : amax; }
+            if (!Q) store8<DT>(a.y + (at + c) * EB, a.d - c, s);
         }
-        if (!a.q) continue;
+        if (!Q) continue;
         const int e = e8m0_of(group_reduce<256, true>(amax, red));
         const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
         if (threadIdx.x == 0) a.scale[r] = e;
@@ -172,7 +188,7 @@ __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_wide_kernel(NormArgs a) {
             sum_row<DT>(a, at, c, s);
             load_weight<DT>(a.w, a.w_f32, c, a.d, w);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] = s[i] * rs * w[i];
+            for (int i = 0; i < 8; ++i) s[i] = (float)((T)s[i] * rs * (T)w[i]);
             store_fp8(a.q + at + c, a.d - c, s, inv);
         }
     }
@@ -325,15 +341,15 @@ static Shape shape_of(int d) {
     return {0, 0};
 }
 
-template <int DT>
+template <int DT, bool Q>
 static int launch_fwd(const NormArgs &a, hipStream_t st) {
     const Shape sh = shape_of(a.d);
     if (!sh.g) {
-        hipLaunchKernelGGL(rms_norm_wide_kernel<DT>, dim3((unsigned)(a.R < 4096 ? a.R : 4096)), dim3(NORM_BLOCK), 0, st, a);
+        hipLaunchKernelGGL((rms_norm_wide_kernel<DT, Q>), dim3((unsigned)(a.R < 4096 ? a.R : 4096)), dim3(NORM_BLOCK), 0, st, a);
         return W3D_OK;
     }
     const dim3 grid(w3d_grid(a.R, NORM_BLOCK / sh.g, 8192)), block(NORM_BLOCK);
-#define W3D_NORM(G, NV) hipLaunchKernelGGL((rms_norm_kernel<DT, G, NV>), grid, block, 0, st, a)
+#define W3D_NORM(G, NV) hipLaunchKernelGGL((rms_norm_kernel<DT, G, NV, Q>), grid, block, 0, st, a)
     if (sh.g == 8) W3D_NORM(8, 1);
     else if (sh.g == 16) W3D_NORM(16, 1);
     else if (sh.g == 32) W3D_NORM(32, 1);
@@ -386,10 +402,11 @@ static int rms_norm_any(const void *x, const void *residual, const void *weight,
     if (R == 0) return W3D_OK;
     if (!x || (s && !residual)) return W3D_ERR_ARG;
     NormArgs a = {(const char *)x, (const char *)residual, (const char *)weight, (char *)y, (char *)s, rstd, (uint8_t *)q, scale, R, d,
-                  weight_dtype == W3D_DTYPE_F32 && dtype != W3D_DTYPE_F32, eps, 1.0f / (float)d};
-    if (dtype == W3D_DTYPE_F32) launch_fwd<W3D_DTYPE_F32>(a, w3d_s(stream));
-    else if (dtype == W3D_DTYPE_BF16) launch_fwd<W3D_DTYPE_BF16>(a, w3d_s(stream));
-    else launch_fwd<W3D_DTYPE_F16>(a, w3d_s(stream));
+                  weight_dtype == W3D_DTYPE_F32 && dtype != W3D_DTYPE_F32, eps, 1.0 / (double)d};
+    hipStream_t st = w3d_s(stream);
+    if (dtype == W3D_DTYPE_F32) q ? launch_fwd<W3D_DTYPE_F32, true>(a, st) : launch_fwd<W3D_DTYPE_F32, false>(a, st);
+    else if (dtype == W3D_DTYPE_BF16) q ? launch_fwd<W3D_DTYPE_BF16, true>(a, st) : launch_fwd<W3D_DTYPE_BF16, false>(a, st);
+    else q ? launch_fwd<W3D_DTYPE_F16, true>(a, st) : launch_fwd<W3D_DTYPE_F16, false>(a, st);
     W3D_CHECK_LAUNCH();
     return W3D_OK;
 }
