@@ -596,6 +596,14 @@ def step_inputs(dt, seed, R=300, K=128, H=352):
             rnd(H, K, seed=seed + 3, dtype=dt, scale=K ** -0.5), (1 + 0.1 * rnd(K, seed=seed + 4)).to(dt), rnd(R, K, seed=seed + 5, dtype=dt)]
 
 
+def test_no_rows_large_weights():
+    """The weight gradient of no rows is zeros, also for more weights than a launch has threads / 16."""
+    N, K = 20001, 16000
+    dw = torch.full((N, K), 7.0, dtype=BF16, device="cuda")
+    ops._launch("w3d_linear_bwd", 0, _lib.lib().w3d_linear_bwd, None, None, None, 0, None, None, 0, K, N, _lib.BF16, 0, None, dw.data_ptr(), None, None, 0)
+    assert not dw.any()
+
+
 def test_the_same_bits_every_time():
     for dt in (BF16, F32):
         a = step_inputs(dt, 100, R=1500)

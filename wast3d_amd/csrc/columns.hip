@@ -9,24 +9,28 @@ template <int DT>
 __global__ __launch_bounds__(1024) void fold_columns_kernel(const float *__restrict__ part, int parts, int64_t ld, int64_t n, void *__restrict__ out) {
     __shared__ float sm[16][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
-    float s[8] = {};
-    if (c < n) {
-        int p = w;
-        for (; p + 112 < parts; p += 128)
+    for (int64_t c0 = (int64_t)blockIdx.x * 64; c0 < n; c0 += (int64_t)gridDim.x * 64) {
+        const int64_t c = c0 + lane;
+        float s[8] = {};
+        if (c < n) {
+            int p = w;
+            for (; p + 112 < parts; p += 128)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] += part[(int64_t)(p + 16 * i) * ld + c];
+                for (int i = 0; i < 8; ++i) s[i] += part[(int64_t)(p + 16 * i) * ld + c];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (p + 16 * i < parts) s[i] += part[(int64_t)(p + 16 * i) * ld + c];
+            for (int i = 0; i < 8; ++i)
+                if (p + 16 * i < parts) s[i] += part[(int64_t)(p + 16 * i) * ld + c];
+        }
+        sm[w][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+        __syncthreads();
+        if (w == 0 && c < n) {
+            float t = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) t += sm[i][lane];
+            store1<DT>((char *)out + c * Elem<DT>::B, t);
+        }
+        __syncthreads();                                     // (the next columns' sums)
     }
-    sm[w][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
-    __syncthreads();
-    if (w != 0 || c >= n) return;
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) t += sm[i][lane];
-    store1<DT>((char *)out + c * Elem<DT>::B, t);
 }
 
 // part[strip][c] = sum of x[r][c] over the strip's rows: a lane owns one column, the four waves of a block every fourth row of the strip
@@ -55,7 +59,8 @@ __global__ __launch_bounds__(256) void column_sums_kernel(const char *__restrict
 // fold of `parts` rows of partial sums (0 parts: zeros) into out[n] of the given dtype
 int w3d_fold_columns(const float *part, int parts, int64_t ld, int64_t n, void *out, int out_dtype, hipStream_t st) {
     if (n < 1) return W3D_OK;
-    const dim3 grid((unsigned)((n + 63) / 64)), block(1024);
+    const int64_t cols = (n + 63) / 64;
+    const dim3 grid((unsigned)(cols < 65536 ? cols : 65536)), block(1024);      // (a launch has less than 2^32 threads; the weight gradient of no rows can be longer)
     if (out_dtype == W3D_DTYPE_F32) hipLaunchKernelGGL(fold_columns_kernel<W3D_DTYPE_F32>, grid, block, 0, st, part, parts, ld, n, out);
     else if (out_dtype == W3D_DTYPE_BF16) hipLaunchKernelGGL(fold_columns_kernel<W3D_DTYPE_BF16>, grid, block, 0, st, part, parts, ld, n, out);
     else hipLaunchKernelGGL(fold_columns_kernel<W3D_DTYPE_F16>, grid, block, 0, st, part, parts, ld, n, out);
