@@ -7,11 +7,11 @@
 //
 // Bound by HBM: every element is read once and written once.  A row stays in registers between its sum and its output, in f32.  Sums are f32 for 16-bit rows.
 // For 8-bit rows the forward pass is 64-bit between the loads and one rounding to f32: what 32 bits lose (2^-23 or so) moves values over e4m3's borders by whole steps: 100 - 127 of 256 million at
-// 1 000 000 x 256, none this way (360 us; 327 in 32 bits).  f32 rows are formed alike, so that quantising them afterwards gives the same bytes.
+// 1 000 000 x 256, none this way (at the same speed).  f32 rows are formed alike, so that quantising them afterwards gives the same bytes.
 // G lanes share a row (a wave holds 64 / G rows), 8 elements per lane and vector, NV vectors per lane: G x NV is the smallest that covers the row, wide
 // rows take the whole block of 256 lanes.  Rows beyond 8 192 elements are read again instead of kept (second and third reading come from L2).
 //
-// Measured, bf16: 1 000 000 x 256 with a residual into 8 bits 360 us (5.0 TB/s); 65 536 x 256 with a residual 22.8 us, backward 27.2 + 4.4 us (fold of dw); kept rows 4.7 - 6.4 TB/s forward,
+// Measured, bf16: 1 000 000 x 256 with a residual into 8 bits 326 us (5.5 TB/s); 65 536 x 256 with a residual 22.8 us, backward 27.2 + 4.4 us (fold of dw); kept rows 4.7 - 6.4 TB/s forward,
 // 3.4 - 5.4 backward (131 072 x 256 .. 16 384 x 8 192), rows read again 3.4 - 3.7 and 2.4 (16 384 wide).
 #include <type_traits>
 #include "rows16.h"
@@ -348,7 +348,11 @@ static int launch_fwd(const NormArgs &a, hipStream_t st) {
         hipLaunchKernelGGL((rms_norm_wide_kernel<DT, Q>), dim3((unsigned)(a.R < 4096 ? a.R : 4096)), dim3(NORM_BLOCK), 0, st, a);
         return W3D_OK;
     }
-    const dim3 grid(w3d_grid(a.R, NORM_BLOCK / sh.g, 8192)), block(NORM_BLOCK);
+    // Two turns a block, or 8 192 blocks if that is more turns for rows that take a whole block (which load the weight for one row at a time).  Blocks at 1 000 000 x 256 with a residual, into
+    // 8 bits | bf16: 4 096 370 us | 375, 8 192 364 | 377, 65 536 (two turns) 326 | 344, 125 000 346 | 329; at 131 072 x 256 8 192 (two turns) 23.5, 16 384 24.8; at 130 055 x 1 032 8 192 129,
+    // 65 536 149; at 16 384 x 8 192 8 192 113, 16 384 128.
+    const int64_t turns = (a.R + NORM_BLOCK / sh.g - 1) / (NORM_BLOCK / sh.g), two = (turns + 1) / 2, most = 1 << 22;
+    const dim3 grid((unsigned)(turns < 8192 ? turns : sh.g == 256 || two < 8192 ? 8192 : two < most ? two : most)), block(NORM_BLOCK);
 #define W3D_NORM(G, NV) hipLaunchKernelGGL((rms_norm_kernel<DT, G, NV, Q>), grid, block, 0, st, a)
     if (sh.g == 8) W3D_NORM(8, 1);
     else if (sh.g == 16) W3D_NORM(16, 1);
