@@ -644,8 +644,8 @@ int w3d_rms_norm_bwd(const void *x, const void *residual, const void *weight, in
  * Gated linear layer: y = act(x Wg^T + bg) * (x Wu^T + bu), one launch for both products.
  * act: W3D_ACT_*; gelu is z * Phi(z).  Rows of x, w and y shorter than 8 MB (W3D_ERR_UNSUPPORTED otherwise).
  * The _fp8 forms take e4m3 rows with one E8M0 exponent (1..254) each for x AND the weights, and write bf16 or f16 (residual and biases of out_dtype, biases also f32).
- * W3D_DTYPE_F32 forward calls can keep the values before the activation: z, f32 [R][w3d_linear_z_stride(N, gated)], 16-byte aligned, or NULL (always, for 16-bit rows).
- * The _bwd forms need the forward's inputs and dy [R,N]; 16-bit ones form z again (z NULL), f32 ones take the z that was kept (unless act is W3D_ACT_NONE in a linear layer): dx [R,K], dw [N,K], dbias [N] (of bias_dtype), each optional; the residual's gradient is dy itself.
+ * Forward calls can keep the values before the activation: z, f32 [R][w3d_linear_z_stride(N, gated)], 16-byte aligned, or NULL.
+ * The _bwd forms need the forward's inputs and dy [R,N]; they take the z that was kept, 16-bit ones form it again without (z NULL; a linear layer with W3D_ACT_NONE needs none): dx [R,K], dw [N,K], dbias [N] (of bias_dtype), each optional; the residual's gradient is dy itself.
  * workspace: w3d_linear_workspace_bytes (dtype W3D_DTYPE_FP8_E4M3 for the _fp8 forms) / w3d_linear_bwd_workspace_bytes (kept: 1 if z is passed); views: 1 if x, a weight matrix or dy may start at an address that
  * is no multiple of 16 (room for aligned copies; widths that are no multiple of 16 bytes get theirs without it). */
 #define W3D_ACT_NONE 0

@@ -59,7 +59,7 @@ def test_linear_arguments(L):
     assert L.w3d_linear_workspace_bytes(300, 64, 64, 1, 0, 1) >= 300 * 128 + 64 * 128 and L.w3d_linear_workspace_bytes(300, 63, 64, 1, 0, 0) >= 300 * 128 + 64 * 128      # aligned copies
     assert f(P, P, None, 0, None, 300, 63, 64, 1, 0, P, None, 0, None) == WS
     assert L.w3d_gated_linear_fwd(P, P, None, None, None, 0, 4, 8, 6, 0, 3, P, None, None, 0, None) == ARG
-    assert L.w3d_linear_fwd(P, P, None, 0, None, 4, 8, 6, 1, 2, P, P, None, 0, None) == ARG             # z is kept by f32 calls only
+    assert L.w3d_linear_fwd(P, P, None, 0, None, 4, 8, 6, 1, 2, P, P.value + 4, None, 0, None) == ARG   # z off its 16 bytes
     assert L.w3d_linear_z_stride(515, 0) == 528 and L.w3d_linear_z_stride(515, 1) == 1056 and L.w3d_linear_z_stride(0, 0) == 0
     e = L.w3d_linear_fp8_fwd
     assert e(P, P, P, P, None, 0, None, 4, 8, 6, 0, 0, P, None, 0, None) == ARG                 # f32 output
@@ -72,7 +72,7 @@ def test_linear_arguments(L):
     assert b(P, P, None, 0, None, 4, 8, 6, 0, 0, P, P, None, P, 4096, None) == ARG
     assert b(P, P, None, 0, P, 400, 8, 6, 1, 2, P, P, None, P, 16, None) == WS
     assert b(P, P, None, 0, P, 400, 8, 6, 0, 2, P, P, None, P, 1 << 20, None) == ARG             # f32: z is needed
-    assert L.w3d_linear_bwd(P, P, None, 0, P, P, 400, 8, 6, 1, 2, P, P, None, P, 1 << 20, None) == ARG
+    assert L.w3d_linear_bwd(P, P, None, 0, P, P.value + 4, 400, 8, 6, 1, 2, P, P, None, P, 1 << 20, None) == ARG
     assert L.w3d_linear_bwd_workspace_bytes(0, 8, 6, 0, 0, 0, 0, 0) == 0
     assert L.w3d_gated_linear_bwd(P, P, None, None, None, 0, P, None, 4, 8, 6, 0, 3, P, P, P, None, None, P, 4096, None) == ARG
 

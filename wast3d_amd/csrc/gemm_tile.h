@@ -40,7 +40,7 @@ struct GemmArgs {
     int64_t colsum_ld;
     float *part;                        // slices > 1: [slice][M][part_ld] f32
     int64_t part_ld;
-    float *z;                           // forward, f32: where the values before the activation go, [M][part_ld] (gated: the second half part_ld / 2 further), or NULL
+    float *z;                           // forward: where the values before the activation go, [M][part_ld] (gated: the second half part_ld / 2 further), or NULL
     int64_t strip;                      // rows of one partial column sum of the joining launch
     int bias_f32, act, slices, tiles_m, tiles_n, out_dt;
 };
@@ -374,7 +374,7 @@ struct Out {
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) { v[e] += b0[e]; if (GATED) u[e] += b1[e]; }
-            if (DT == W3D_DTYPE_F32 && !BWD && a.z && live && n < a.N) {
+            if (DT != W3D_DTYPE_FP8_E4M3 && !BWD && a.z && live && n < a.N) {
                 float *z = a.z + (mw + lane / LPR + r) * a.part_ld + n;
                 store_run<W3D_DTYPE_F32, 8>((uint8_t *)z, a.N - n, v);
                 if (GATED) store_run<W3D_DTYPE_F32, 8>((uint8_t *)(z + a.part_ld / 2), a.N - n, u);

@@ -5,10 +5,10 @@
 //   * tiles of 256 x 256 (gemm_pipe.h), 128 x 128 or 64 x 64 (gemm_tile.h) through LDS
 //   * when the tiles are few for 256 CUs the contraction is cut into slices; partial tiles are added in slice order, and the epilogue applied, by a second launch
 //
-// Backward keeps nothing of a 16-bit forward pass but its inputs: z is formed again and turned into dz in the epilogue, where the column sums for the bias
-// gradient are taken too — storing z in 16 bits would put its rounding into every gradient, storing it in 32 costs more traffic than forming it again
-// (R x N x 12 bytes written and read, against 2 R N K operations).  An f32 forward pass keeps z (at a tenth of the 16-bit rate forming it again is the dearer way).  dz is rounded once to the
-// operands' type (it is an operand of two products); sums are f32.
+// Backward from nothing but the inputs (16-bit rows, z not given): z is formed again and turned into dz in the epilogue, where the column sums for the bias
+// gradient are taken too.  Backward from the z that the forward pass kept (always for f32, at a tenth of the 16-bit rate): one pass over z and dy (dz_kernel).  z is kept in 32 bits (16 would put
+// their rounding into every gradient): 8 bytes an output written and read against 2 K operations, even at K of 900 or so.  dz is rounded once to the operands' type (it is an operand of two
+// products); sums are f32.
 //
 // One translation unit per operand type (W3D_LIN_DT: the tiles), one for the entry points.
 #include "gemm_pipe.h"
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
                     if (GATED) u[e] = __builtin_ldexpf(u[e], a.xs[m] + a.ws2[c + e] - 254);
                 }
                 const float z = v[e] + bias_at<OT>(a.bias, a.bias_f32, c + e, a.N), z2 = GATED ? u[e] + bias_at<OT>(a.bias2, a.bias_f32, c + e, a.N) : 0.f;
-                if (DT == W3D_DTYPE_F32 && a.z) { a.z[m * a.part_ld + c + e] = z; if (GATED) a.z[m * a.part_ld + a.part_ld / 2 + c + e] = z2; }
+                if (DT != W3D_DTYPE_FP8_E4M3 && a.z) { a.z[m * a.part_ld + c + e] = z; if (GATED) a.z[m * a.part_ld + a.part_ld / 2 + c + e] = z2; }
                 float y = act_fwd<ACT>(z);
                 if (GATED) y *= z2;
                 else if (a.res) y += load1<OT>(a.res + (m * a.N + c + e) * OB);
@@ -220,7 +220,7 @@ int W3D_LIN_NAME(w3d_lin_skinny)(const GemmArgs &a, int prod, hipStream_t st) {
 
 namespace {
 
-// Partial sums of a sliced product: part[slice][m][ld] -> the epilogue of the product (one slice: the values before the activation that an f32 forward pass kept, for the gradient's).  A block
+// Partial sums of a sliced product: part[slice][m][ld] -> the epilogue of the product.  A block
 // takes 64 columns of a strip of rows (a multiple of JOIN_ROWS), JOIN_ROWS at a time (a quarter per wave), so that the column sums of dz are complete per strip; up to 8
 // slices of every row are loaded before the first sum (one after another, 16 slices of 16 rows waited 12 us).  Measured: 4 slices of 1024 x 4096 in f32, 75 MB, 18 us.
 constexpr int JOIN_ROWS = 16;
@@ -276,7 +276,7 @@ __global__ __launch_bounds__(256) void join_slices_kernel(GemmArgs a) {
             float x = v[i], y = u[i];
             if (a.xs) { x = __builtin_ldexpf(x, a.xs[m] + s0); if (GATED) y = __builtin_ldexpf(y, a.xs[m] + s1); }
             x += b0; y += b1;
-            if (OT == W3D_DTYPE_F32 && (EPI == EPI_LINEAR || EPI == EPI_GATED) && a.z && in) { a.z[m * a.part_ld + n] = x; if (GATED) a.z[m * a.part_ld + a.part_ld / 2 + n] = y; }
+            if ((EPI == EPI_LINEAR || EPI == EPI_GATED) && a.z && in) { a.z[m * a.part_ld + n] = x; if (GATED) a.z[m * a.part_ld + a.part_ld / 2 + n] = y; }
             uint8_t *o = (EPI == EPI_STORE && z ? a.out2 : a.out) + m * a.ld_out + n * OB;
             if (EPI == EPI_STORE) store1<OT>(o, x);
             else if (EPI == EPI_LINEAR) {
@@ -315,10 +315,68 @@ int join_as(GemmArgs a, int prod, int z, hipStream_t st) {
     switch (prod) {
         case PROD_LINEAR: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_LINEAR>), grid, block, 0, st, a); break;
         case PROD_GATED: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_GATED>), grid, block, 0, st, a); break;
-        case PROD_LINEAR_BWD: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_LINEAR_BWD>), grid, block, 0, st, a); break;
-        case PROD_GATED_BWD: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_GATED_BWD>), grid, block, 0, st, a); break;
+        case PROD_LINEAR_BWD: if constexpr (OT != W3D_DTYPE_F32) hipLaunchKernelGGL((join_slices_kernel<OT, EPI_LINEAR_BWD>), grid, block, 0, st, a); break;      // (f32 calls keep z)
+        case PROD_GATED_BWD: if constexpr (OT != W3D_DTYPE_F32) hipLaunchKernelGGL((join_slices_kernel<OT, EPI_GATED_BWD>), grid, block, 0, st, a); break;
         default: hipLaunchKernelGGL((join_slices_kernel<OT, EPI_STORE>), grid, block, 0, st, a); break;
     }
+    W3D_CHECK_LAUNCH();
+    return W3D_OK;
+}
+
+// dz (both halves of it), and its column sums per strip of rows, from the z that the forward pass kept: a.part = z.  Bound by HBM: a lane takes 8 columns, the four waves of a block every fourth
+// row of the strip.  Padding columns become zeros (z and dy are read as zeros there).  A step of 16 384 rows 1024 -> 4096 590 us with it, 613 with the product once more.
+template <int OT, bool GATED>
+__global__ __launch_bounds__(256) void dz_kernel(GemmArgs a) {
+    constexpr int OB = Elem<OT>::B;
+    __shared__ float sums[4][64 * 8];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t n = ((int64_t)blockIdx.x * 64 + lane) * 8, pad = (GATED ? a.half_out : a.ld_out) / OB;
+    const int64_t r_begin = (int64_t)blockIdx.y * a.strip, r_end = min(a.M, r_begin + a.strip);
+    const int in = (int)max(a.N - n, (int64_t)0), room = (int)(pad - n);
+    float c0[8] = {}, c1[8] = {};
+    if (room > 0)
+        with_act(a.act, [&](auto act_c) {
+            constexpr int ACT = decltype(act_c)::value;
+#pragma unroll 2
+            for (int64_t r = r_begin + wave; r < r_end; r += 4) {
+                float v[8], u[8], t[8];
+                load8<W3D_DTYPE_F32>(a.part + r * a.part_ld + n, in, v);
+                if (GATED) load8<W3D_DTYPE_F32>(a.part + r * a.part_ld + a.part_ld / 2 + n, in, u);
+                load8<OT>(a.dy + (r * a.N + n) * OB, in, t);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float f, d;
+                    act_both<ACT>(v[e], f, d);
+                    if (GATED) { v[e] = t[e] * (u[e] * d); u[e] = t[e] * f; c1[e] += u[e]; }
+                    else v[e] = t[e] * d;
+                    c0[e] += v[e];
+                }
+                uint8_t *o = a.out + r * a.ld_out + n * OB;
+                store8<OT>(o, room, v);
+                if (GATED) store8<OT>(o + a.half_out, room, u);
+            }
+        });
+    if (!a.colsum) return;
+#pragma unroll
+    for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sums[wave][e * 64 + lane] = h ? c1[e] : c0[e];
+        __syncthreads();
+#pragma unroll
+        for (int e = 2 * wave; e < 2 * wave + 2; ++e)
+            if (n + e < a.N)
+                a.colsum[(int64_t)blockIdx.y * a.colsum_ld + h * (a.colsum_ld / 2) + n + e] =
+                    (sums[0][e * 64 + lane] + sums[1][e * 64 + lane]) + (sums[2][e * 64 + lane] + sums[3][e * 64 + lane]);
+    }
+}
+template <int OT>
+int dz_as(GemmArgs a, bool gated, hipStream_t st) {
+    const int64_t pad = (gated ? a.half_out : a.ld_out) / Elem<OT>::B;
+    a.strip = strip_rows(a.M);
+    const dim3 grid((unsigned)((pad + 511) / 512), (unsigned)((a.M + a.strip - 1) / a.strip)), block(256);
+    if (gated) hipLaunchKernelGGL((dz_kernel<OT, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((dz_kernel<OT, false>), grid, block, 0, st, a);
     W3D_CHECK_LAUNCH();
     return W3D_OK;
 }
@@ -375,7 +433,7 @@ size_t part_bytes(const Cut &c, int64_t M, int64_t N, bool gated, int batch) {
 
 // floats of a row of partial sums, or of kept values before the activation
 int64_t z_stride(int64_t N, bool gated) { return ceil_to(N, 16) * (gated ? 2 : 1); }
-// the second launch of a sliced product, or of a gradient whose z was kept
+// the second launch of a sliced product
 int join(const GemmArgs &a, int prod, int z, hipStream_t st) {
     switch (a.out_dt) {
         case W3D_DTYPE_F32: return join_as<W3D_DTYPE_F32>(a, prod, z, st);
@@ -465,7 +523,7 @@ int forward(const void *x, const int32_t *xs, const void *w, const int32_t *ws, 
     if (R < 0 || K < 1 || N < 1 || act < 0 || act > ACT_SIGMOID || !float_dtype(out_dtype)) return W3D_ERR_ARG;
     if ((bias || bias2) && bias_dtype != out_dtype && bias_dtype != W3D_DTYPE_F32) return W3D_ERR_ARG;
     if (R == 0) return W3D_OK;
-    if (!x || !w || !y || (gated && !w2) || (z && (dtype != W3D_DTYPE_F32 || ((uintptr_t)z & 15)))) return W3D_ERR_ARG;
+    if (!x || !w || !y || (gated && !w2) || ((uintptr_t)z & 15)) return W3D_ERR_ARG;
     const int eb = eb_of(dtype);
     if (!row_ok(K * eb) || !row_ok(N * eb_of(out_dtype))) return W3D_ERR_UNSUPPORTED;
     GemmArgs a = {};
@@ -557,7 +615,7 @@ int backward(const void *x, const void *w, const void *w2, const void *bias, con
     if (!row_ok(K * eb) || !row_ok((N + 64) * eb * parts)) return W3D_ERR_UNSUPPORTED;
     if (R > 0 && (!x || !w || !dy || (gated && !w2) || ((uintptr_t)z & 15))) return W3D_ERR_ARG;
     const bool no_act = !gated && act == ACT_NONE;
-    if (R > 0 && (dtype == W3D_DTYPE_F32 ? !no_act && !z : z != nullptr)) return W3D_ERR_ARG;
+    if (R > 0 && dtype == W3D_DTYPE_F32 && !no_act && !z) return W3D_ERR_ARG;
     const bool again = !no_act && !z;                                                         // z is formed again
     const bool cx = R > 0 && (again || dw || dw2) && unaligned(x, K * eb), cw = R > 0 && (again || dx) && (unaligned(w, K * eb) || unaligned(w2, K * eb)),
                cdy = R > 0 && no_act && (dx || dw) && unaligned(dy, N * eb);
@@ -585,9 +643,8 @@ int backward(const void *x, const void *w, const void *w2, const void *bias, con
         a.colsum = db || db2 ? colsum : nullptr; a.colsum_ld = b.colsum_ld; a.part = part;
         const int prod = gated ? PROD_GATED_BWD : PROD_LINEAR_BWD;
         if (z) {
-            a.part = const_cast<float *>(z); a.part_ld = z_stride(N, gated); a.slices = 1;
-            a.bias = a.bias2 = nullptr;
-            rc = join(a, prod, 1, st);
+            a.part = const_cast<float *>(z); a.part_ld = z_stride(N, gated);
+            rc = dtype == W3D_DTYPE_F32 ? dz_as<W3D_DTYPE_F32>(a, gated, st) : dtype == W3D_DTYPE_BF16 ? dz_as<W3D_DTYPE_BF16>(a, gated, st) : dz_as<W3D_DTYPE_F16>(a, gated, st);
             strips = join_strips(R);
         } else {
             const Cut c = cut_of(R, gated ? b.pad : N, K, dtype, gated, aligned16(dy, N * eb), 1);          // (the tiles write the padding columns too)

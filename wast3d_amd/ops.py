@@ -1621,9 +1621,15 @@ def raw_gated_linear(x, wg, wu, bg, bu, act: int, y, z=None):
             dt, act, y.data_ptr(), _at(z), _at(ws), nbytes)
 
 
+# 16-bit layers of at least this many inputs keep z for their gradient (4 bytes an output), others form it again.  us of a training step, again | kept, bf16, 16 384 rows onto 4 096:
+# 512 inputs 410 | 466, 1 024 613 | 590, 2 048 1 035 | 924, 4 096 1 802 | 1 493; gated 512 729 | 803, 1 024 1 071 | 1 055, 4 096 3 533 | 2 979; 4 999 rows onto 515: 256 50.6 | 51.9, 1 024 80.7 | 74.2.
+_KEEP_FROM = 896
+
+
 def _kept(x, N: int, gated: int):
-    """Room for the values before the activation: kept for the gradient by 32-bit calls (16-bit ones form them again)."""
-    return x.new_empty(x.numel() // x.shape[-1], lib().w3d_linear_z_stride(N, gated)) if x.dtype == torch.float32 else None
+    """Room for the values before the activation, in f32, where they are kept for the gradient."""
+    K = x.shape[-1]
+    return x.new_empty((x.numel() // K, lib().w3d_linear_z_stride(N, gated)), dtype=torch.float32) if x.dtype == torch.float32 or K >= _KEEP_FROM else None
 
 
 class _Linear(torch.autograd.Function):
@@ -1665,7 +1671,7 @@ def _head_weight(what: str, name: str, w):
 
 def linear(x, weight, bias=None, activation=None, residual=None):
     """y = act(x weight^T + bias) + residual in one launch.  x [..., K] f32 / bf16 / f16, weight [N,K] and residual [..., N] of x's type, bias [N] of x's type or f32;
-    activation None, 'relu', 'gelu' (z Phi(z)), 'silu' or 'sigmoid'.  Sums in f32, one rounding at the end.  Differentiable in everything; for it 16-bit calls keep nothing but the inputs, f32 calls the values before the activation."""
+    activation None, 'relu', 'gelu' (z Phi(z)), 'silu' or 'sigmoid'.  Sums in f32, one rounding at the end.  Differentiable in everything; for it f32 calls, and 16-bit ones with K >= 896, keep the values before the activation in f32; other calls keep nothing but the inputs."""
     _head_rows("linear", x)
     act = _head_act(activation)
     N, _ = _head_weight("linear", "weight", weight)
@@ -1721,7 +1727,7 @@ def _gated_args(what, x, wg, wu, bg, bu, dtype, bias_dtype):
 
 def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     """y = act(x w_gate^T + b_gate) * (x w_up^T + b_up): both products, the activation and the product in one launch.  x [..., K] f32 / bf16 / f16, weights [N,K] of x's type, biases
-    [N] of x's type or f32 (both alike); activation as in linear.  Sums in f32, one rounding at the end.  Differentiable in everything; for it 16-bit calls keep nothing but the inputs, f32 calls the values before the activation."""
+    [N] of x's type or f32 (both alike); activation as in linear.  Sums in f32, one rounding at the end.  Differentiable in everything; for it f32 calls, and 16-bit ones with K >= 896, keep the values before the activation in f32; other calls keep nothing but the inputs."""
     _head_rows("gated_linear", x)
     act = _head_act(activation)
     N, w_gate, w_up, b_gate, b_up = _gated_args("gated_linear", x, w_gate, w_up, b_gate, b_up, x.dtype, x.dtype)
