@@ -15,6 +15,7 @@ import ctypes as C
 import functools
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 from ._lib import BF16, F16, F32, FP8, W3dError, check, clear_stale_hip_error, lib, ptr, require_cuda, stream_ptr
@@ -1444,10 +1445,14 @@ def _head_eps(eps) -> float:
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_dispatch_mode, _PROXY = torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY
+_tracing = torch._C._get_tracing_state
 
 
 def _launch(what: str, index: int, fn, *args):
     """One call of the library on the current stream of the tensors' own device (the stream is the last argument; tensors travel as addresses, None as NULL)."""
+    if _dispatch_mode(_PROXY) is not None:
+        raise W3dError(f"{what}: a symbolic trace (make_fx) cannot record the call, only the allocation of its output")
     if index == torch.cuda.current_device():
         clear_stale_hip_error()
         code = fn(*args, _raw_stream(index))
@@ -1486,12 +1491,27 @@ def _views(*tensors) -> int:
     return 0
 
 
-def _wants_grad(*tensors) -> bool:
+def _through_autograd(*tensors) -> bool:
+    """Does a call go through its autograd function?  Where something asks for a gradient, where an open forward-mode level may carry tangents (the function refuses them), and under
+    torch.jit.trace (which records the function; of a direct call it would see the allocation of the output alone)."""
+    if _tracing() is not None or _forward_ad._current_level >= 0:
+        return True
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
     return False
+
+
+def _no_gradient(what: str, *tensors):
+    """The 8-bit forms have no derivative of any kind and no function that a trace could record."""
+    if not _through_autograd(*tensors):
+        return
+    if _tracing() is not None:
+        raise W3dError(f"{what} cannot be traced")
+    given = [t for t in tensors if t is not None]
+    if (torch.is_grad_enabled() and any(t.requires_grad for t in given)) or any(_forward_ad.unpack_dual(t).tangent is not None for t in given if t.is_floating_point()):
+        raise W3dError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
 def _code(t) -> int:
@@ -1571,7 +1591,7 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-6):
         weight = _head_arg("rms_norm", "weight", weight, x.shape[-1:], x.dtype, x.device, True)
     if residual is not None:
         residual = _head_arg("rms_norm", "residual", residual, x.shape, x.dtype, x.device)
-    if _wants_grad(x, weight, residual):
+    if _through_autograd(x, weight, residual):
         return _RmsNorm.apply(xc, weight, residual, eps)
     y = torch.empty_like(xc)
     s = torch.empty_like(xc) if residual is not None else None
@@ -1587,8 +1607,7 @@ def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-6):
     if x.dim() != 2:
         raise W3dError(f"rms_norm_fp8: rows [R,d] expected, got a tensor of shape {tuple(x.shape)}")
     eps = _head_eps(eps)
-    if _wants_grad(x, weight, residual):
-        raise W3dError("rms_norm_fp8 has no gradient: call it under torch.no_grad() or on detached tensors")
+    _no_gradient("rms_norm_fp8", x, weight, residual)
     R, d = x.shape
     xc = x.contiguous()
     if weight is not None:
@@ -1681,7 +1700,7 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     if residual is not None:
         residual = _head_arg("linear", "residual", residual, (*x.shape[:-1], N), x.dtype, x.device)
     xc = x.contiguous()
-    if _wants_grad(x, weight, bias, residual):
+    if _through_autograd(x, weight, bias, residual):
         return _Linear.apply(xc, weight, bias, residual, act)
     y = xc.new_empty((*x.shape[:-1], N))
     raw_linear(xc, weight, bias, residual, act, y)
@@ -1732,7 +1751,7 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     act = _head_act(activation)
     N, w_gate, w_up, b_gate, b_up = _gated_args("gated_linear", x, w_gate, w_up, b_gate, b_up, x.dtype, x.dtype)
     xc = x.contiguous()
-    if _wants_grad(x, w_gate, w_up, b_gate, b_up):
+    if _through_autograd(x, w_gate, w_up, b_gate, b_up):
         return _GatedLinear.apply(xc, w_gate, w_up, b_gate, b_up, act)
     y = xc.new_empty((*x.shape[:-1], N))
     raw_gated_linear(xc, w_gate, w_up, b_gate, b_up, act, y)
@@ -1751,8 +1770,7 @@ def _fp8_rows(what, name, q, scale, device):
 def _fp8_out(what, out_dtype, *tensors):
     if out_dtype not in (torch.bfloat16, torch.float16):
         raise W3dError(f"{what}: out_dtype {out_dtype} (torch.bfloat16 or torch.float16)")
-    if _wants_grad(*tensors):
-        raise W3dError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+    _no_gradient(what, *tensors)
     return _DTYPE_CODES[out_dtype]
 
 
