@@ -626,11 +626,12 @@ int w3d_raster_preprocess_backward(const W3dRasterIn *in, const int32_t *radii, 
 /* ---- layers of a feature head (no counterpart in the reference): rows of any width -> the rows the match takes.
  * Row-major, contiguous; any row count (0 is a no-op), any width, any element alignment of the pointers; aligned tensors (16 B, widths that are multiples of 16 B) run fastest.
  * dtype: W3D_DTYPE_F32 / BF16 / F16 for rows, weights, residual and outputs alike; weight_dtype / bias_dtype (norm weight, biases): dtype or W3D_DTYPE_F32.
- * All sums are f32, outputs are rounded once.  Results do not depend on the launch (no atomics).  Workspaces: 16-byte aligned, contents irrelevant before and after, one per call in flight.
+ * All sums are f32 or wider, outputs are rounded once.  Results do not depend on the launch (no atomics).  Workspaces: 16-byte aligned, contents irrelevant before and after, one per call in flight.
  *
  * Root-mean-square norm: s = x + residual (residual NULL: s = x); rstd = 1 / sqrt(mean(s^2) + eps); y = s * rstd * weight (weight NULL: 1).
  *   w3d_rms_norm_fwd: y [R,d]; s [R,d] (optional, only with a residual; the sum, rounded); rstd f32 [R] (optional, for the backward pass).
  *   w3d_rms_norm_fp8: the same y as e4m3 bytes q [R,d] + E8M0 exponents [R] (the format and the scale rule of w3d_quantize_rows_fp8), s optional as above.
+ *     Rows of any finite size: the sum of squares is 64-bit where 32 bits do not hold it (rstd and the gradients are f32: not finite for rows whose mean root is below 2.9e-39 and eps 0).
  *   w3d_rms_norm_bwd: from the forward's inputs, rstd, dy and ds (gradient that reaches s itself, optional): dx [R,d] (also the residual's gradient) and / or dweight [d]
  *     (of weight_dtype; needs the workspace). */
 int w3d_rms_norm_fwd(const void *x, const void *residual, const void *weight, int weight_dtype, int64_t R, int d, int dtype, float eps, void *y, void *s, float *rstd,

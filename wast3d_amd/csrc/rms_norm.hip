@@ -5,7 +5,8 @@
 //   given dy (and ds, what reaches s from elsewhere):  g = dy w;  x^ = s r;  dx = r (g - x^ mean(g x^)) + ds;  dw = sum over rows of dy x^
 // The backward pass forms s again from x and the residual, unrounded: from the rounded s its error would show in dw (1.5 x the error of one rounding).
 //
-// Bound by HBM: every element is read once and written once.  A row stays in registers between its sum and its output, in f32.  Sums are f32 for 16-bit rows.
+// Bound by HBM: every element is read once and written once.  A row stays in registers between its sum and its output, in f32.  Sums are f32 for 16-bit rows, 64-bit where a bf16 row's
+// squares leave f32's range.
 // For 8-bit rows the forward pass is 64-bit between the loads and one rounding to f32: what 32 bits lose (2^-23 or so) moves values over e4m3's borders by whole steps: 100 - 127 of 256 million at
 // 1 000 000 x 256, none this way (at the same speed).  f32 rows are formed alike, so that quantising them afterwards gives the same bytes.
 // G lanes share a row (a wave holds 64 / G rows), 8 elements per lane and vector, NV vectors per lane: G x NV is the smallest that covers the row, wide
@@ -70,12 +71,18 @@ __device__ __forceinline__ T group_reduce(T v, T *red) {
 
 // The forward pass's type: 64 bits for 8-bit rows, and for f32 ones (the same rows, quantised afterwards, are the same bytes)
 template <int DT, bool Q> struct Wide { typedef typename std::conditional<Q || DT == W3D_DTYPE_F32, double, float>::type T; };
+// Has a 32-bit sum of squares left f32's range, or come near its end?  (bf16 rows past 1.8e19 or below 1e-15 or so, rows of zeros: they are summed again in 64 bits.  In 64 bits throughout, 65 536 x 256 from the
+// caches take 14.8 us instead of 13.8.)
+template <int DT> __device__ __forceinline__ bool out_of_range(float sum) { return DT == W3D_DTYPE_BF16 && !(sum >= 0x1p-100f && sum <= 0x1.fffffep127f); }
+template <int DT> __device__ __forceinline__ bool out_of_range(double) { return false; }
 __device__ __forceinline__ float inverse_rms(float sum, const NormArgs &a) { return 1.0f / sqrtf(sum * (float)a.inv_d + a.eps); }
-// 1 / sqrt(mean + eps) of a row's 64-bit sum of squares: the 32-bit value and one Newton step in 64 bits.  Where that step is not a number (a mean of 0, infinity, NaN or past 32 bits) the first
-// value stands.
+// 1 / sqrt(mean + eps) of a row's 64-bit sum of squares: the instruction's estimate and two Newton steps.  Where they give no number (a mean of 0, infinity, NaN) the estimate stands: infinity, 0, NaN.
 __device__ __forceinline__ double inverse_rms(double sum, const NormArgs &a) {
-    const double v = sum * a.inv_d + (double)a.eps, r0 = (double)(1.0f / sqrtf((float)v)), r = r0 * fma(-0.5 * v * r0, r0, 1.5);
-    return r > 0.0 && r < 1e300 ? r : r0;
+    const double v = sum * a.inv_d + (double)a.eps, r0 = __builtin_amdgcn_rsq(v);
+    double r = r0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) r = r * fma(-0.5 * v * r, r, 1.5);
+    return r > 0.0 ? r : r0;
 }
 
 // the E8M0 exponent of a row: the smallest power of two that takes amax into e4m3's range (448 = 0.875 2^9), 127 for a row of zeros (or one without a finite maximum below 2^127)
@@ -107,6 +114,7 @@ __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_kernel(NormArgs a) {
     constexpr int EB = Elem<DT>::B, RPB = NORM_BLOCK / G;
     __shared__ float red[4];
     __shared__ T red_sum[4];
+    __shared__ double red_again[4];
     const int gl = threadIdx.x & (G - 1), c0 = gl * 8;
     float w[NV][8];
 #pragma unroll
@@ -126,7 +134,16 @@ __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_kernel(NormArgs a) {
         for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum = fma((T)s[v][i], (T)s[v][i], sum);
-        const T rs = inverse_rms(group_reduce<G, false>(sum, red_sum), a);
+        sum = group_reduce<G, false>(sum, red_sum);
+        T rs = inverse_rms(sum, a);
+        if (out_of_range<DT>(sum)) {                                        // (alike for all lanes of a row)
+            double again = 0;
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) again = fma((double)s[v][i], (double)s[v][i], again);
+            rs = (T)inverse_rms(group_reduce<G, false>(again, red_again), a);
+        }
         if (a.rstd && live && gl == 0) a.rstd[r] = (float)rs;
         if (a.s && live) {
 #pragma unroll
@@ -160,6 +177,7 @@ __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_wide_kernel(NormArgs a) {
     constexpr int EB = Elem<DT>::B;
     __shared__ float red[4];
     __shared__ T red_sum[4];
+    __shared__ double red_again[4];
     for (int64_t r = blockIdx.x; r < a.R; r += gridDim.x) {
         const int64_t at = r * a.d;
         float s[8], w[8];
@@ -169,7 +187,17 @@ __global__ __launch_bounds__(NORM_BLOCK) void rms_norm_wide_kernel(NormArgs a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum = fma((T)s[i], (T)s[i], sum);
         }
-        const T rs = inverse_rms(group_reduce<256, false>(sum, red_sum), a);
+        sum = group_reduce<256, false>(sum, red_sum);
+        T rs = inverse_rms(sum, a);
+        if (out_of_range<DT>(sum)) {
+            double again = 0;
+            for (int c = threadIdx.x * 8; c < a.d; c += NORM_BLOCK * 8) {
+                sum_row<DT>(a, at, c, s);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) again = fma((double)s[i], (double)s[i], again);
+            }
+            rs = (T)inverse_rms(group_reduce<256, false>(again, red_again), a);
+        }
         if (a.rstd && threadIdx.x == 0) a.rstd[r] = (float)rs;
         float amax = 0.f;
         for (int c = threadIdx.x * 8; c < a.d; c += NORM_BLOCK * 8) {

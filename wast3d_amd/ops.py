@@ -1581,7 +1581,7 @@ class _RmsNorm(torch.autograd.Function):
 
 def rms_norm(x, weight=None, residual=None, eps: float = 1e-6):
     """y = s / sqrt(mean(s^2) + eps) * weight over the last dimension of s = x + residual.  x [..., d] f32 / bf16 / f16, residual like x, weight [d] of x's type or f32.
-    Returns y, or (y, s) with a residual (s rounded to x's type: what the next block adds to).  The norm is taken of the unrounded sum; sums are f32.
+    Returns y, or (y, s) with a residual (s rounded to x's type: what the next block adds to).  The norm is taken of the unrounded sum, the mean of squares in 32 bits or more (rows of any finite size).
     Differentiable in x, weight and residual."""
     _head_rows("rms_norm", x)
     _norm_width("rms_norm", x)
