@@ -98,6 +98,18 @@ __device__ __forceinline__ void act_both(float z, float &a, float &d) {
         else { a = s; d = s * (1.0f - s); }
     }
 }
+// The gradient that passes the activation: dy d, of a gated layer's gate dy (u d).  relu is a choice and no product: where it is off, nothing passes, whatever dy is (infinity, NaN); where z is
+// not a number, dy does (as torch's relu).
+template <int ACT>
+__device__ __forceinline__ float through(float dy, float z, float d) {
+    if (ACT == ACT_RELU) return z <= 0.f ? 0.f : dy;
+    return dy * d;
+}
+template <int ACT>
+__device__ __forceinline__ float through(float dy, float z, float d, float u) {
+    if (ACT == ACT_RELU) return z <= 0.f ? 0.f : dy * u;
+    return dy * (u * d);
+}
 // calls f with the activation as a compile-time value
 template <typename F>
 __device__ __forceinline__ void with_act(int act, F f) {
@@ -390,8 +402,8 @@ struct Out {
                     } else {
                         float f, d;
                         act_both<ACT>(v[e], f, d);
-                        if (EPI == EPI_LINEAR_BWD) v[e] = t[e] * d;
-                        else { v[e] = t[e] * (u[e] * d); u[e] = t[e] * f; }
+                        if (EPI == EPI_LINEAR_BWD) v[e] = through<ACT>(t[e], v[e], d);
+                        else { v[e] = through<ACT>(t[e], v[e], d, u[e]); u[e] = t[e] * f; }
                     }
                 }
             };
