@@ -67,18 +67,36 @@ constexpr int SLAB = 128;                        // bytes of contraction per sla
 constexpr uint32_t OUT_OF_RANGE = 0x80000000u;   // buffer offset past num_records: the load returns zeros
 
 // ---- activations.  a = act(z), d = act'(z).
-// gelu(z) = z Phi(z) = max(z, 0) - h Phi(-h), h = |z|.  log2 Phi(-h) is nearly a parabola: a polynomial of degree 6, fitted on [0, 5.75] to the smallest maximum of h |error of Phi|, and
-// one exponential give gelu to 2.4e-7 and Phi to 8e-7, the tail without cancellation; past 5.75, h Phi(-h) < 3e-8 stays what it is there.
-__device__ __forceinline__ float normal_tail(float h) {                                        // Phi(-h), 0 <= h <= 5.75
-    const float p = fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, 3.2983829e-5f, -7.6224754e-4f), 8.0370521e-3f), -5.3309143e-2f), -4.5887902e-1f), -1.1511532f), -1.0000001f);
+// gelu(z) = z Phi(z) = max(z, 0) - h Phi(-h), h = |z|, with Phi(-h) to a relative bound: a gated layer multiplies the tail by what it likes.  Two forms of it:
+//   Phi(-h) = e t P(t), e = exp(-h^2 / 2), t = 1 / (1 + 0.3 h): P of degree 7, fitted on [0, 14.3] to the smallest maximum of the relative error, 1.4e-7; in f32 2^-21 and the argument's rounding (h^2 2^-24), which
+//     z's own last place costs too.  For f32 layers and for derivatives, which need e themselves.
+//   log2 Phi(-h) by a polynomial, for the outputs of 16-bit layers, where the epilogue is what a short contraction waits for (one polynomial of degree 10 for both: 65 536 x 256 -> 1 024 88 us in bf16 and 90 in f16, these 84 and 78).  bf16: degree 8,
+//     fitted on [0, 13.2] to h |error of Phi| <= 2.5e-7 and 1.2e-3 of Phi (half a step is 3.9e-3); f16: degree 7 on [0, 8], 2.3e-7 and 2.1e-4 (4.9e-4), and h Phi(-h) stays at 5e-15 past 8: less than any f16
+//     number's last place can show of it, times the largest.
+// Past 13.2 (14.4 in the first form) the exponential is below 2^-126 and becomes 0.
+__device__ __forceinline__ float normal_tail(float h, float e) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(h, 0.3f, 1.0f));
+    const float p = fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, 3.5531368e-2f, -1.5657105e-1f), 2.0520240e-1f), -5.2566256e-2f), 1.2794091e-1f), 1.0010950e-1f), 1.2072159e-1f), 1.1963145e-1f);
+    return e * (t * p);
+}
+template <int OT>
+__device__ __forceinline__ float normal_tail_16(float h) {
+    float p;
+    if (OT == W3D_DTYPE_F16)
+        p = fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, -1.4817135e-06f, 5.4606211e-05f), -0.000879072f), 0.0083331997f), -0.05368023f), -0.45865902f), -1.1512053f), -0.99999714f);
+    else
+        p = fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, 4.2807482e-8f, -2.5480883e-6f), 6.4550513e-5f), -9.2313864e-4f), 8.4335105e-3f), -5.3797774e-2f), -4.5859316e-1f), -1.1512195f), -9.9999672e-1f);
     return __builtin_amdgcn_exp2f(p);
 }
-template <int ACT>
+__device__ __forceinline__ float exp_half_square(float h) { return __builtin_amdgcn_exp2f(h * h * -0.72134752f); }
+// OT: the layer's output type
+template <int ACT, int OT>
 __device__ __forceinline__ float act_fwd(float z) {
     if (ACT == ACT_RELU) return z < 0.f ? 0.f : z;                       // (a NaN stays)
     if (ACT == ACT_GELU) {
-        const float h = fminf(fabsf(z), 5.75f);
-        return fmaf(-h, normal_tail(h), z < 0.f ? 0.f : z);
+        const bool wide = OT == W3D_DTYPE_F32;
+        const float h = fminf(fabsf(z), wide ? 16.0f : OT == W3D_DTYPE_F16 ? 8.0f : 13.2f), tail = wide ? normal_tail(h, exp_half_square(h)) : normal_tail_16<OT>(h);
+        return fmaf(-h, tail, __builtin_elementwise_maximum(z, 0.f));    // (a NaN stays)
     }
     if (ACT == ACT_SILU) return z * __builtin_amdgcn_rcpf(1.0f + __expf(-z));
     if (ACT == ACT_SIGMOID) return __builtin_amdgcn_rcpf(1.0f + __expf(-z));
@@ -89,7 +107,7 @@ __device__ __forceinline__ void act_both(float z, float &a, float &d) {
     if (ACT == ACT_NONE) { a = z; d = 1.f; }
     else if (ACT == ACT_RELU) { a = z < 0.f ? 0.f : z; d = z > 0.f ? 1.f : 0.f; }
     else if (ACT == ACT_GELU) {
-        const float h = fminf(fabsf(z), 5.75f), tail = normal_tail(h), e = __builtin_amdgcn_exp2f(z * z * -0.72134752f);      // exp(-z^2 / 2)
+        const float h = fminf(fabsf(z), 16.0f), e = exp_half_square(h), tail = normal_tail(h, e);
         a = fmaf(-h, tail, z < 0.f ? 0.f : z);
         d = fmaf(z * 0.39894228f, e, z < 0.f ? tail : 1.0f - tail);
     } else {
@@ -396,7 +414,7 @@ struct Out {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     if (!BWD) {
-                        v[e] = act_fwd<ACT>(v[e]);
+                        v[e] = act_fwd<ACT, OT>(v[e]);
                         if (EPI == EPI_GATED) v[e] *= u[e];
                         else if (decltype(src_c)::value) v[e] += t[e];
                     } else {

@@ -178,7 +178,7 @@ __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
                 }
                 const float z = v[e] + bias_at<OT>(a.bias, a.bias_f32, c + e, a.N), z2 = GATED ? u[e] + bias_at<OT>(a.bias2, a.bias_f32, c + e, a.N) : 0.f;
                 if (DT != W3D_DTYPE_FP8_E4M3 && a.z) { a.z[m * a.part_ld + c + e] = z; if (GATED) a.z[m * a.part_ld + a.part_ld / 2 + c + e] = z2; }
-                float y = act_fwd<ACT>(z);
+                float y = act_fwd<ACT, OT>(z);
                 if (GATED) y *= z2;
                 else if (a.res) y += load1<OT>(a.res + (m * a.N + c + e) * OB);
                 store1<OT>(a.out + m * a.ld_out + (c + e) * OB, y);
@@ -280,10 +280,10 @@ __global__ __launch_bounds__(256) void join_slices_kernel(GemmArgs a) {
             uint8_t *o = (EPI == EPI_STORE && z ? a.out2 : a.out) + m * a.ld_out + n * OB;
             if (EPI == EPI_STORE) store1<OT>(o, x);
             else if (EPI == EPI_LINEAR) {
-                x = act_fwd<ACT>(x);
+                x = act_fwd<ACT, OT>(x);
                 if (a.res) x += load1<OT>(a.res + (m * a.N + n) * OB);
                 store1<OT>(o, x);
-            } else if (EPI == EPI_GATED) store1<OT>(o, act_fwd<ACT>(x) * y);
+            } else if (EPI == EPI_GATED) store1<OT>(o, act_fwd<ACT, OT>(x) * y);
             else {
                 float act, der;
                 act_both<ACT>(x, act, der);
