@@ -58,7 +58,7 @@ def forward_bound(z, a, act, dt):
 
 
 @pytest.mark.parametrize("dt", [BF16, F16, F32])
-@pytest.mark.parametrize("act", ["relu", "gelu"])
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu", "sigmoid"])
 @pytest.mark.parametrize("R,K,N", SHAPES)
 def test_forward_values(R, K, N, act, dt):
     z, x, w = operands(R, K, N, dt)
@@ -82,7 +82,7 @@ def test_forward_values(R, K, N, act, dt):
 
 @pytest.mark.parametrize("kept", [False, True])
 @pytest.mark.parametrize("dt", [BF16, F16, F32])
-@pytest.mark.parametrize("act", ["relu", "gelu"])
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu", "sigmoid"])
 @pytest.mark.parametrize("R,K,N", SHAPES)
 def test_derivatives(R, K, N, act, dt, kept, monkeypatch):
     """dx of one input column that reaches one output with weight 1, and the bias gradients' terms: the derivative itself."""

@@ -88,6 +88,13 @@ __device__ __forceinline__ float normal_tail_16(float h) {
         p = fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, 4.2807482e-8f, -2.5480883e-6f), 6.4550513e-5f), -9.2313864e-4f), 8.4335105e-3f), -5.3797774e-2f), -4.5859316e-1f), -1.1512195f), -9.9999672e-1f);
     return __builtin_amdgcn_exp2f(p);
 }
+// e = exp(-|z|), s = 1 / (1 + exp(-z)) and q = 1 - s without the cancellation (1 - s is 0 past z = 17, and wrong by 2^-24 before it).  The exponential's argument is rounded in 16-bit layers: |z| 2^-24 of the value.
+template <int OT>
+__device__ __forceinline__ void sigmoid_pair(float z, float &s, float &q) {
+    const float e = OT == W3D_DTYPE_F32 ? expf(-fabsf(z)) : __expf(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + e), er = e * r;
+    s = z < 0.f ? er : r;
+    q = z < 0.f ? r : er;
+}
 __device__ __forceinline__ float exp_half_square(float h) { return __builtin_amdgcn_exp2f(h * h * -0.72134752f); }
 // OT: the layer's output type
 template <int ACT, int OT>
@@ -98,11 +105,16 @@ __device__ __forceinline__ float act_fwd(float z) {
         const float h = fminf(fabsf(z), wide ? 16.0f : OT == W3D_DTYPE_F16 ? 8.0f : 13.2f), tail = wide ? normal_tail(h, exp_half_square(h)) : normal_tail_16<OT>(h);
         return fmaf(-h, tail, __builtin_elementwise_maximum(z, 0.f));    // (a NaN stays)
     }
+    if (OT == W3D_DTYPE_F32 && (ACT == ACT_SILU || ACT == ACT_SIGMOID)) {
+        float s, q;
+        sigmoid_pair<OT>(z, s, q);
+        return ACT == ACT_SILU ? z * s : s;
+    }
     if (ACT == ACT_SILU) return z * __builtin_amdgcn_rcpf(1.0f + __expf(-z));
     if (ACT == ACT_SIGMOID) return __builtin_amdgcn_rcpf(1.0f + __expf(-z));
     return z;
 }
-template <int ACT>
+template <int ACT, int OT>
 __device__ __forceinline__ void act_both(float z, float &a, float &d) {
     if (ACT == ACT_NONE) { a = z; d = 1.f; }
     else if (ACT == ACT_RELU) { a = z < 0.f ? 0.f : z; d = z > 0.f ? 1.f : 0.f; }
@@ -111,9 +123,10 @@ __device__ __forceinline__ void act_both(float z, float &a, float &d) {
         a = fmaf(-h, tail, z < 0.f ? 0.f : z);
         d = fmaf(z * 0.39894228f, e, z < 0.f ? tail : 1.0f - tail);
     } else {
-        const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-z));
-        if (ACT == ACT_SILU) { a = z * s; d = s * fmaf(z, 1.0f - s, 1.0f); }
-        else { a = s; d = s * (1.0f - s); }
+        float s, q;
+        sigmoid_pair<OT>(z, s, q);
+        if (ACT == ACT_SILU) { a = z * s; d = s * fmaf(z, q, 1.0f); }
+        else { a = s; d = s * q; }
     }
 }
 // The gradient that passes the activation: dy d, of a gated layer's gate dy (u d).  relu is a choice and no product: where it is off, nothing passes, whatever dy is (infinity, NaN); where z is
@@ -419,7 +432,7 @@ struct Out {
                         else if (decltype(src_c)::value) v[e] += t[e];
                     } else {
                         float f, d;
-                        act_both<ACT>(v[e], f, d);
+                        act_both<ACT, OT>(v[e], f, d);
                         if (EPI == EPI_LINEAR_BWD) v[e] = through<ACT>(t[e], v[e], d);
                         else { v[e] = through<ACT>(t[e], v[e], d, u[e]); u[e] = t[e] * f; }
                     }

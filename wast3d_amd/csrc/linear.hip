@@ -286,7 +286,7 @@ __global__ __launch_bounds__(256) void join_slices_kernel(GemmArgs a) {
             } else if (EPI == EPI_GATED) store1<OT>(o, act_fwd<ACT, OT>(x) * y);
             else {
                 float act, der;
-                act_both<ACT>(x, act, der);
+                act_both<ACT, OT>(x, act, der);
                 const float dy = in ? load1<OT>(a.dy + (m * a.N + n) * OB) : 0.f;
                 if (EPI == EPI_LINEAR_BWD) x = in ? through<ACT>(dy, x, der) : 0.f;
                 else { x = in ? through<ACT>(dy, x, der, y) : 0.f; y = in ? dy * act : 0.f; store1<OT>(o + a.half_out, y); c1 += y; }
@@ -346,7 +346,7 @@ __global__ __launch_bounds__(256) void dz_kernel(GemmArgs a) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     float f, d;
-                    act_both<ACT>(v[e], f, d);
+                    act_both<ACT, OT>(v[e], f, d);
                     if (GATED) { v[e] = through<ACT>(t[e], v[e], d, u[e]); u[e] = t[e] * f; c1[e] += u[e]; }
                     else v[e] = through<ACT>(t[e], v[e], d);
                     c0[e] += v[e];
