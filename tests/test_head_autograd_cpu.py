@@ -136,3 +136,15 @@ def test_compiled_calls_compute(host):
     for own, plain in calls:
         torch._dynamo.reset()
         _same(torch.compile(lambda t: own(2 * t) + 1, backend="eager")(x), plain(2 * x) + 1)
+
+
+def test_nothing_is_kept_for_a_residual_alone(host):
+    """A frozen layer on a stream that is trained: the residual's gradient is dy, and neither z nor the operands live until then."""
+    x, w, b, dy = torch.randn(R, K), torch.randn(N, K), torch.randn(N), torch.randn(R, N)
+    r = torch.randn(R, N, requires_grad=True)
+    y = ops.linear(x, w, b, activation="gelu", residual=r)
+    assert not [t for t in y.grad_fn.saved_tensors if t is not None]
+    assert torch.equal(torch.autograd.grad(y, r, dy)[0], dy)
+    for leaf in (x, w, b):                                 # any other gradient: the operands, and z (f32)
+        y = ops.linear(*(t.detach().requires_grad_(t is leaf) for t in (x, w, b)), activation="gelu", residual=r)
+        assert any(t is not None and t.shape == (R, N) for t in y.grad_fn.saved_tensors)

@@ -1655,17 +1655,20 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, residual, act):
         y = x.new_empty(x.shape[:-1] + w.shape[:1])
-        z = _kept(x, w.shape[0], 0) if act else None
+        ctx.act, ctx.saves = act, any(ctx.needs_input_grad[:3])
+        z = _kept(x, w.shape[0], 0) if act and ctx.saves else None
         raw_linear(x, w, bias, residual, act, y, z)
-        ctx.save_for_backward(x, w, bias, z)
-        ctx.act = act
+        if ctx.saves:                                               # (the residual's gradient is dy itself: nothing is kept for it)
+            ctx.save_for_backward(x, w, bias, z)
         return y
 
     @staticmethod
     @_first_order
     def backward(ctx, gy):
-        x, w, bias, z = ctx.saved_tensors
         want_x, want_w, want_b, want_r, _ = ctx.needs_input_grad
+        if not ctx.saves:
+            return None, None, None, gy if want_r else None, None
+        x, w, bias, z = ctx.saved_tensors
         N, K = w.shape
         dx = torch.empty_like(x) if want_x else None
         dw = torch.empty_like(w) if want_w else None
