@@ -643,7 +643,7 @@ int w3d_rms_norm_bwd(const void *x, const void *residual, const void *weight, in
                      void *workspace, size_t workspace_bytes, w3d_stream_t stream);
 /* Linear layer: y = act(x W^T + bias) + residual;  x [R,K], w [N,K], bias [N] or NULL, residual [R,N] or NULL, y [R,N].
  * Gated linear layer: y = act(x Wg^T + bg) * (x Wu^T + bu), one launch for both products.
- * act: W3D_ACT_*; gelu is z * Phi(z), its tail to less than half a step of the output's type.  Rows of x, w and y shorter than 8 MB (W3D_ERR_UNSUPPORTED otherwise).
+ * act: W3D_ACT_*; gelu is z * Phi(z), its tail to less than half a step of the output's type.  Rows of x, w and y shorter than 8 MB, fewer than 2^30 of them (W3D_ERR_UNSUPPORTED otherwise).
  * The _fp8 forms take e4m3 rows with one E8M0 exponent (1..254) each for x AND the weights, and write bf16 or f16 (residual and biases of out_dtype, biases also f32).
  * Forward calls can keep the values before the activation: z, f32 [R][w3d_linear_z_stride(N, gated)], 16-byte aligned, or NULL.
  * The _bwd forms need the forward's inputs and dy [R,N]; they take the z that was kept, 16-bit ones form it again without (z NULL; a linear layer with W3D_ACT_NONE needs none): dx [R,K], dw [N,K], dbias [N] (of bias_dtype), each optional; the residual's gradient is dy itself.

@@ -38,7 +38,7 @@ namespace {
 int launch_kernel(void (*kernel)(GemmArgs), int threads, int lds, const GemmArgs &a, int z, hipStream_t st) {
     if (lds > 65536) W3D_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     const int64_t blocks = (int64_t)a.tiles_m * a.tiles_n * a.slices;
-    if (blocks < 1 || blocks > 0x7fffffff) return W3D_ERR_UNSUPPORTED;
+    if (blocks < 1 || blocks * threads > 0xffffffffll) return W3D_ERR_UNSUPPORTED;             // (a launch has less than 2^32 threads)
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, 1, z), dim3(threads), lds, st, a);
     W3D_CHECK_LAUNCH();
     return W3D_OK;
