@@ -1651,6 +1651,26 @@ def _kept(x, N: int, gated: int):
     return x.new_empty((x.numel() // K, lib().w3d_linear_z_stride(N, gated)), dtype=torch.float32) if x.dtype == torch.float32 or K >= _KEEP_FROM else None
 
 
+def raw_linear_bwd(x, w, bias, act: int, dy, z=None, dx=None, dw=None, db=None):
+    """Gradients of contiguous rows into the tensors given, from dy [..., N] and the z that raw_linear kept (f32 rows with an activation need it; 16-bit ones form it again without).  The residual's is dy."""
+    N, K = w.shape
+    R, dt = x.numel() // K, _DTYPE_CODES[x.dtype]
+    nbytes = _backward_bytes(R, K, N, dt, act, 0, z is not None, _views(x, w, dy))
+    ws = _scratch(nbytes, x.device)
+    _launch("w3d_linear_bwd", x.get_device(), lib().w3d_linear_bwd, x.data_ptr(), w.data_ptr(), _at(bias), _code(bias), dy.data_ptr(), _at(z), R, K, N, dt, act, _at(dx), _at(dw), _at(db),
+            _at(ws), nbytes)
+
+
+def raw_gated_linear_bwd(x, wg, wu, bg, bu, act: int, dy, z=None, dx=None, dwg=None, dwu=None, dbg=None, dbu=None):
+    """The same of a gated layer."""
+    N, K = wg.shape
+    R, dt = x.numel() // K, _DTYPE_CODES[x.dtype]
+    nbytes = _backward_bytes(R, K, N, dt, act, 1, z is not None, _views(x, wg, wu))
+    ws = _scratch(nbytes, x.device)
+    _launch("w3d_gated_linear_bwd", x.get_device(), lib().w3d_gated_linear_bwd, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), _at(bg), _at(bu), _code(bg if bg is not None else bu),
+            dy.data_ptr(), _at(z), R, K, N, dt, act, _at(dx), _at(dwg), _at(dwu), _at(dbg), _at(dbu), _at(ws), nbytes)
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, residual, act):
@@ -1677,11 +1697,7 @@ class _Linear(torch.autograd.Function):
         if R == 0:
             dw, db = (t.zero_() if t is not None else None for t in (dw, db))
         elif want_x or want_w or want_b:
-            dt, gyc = _code(x), gy.contiguous()
-            nbytes = _backward_bytes(R, K, N, dt, ctx.act, 0, z is not None, _views(x, w, gyc))
-            ws = _scratch(nbytes, x.device)
-            _launch("w3d_linear_bwd", x.get_device(), lib().w3d_linear_bwd, x.data_ptr(), w.data_ptr(), _at(bias), _code(bias), gyc.data_ptr(), _at(z), R, K, N, dt, ctx.act, _at(dx), _at(dw),
-                    _at(db), _at(ws), nbytes)
+            raw_linear_bwd(x, w, bias, ctx.act, gy.contiguous(), z, dx, dw, db)
         return dx, dw, db, gy if want_r else None, None
 
 
@@ -1730,11 +1746,7 @@ class _GatedLinear(torch.autograd.Function):
         if R == 0:
             grads = [t.zero_() if t is not None else None for t in grads]
         else:
-            dt = _code(x)
-            nbytes = _backward_bytes(R, K, N, dt, ctx.act, 1, z is not None, _views(x, wg, wu))
-            ws, gyc = _scratch(nbytes, x.device), gy.contiguous()
-            _launch("w3d_gated_linear_bwd", x.get_device(), lib().w3d_gated_linear_bwd, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), _at(bg), _at(bu), _code(bg if bg is not None else bu),
-                    gyc.data_ptr(), _at(z), R, K, N, dt, ctx.act, *(_at(g) for g in grads), _at(ws), nbytes)
+            raw_gated_linear_bwd(x, wg, wu, bg, bu, ctx.act, gy.contiguous(), z, *grads)
         return (*grads, None)
 
 
