@@ -626,7 +626,7 @@ int w3d_raster_preprocess_backward(const W3dRasterIn *in, const int32_t *radii, 
 /* ---- layers of a feature head (no counterpart in the reference): rows of any width -> the rows the match takes.
  * Row-major, contiguous; any row count (0 is a no-op), any width, any element alignment of the pointers; aligned tensors (16 B, widths that are multiples of 16 B) run fastest.
  * dtype: W3D_DTYPE_F32 / BF16 / F16 for rows, weights, residual and outputs alike; weight_dtype / bias_dtype (norm weight, biases): dtype or W3D_DTYPE_F32.
- * All sums are f32 or wider, outputs are rounded once.  Results do not depend on the launch (no atomics).  Workspaces: 16-byte aligned, contents irrelevant before and after, one per call in flight.
+ * All sums are f32 or wider (e4m3 products: see the _fp8 forms), outputs are rounded once.  Results do not depend on the launch (no atomics).  Workspaces: 16-byte aligned, contents irrelevant before and after, one per call in flight.
  *
  * Root-mean-square norm: s = x + residual (residual NULL: s = x); rstd = 1 / sqrt(mean(s^2) + eps); y = s * rstd * weight (weight NULL: 1).
  *   w3d_rms_norm_fwd: y [R,d]; s [R,d] (optional, only with a residual; the sum, rounded); rstd f32 [R] (optional, for the backward pass).
@@ -645,6 +645,7 @@ int w3d_rms_norm_bwd(const void *x, const void *residual, const void *weight, in
  * Gated linear layer: y = act(x Wg^T + bg) * (x Wu^T + bu), one launch for both products.
  * act: W3D_ACT_*; gelu is z * Phi(z), its tail to less than half a step of the output's type.  Rows of x, w and y shorter than 8 MB, fewer than 2^30 of them (W3D_ERR_UNSUPPORTED otherwise).
  * The _fp8 forms take e4m3 rows with one E8M0 exponent (1..254) each for x AND the weights, and write bf16 or f16 (residual and biases of out_dtype, biases also f32).
+ *   The matrix instruction cuts the products of eight consecutive contraction elements at 2^-13 of the largest of them (at most 7 * 2^-13 of it in all); between such groups sums are f32.
  * Forward calls can keep the values before the activation: z, f32 [R][w3d_linear_z_stride(N, gated)], 16-byte aligned, or NULL.
  * The _bwd forms need the forward's inputs and dy [R,N]; they take the z that was kept, 16-bit ones form it again without (z NULL; a linear layer with W3D_ACT_NONE needs none): dx [R,K], dw [N,K], dbias [N] (of bias_dtype), each optional; the residual's gradient is dy itself.
  * workspace: w3d_linear_workspace_bytes (dtype W3D_DTYPE_FP8_E4M3 for the _fp8 forms) / w3d_linear_bwd_workspace_bytes (kept: 1 if z is passed); views: 1 if x, a weight matrix or dy may start at an address that

@@ -1791,7 +1791,8 @@ def _fp8_out(what, out_dtype, *tensors):
 
 def linear_fp8(q, scale, weight_q, weight_scale, bias=None, activation=None, residual=None, out_dtype=torch.bfloat16):
     """linear on 8-bit rows: q [R,K], weight_q [N,K] e4m3 bytes with one E8M0 exponent a row (quantize_rows_fp8, rms_norm_fp8), products on the fp8 matrix cores, the exponents applied to
-    the f32 sums.  y [R,N] of out_dtype (bf16 / f16), residual [R,N] of out_dtype, bias [N] of out_dtype or f32.  No gradient."""
+    the f32 sums.  The matrix instruction cuts the products of eight consecutive elements at 2^-13 of their largest (the sums of normal rows are right to 2^-16 of their magnitudes, of rows that span
+    e4m3's whole range to 2^-10).  y [R,N] of out_dtype (bf16 / f16), residual [R,N] of out_dtype, bias [N] of out_dtype or f32.  No gradient."""
     act, dev = _head_act(activation), q.device
     q, scale = _fp8_rows("linear_fp8", "q, scale", q, scale, dev)
     weight_q, weight_scale = _fp8_rows("linear_fp8", "weight_q, weight_scale", weight_q, weight_scale, dev)
