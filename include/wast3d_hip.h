@@ -648,6 +648,7 @@ int w3d_rms_norm_bwd(const void *x, const void *residual, const void *weight, in
  *   The matrix instruction cuts the products of eight consecutive contraction elements at 2^-13 of the largest of them (at most 7 * 2^-13 of it in all); between such groups sums are f32.
  * Forward calls can keep the values before the activation: z, f32 [R][w3d_linear_z_stride(N, gated)], 16-byte aligned, or NULL.
  * The _bwd forms need the forward's inputs and dy [R,N]; they take the z that was kept, 16-bit ones form it again without (z NULL; a linear layer with W3D_ACT_NONE needs none): dx [R,K], dw [N,K], dbias [N] (of bias_dtype), each optional; the residual's gradient is dy itself.
+ *   dz = dy * act'(z) (of a gated layer dy * up * act'(gate) and dy * act(gate)) is rounded to dtype, with dtype's range, before the products that form dx and dw; dbias is summed before that.
  * workspace: w3d_linear_workspace_bytes (dtype W3D_DTYPE_FP8_E4M3 for the _fp8 forms) / w3d_linear_bwd_workspace_bytes (kept: 1 if z is passed); views: 1 if x, a weight matrix or dy may start at an address that
  * is no multiple of 16 (room for aligned copies; widths that are no multiple of 16 bytes get theirs without it). */
 #define W3D_ACT_NONE 0

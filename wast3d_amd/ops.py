@@ -1708,8 +1708,10 @@ def _head_weight(what: str, name: str, w):
 
 
 def linear(x, weight, bias=None, activation=None, residual=None):
-    """y = act(x weight^T + bias) + residual in one launch.  x [..., K] f32 / bf16 / f16, weight [N,K] and residual [..., N] of x's type, bias [N] of x's type or f32;
-    activation None, 'relu', 'gelu' (z Phi(z)), 'silu' or 'sigmoid'.  Sums in f32, one rounding at the end.  Differentiable in everything; for it f32 calls, and 16-bit ones with K >= 896, keep the values before the activation in f32; other calls keep nothing but the inputs."""
+    """y = act(x weight^T + bias) + residual.  x [..., K] f32 / bf16 / f16, weight [N,K] and residual [..., N] of x's type, bias [N] of x's type or f32; activation None, 'relu', 'gelu' (z Phi(z)),
+    'silu' or 'sigmoid'.  Sums in f32, y rounded once.  One launch; a second one where the contraction is sliced (products of few tiles), another where rows that are not 16-byte aligned are copied first.
+    Differentiable in everything, first order.  dz = dy act'(z) is an operand of two matrix products and is rounded to x's type for them (with f16's range: scale the loss as for any f16 gradient); the bias
+    gradient is summed before that.  f32 calls, and 16-bit ones with K >= 896, keep the values before the activation in f32 until then; other calls keep nothing but the inputs."""
     _head_rows("linear", x)
     act = _head_act(activation)
     N, _ = _head_weight("linear", "weight", weight)
@@ -1760,8 +1762,9 @@ def _gated_args(what, x, wg, wu, bg, bu, dtype, bias_dtype):
 
 
 def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
-    """y = act(x w_gate^T + b_gate) * (x w_up^T + b_up): both products, the activation and the product in one launch.  x [..., K] f32 / bf16 / f16, weights [N,K] of x's type, biases
-    [N] of x's type or f32 (both alike); activation as in linear.  Sums in f32, one rounding at the end.  Differentiable in everything; for it f32 calls, and 16-bit ones with K >= 896, keep the values before the activation in f32; other calls keep nothing but the inputs."""
+    """y = act(x w_gate^T + b_gate) * (x w_up^T + b_up): both products, the activation and the product in one launch (and those of linear).  x [..., K] f32 / bf16 / f16, weights [N,K] of x's type, biases
+    [N] of x's type or f32 (both alike); activation as in linear.  Sums in f32, y rounded once.  Differentiable in everything, as linear: both halves of dz are rounded to x's type, and f32 calls, and 16-bit
+    ones with K >= 896, keep the values before the activation in f32."""
     _head_rows("gated_linear", x)
     act = _head_act(activation)
     N, w_gate, w_up, b_gate, b_up = _gated_args("gated_linear", x, w_gate, w_up, b_gate, b_up, x.dtype, x.dtype)
