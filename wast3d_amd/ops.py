@@ -1445,13 +1445,13 @@ def _head_eps(eps) -> float:
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
-_dispatch_mode, _PROXY = torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY
+_modes, _dispatch_mode, _PROXY = torch._C._len_torch_dispatch_stack, torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY
 _tracing = torch._C._get_tracing_state
 
 
 def _launch(what: str, index: int, fn, *args):
     """One call of the library on the current stream of the tensors' own device (the stream is the last argument; tensors travel as addresses, None as NULL)."""
-    if _dispatch_mode(_PROXY) is not None:
+    if _modes() and _dispatch_mode(_PROXY) is not None:
         raise W3dError(f"{what}: a symbolic trace (make_fx) cannot record the call, only the allocation of its output")
     if index == torch.cuda.current_device():
         clear_stale_hip_error()
