@@ -2,8 +2,8 @@
 
 One nonzero column in x and in the weights makes z an exact product: what is left is the activation's own error.  W = 2^-24.  An exponential of an argument a that was rounded has a relative error of
 |a| W: gelu of f32 layers and gelu' evaluate exp(-z^2 / 2) (its argument rounded three times: 1.5 z^2 W) and a polynomial of relative error 1.4e-7 (2.4 W, 6 W in f32), silu and sigmoid exp(-|z|).
-Outputs of 16-bit layers take a polynomial in the exponent for gelu's tail, fitted to less than half a step of the type: bf16 1.2e-3 of it, f16 2.1e-4 up to z = -8 and 5e-15 beyond; 2.5e-7 next to
-zero.  Outputs are rounded once; results whose exponential is below 2^-126 may be zero."""
+Outputs of 16-bit layers take a polynomial in the exponent for gelu's tail, fitted to less than half a step of the type: bf16 1.2e-3 of it, f16 2.1e-4 up to z = -8 and less than all of it (5e-15) beyond; 2.5e-7
+next to zero.  Outputs are rounded once; results whose exponential is below 2^-126 may be zero."""
 import math
 
 import pytest
@@ -52,7 +52,7 @@ def forward_bound(z, a, act, dt):
     if act == "gelu":
         e = (16 + 2 * z * z) * W * a.abs()
         if dt != F32:
-            e = e + torch.where(z < -1, (2.1e-4 if dt == F16 else 1.2e-3) * a.abs() + (5.1e-15 if dt == F16 else 0.0), 2.5e-7)
+            e = e + torch.where(z < -1, (torch.where(z < -8, 1.0, 2.1e-4) if dt == F16 else 1.2e-3) * a.abs(), 2.5e-7)
         return e
     return (12 + 2 * z.abs()) * W * a.abs()
 
@@ -134,3 +134,16 @@ def test_relu_passes_no_gradient_where_it_is_off(R, K, N, dt, kept, monkeypatch)
     v = torch.zeros_like(w)
     for got, want in zip(torch.autograd.grad(ops.gated_linear(x, w, v, b, None, activation="relu"), (w, b), bad), torch.autograd.grad(ops.gated_linear(x, w, v, b, None, activation="relu"), (w, b), dy)):
         assert got.isfinite().all() and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dt", [F16, F32])
+@pytest.mark.parametrize("act", ["gelu", "silu", "sigmoid", "relu"])
+def test_a_closed_gate_stays_closed(act, dt):
+    """The other half of a gated layer is f32 inside and can be far past its type's range: 6e4 * 6e4 * 16 here, times act(z) of a closed gate."""
+    for R, K, N in SHAPES:
+        x, w, v = torch.zeros(R, K, dtype=dt, device="cuda"), torch.zeros(N, K, dtype=dt, device="cuda"), torch.zeros(N, K, dtype=dt, device="cuda")
+        x[:, :16], v[:, :16] = 6e4, 6e4
+        x[:, K - 1], w[:, K - 1] = -100.0, 1.0
+        y = ops.gated_linear(x, w, v, activation=act).double()
+        # silu's own value; gelu's and relu's is 0.  exp(-100) = 3.72e-44 lies among f32's subnormals, 2^-149 = 1.4e-45 apart: half a step is 2 % of it
+        assert float(y.abs().max()) <= 100 * (math.exp(-100.0) + 2.0 ** -149) * 16 * 3.6e9 * 1.01

@@ -71,8 +71,8 @@ constexpr uint32_t OUT_OF_RANGE = 0x80000000u;   // buffer offset past num_recor
 //   Phi(-h) = e t P(t), e = exp(-h^2 / 2), t = 1 / (1 + 0.3 h): P of degree 7, fitted on [0, 14.3] to the smallest maximum of the relative error, 1.4e-7; in f32 2^-21 and the argument's rounding (h^2 2^-24), which
 //     z's own last place costs too.  For f32 layers and for derivatives, which need e themselves.
 //   log2 Phi(-h) by a polynomial, for the outputs of 16-bit layers, where the epilogue is what a short contraction waits for (one polynomial of degree 10 for both: 65 536 x 256 -> 1 024 88 us in bf16 and 90 in f16, these 84 and 78).  bf16: degree 8,
-//     fitted on [0, 13.2] to h |error of Phi| <= 2.5e-7 and 1.2e-3 of Phi (half a step is 3.9e-3); f16: degree 7 on [0, 8], 2.3e-7 and 2.1e-4 (4.9e-4), and h Phi(-h) stays at 5e-15 past 8: less than any f16
-//     number's last place can show of it, times the largest.
+//     fitted on [0, 13.2] to h |error of Phi| <= 2.5e-7 and 1.2e-3 of Phi (half a step is 3.9e-3); f16: degree 7 on [0, 8], 2.3e-7 and 2.1e-4 (4.9e-4); past 8,
+//     where no f16 number shows it unless the other half is large, it falls a little faster than Phi (0.3 % of it at 9, 3 % at 10).
 // Past 13.2 (14.4 in the first form) the exponential is below 2^-126 and becomes 0.
 __device__ __forceinline__ float normal_tail(float h, float e) {
     const float t = __builtin_amdgcn_rcpf(fmaf(h, 0.3f, 1.0f));
@@ -102,7 +102,7 @@ __device__ __forceinline__ float act_fwd(float z) {
     if (ACT == ACT_RELU) return z < 0.f ? 0.f : z;                       // (a NaN stays)
     if (ACT == ACT_GELU) {
         const bool wide = OT == W3D_DTYPE_F32;
-        const float h = fminf(fabsf(z), wide ? 16.0f : OT == W3D_DTYPE_F16 ? 8.0f : 13.2f), tail = wide ? normal_tail(h, exp_half_square(h)) : normal_tail_16<OT>(h);
+        const float h = fminf(fabsf(z), wide ? 16.0f : 13.2f), tail = wide ? normal_tail(h, exp_half_square(h)) : normal_tail_16<OT>(h);
         return fmaf(-h, tail, __builtin_elementwise_maximum(z, 0.f));    // (a NaN stays)
     }
     if (OT == W3D_DTYPE_F32 && (ACT == ACT_SILU || ACT == ACT_SIGMOID)) {
