@@ -2,8 +2,8 @@
 
 One nonzero column in x and in the weights makes z an exact product: what is left is the activation's own error.  W = 2^-24.  An exponential of an argument a that was rounded has a relative error of
 |a| W: gelu of f32 layers and gelu' evaluate exp(-z^2 / 2) (its argument rounded three times: 1.5 z^2 W) and a polynomial of relative error 1.4e-7 (2.4 W, 6 W in f32), silu and sigmoid exp(-|z|).
-Outputs of 16-bit layers take a polynomial in the exponent for gelu's tail, fitted to less than half a step of the type: bf16 1.2e-3 of it, f16 2.1e-4 up to z = -8 and less than all of it (5e-15) beyond; 2.5e-7
-next to zero.  Outputs are rounded once; results whose exponential is below 2^-126 may be zero."""
+Outputs of 16-bit layers take a polynomial in the exponent for gelu's tail, fitted to less than half a step of the type: bf16 2.1e-3 of it up to z = -10.5,
+f16 2.1e-4 up to -8, and less than all of it beyond (of 5e-25 and 5e-15); 2.5e-7 next to zero.  Outputs are rounded once; results whose exponential is below 2^-126 may be zero."""
 import math
 
 import pytest
@@ -52,7 +52,7 @@ def forward_bound(z, a, act, dt):
     if act == "gelu":
         e = (16 + 2 * z * z) * W * a.abs()
         if dt != F32:
-            e = e + torch.where(z < -1, (torch.where(z < -8, 1.0, 2.1e-4) if dt == F16 else 1.2e-3) * a.abs(), 2.5e-7)
+            e = e + torch.where(z < -1, (torch.where(z < -8, 1.0, 2.1e-4) if dt == F16 else torch.where(z < -10.5, 1.0, 2.1e-3)) * a.abs(), 2.5e-7)
         return e
     return (12 + 2 * z.abs()) * W * a.abs()
 

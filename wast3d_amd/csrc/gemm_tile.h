@@ -70,9 +70,9 @@ constexpr uint32_t OUT_OF_RANGE = 0x80000000u;   // buffer offset past num_recor
 // gelu(z) = z Phi(z) = max(z, 0) - h Phi(-h), h = |z|, with Phi(-h) to a relative bound: a gated layer multiplies the tail by what it likes.  Two forms of it:
 //   Phi(-h) = e t P(t), e = exp(-h^2 / 2), t = 1 / (1 + 0.3 h): P of degree 7, fitted on [0, 14.3] to the smallest maximum of the relative error, 1.4e-7; in f32 2^-21 and the argument's rounding (h^2 2^-24), which
 //     z's own last place costs too.  For f32 layers and for derivatives, which need e themselves.
-//   log2 Phi(-h) by a polynomial, for the outputs of 16-bit layers, where the epilogue is what a short contraction waits for (one polynomial of degree 10 for both: 65 536 x 256 -> 1 024 88 us in bf16 and 90 in f16, these 84 and 78).  bf16: degree 8,
-//     fitted on [0, 13.2] to h |error of Phi| <= 2.5e-7 and 1.2e-3 of Phi (half a step is 3.9e-3); f16: degree 7 on [0, 8], 2.3e-7 and 2.1e-4 (4.9e-4); past 8,
-//     where no f16 number shows it unless the other half is large, it falls a little faster than Phi (0.3 % of it at 9, 3 % at 10).
+//   log2 Phi(-h) by a polynomial of degree 7, for the outputs of 16-bit layers, where the epilogue is what a short contraction waits for (us at 65 536 x 256 -> 1 024, gated: degree 7 in either type 123 - 124,
+//     degree 8 in bf16 126; linear, degree 10 for both: 88 in bf16 and 90 in f16 instead of 82 and 79).  bf16: fitted on [0, 10.5] to h |error of Phi| <= 1.9e-7 and 2.1e-3 of Phi (half a step is 3.9e-3); f16: on
+//     [0, 8], 2.3e-7 and 2.1e-4 (4.9e-4).  Past its range, where Phi is below 5e-26 (7e-16), either falls a little faster than Phi.
 // Past 13.2 (14.4 in the first form) the exponential is below 2^-126 and becomes 0.
 __device__ __forceinline__ float normal_tail(float h, float e) {
     const float t = __builtin_amdgcn_rcpf(fmaf(h, 0.3f, 1.0f));
@@ -81,11 +81,9 @@ __device__ __forceinline__ float normal_tail(float h, float e) {
 }
 template <int OT>
 __device__ __forceinline__ float normal_tail_16(float h) {
-    float p;
-    if (OT == W3D_DTYPE_F16)
-        p = fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, -1.4817135e-06f, 5.4606211e-05f), -0.000879072f), 0.0083331997f), -0.05368023f), -0.45865902f), -1.1512053f), -0.99999714f);
-    else
-        p = fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, 4.2807482e-8f, -2.5480883e-6f), 6.4550513e-5f), -9.2313864e-4f), 8.4335105e-3f), -5.3797774e-2f), -4.5859316e-1f), -1.1512195f), -9.9999672e-1f);
+    const float p = OT == W3D_DTYPE_F16
+        ? fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, -1.4817135e-06f, 5.4606211e-05f), -0.000879072f), 0.0083331997f), -0.05368023f), -0.45865902f), -1.1512053f), -0.99999714f)
+        : fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, -1.2373911e-06f, 4.9450155e-05f), -0.00084103353f), 0.0082123438f), -0.053499933f), -0.45878318f), -1.1511714f), -0.99999928f);
     return __builtin_amdgcn_exp2f(p);
 }
 // e = exp(-|z|), s = 1 / (1 + exp(-z)) and q = 1 - s without the cancellation (1 - s is 0 past z = 17, and wrong by 2^-24 before it).  The exponential's argument is rounded in 16-bit layers: |z| 2^-24 of the value.
