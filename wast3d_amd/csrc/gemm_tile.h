@@ -69,18 +69,21 @@ constexpr uint32_t OUT_OF_RANGE = 0x80000000u;   // buffer offset past num_recor
 // ---- activations.  a = act(z), d = act'(z).
 // gelu(z) = z Phi(z) = max(z, 0) - h Phi(-h), h = |z|, with Phi(-h) to a relative bound: a gated layer multiplies the tail by what it likes.  Two forms of it:
 //   Phi(-h) = e t P(t), e = exp(-h^2 / 2), t = 1 / (1 + 0.3 h): P of degree 7, fitted on [0, 14.3] to the smallest maximum of the relative error, 1.4e-7; in f32 2^-21 and the argument's rounding (h^2 2^-24), which
-//     z's own last place costs too.  For f32 layers and for derivatives, which need e themselves.
-//   log2 Phi(-h) by a polynomial of degree 7, for the outputs of 16-bit layers, where the epilogue is what a short contraction waits for (us at 65 536 x 256 -> 1 024, gated: degree 7 in either type 123 - 124,
+//     z's own last place costs too.  For f32 layers.
+//   log2 Phi(-h) by a polynomial of degree 7, for 16-bit layers, where the epilogue is what a short contraction waits for (us at 65 536 x 256 -> 1 024, gated: degree 7 in either type 123 - 124,
 //     degree 8 in bf16 126; linear, degree 10 for both: 88 in bf16 and 90 in f16 instead of 82 and 79).  bf16: fitted on [0, 10.5] to h |error of Phi| <= 1.9e-7 and 2.1e-3 of Phi (half a step is 3.9e-3); f16: on
 //     [0, 8], 2.3e-7 and 2.1e-4 (4.9e-4).  Past its range, where Phi is below 5e-26 (7e-16), either falls a little faster than Phi.
+//     (The first form in their derivatives: 65 536 x 256 -> 1 024 f16 in training 276 us instead of 270, bf16 the same.)
 // Past 13.2 (14.4 in the first form) the exponential is below 2^-126 and becomes 0.
-__device__ __forceinline__ float normal_tail(float h, float e) {
-    const float t = __builtin_amdgcn_rcpf(fmaf(h, 0.3f, 1.0f));
-    const float p = fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, 3.5531368e-2f, -1.5657105e-1f), 2.0520240e-1f), -5.2566256e-2f), 1.2794091e-1f), 1.0010950e-1f), 1.2072159e-1f), 1.1963145e-1f);
-    return e * (t * p);
-}
+__device__ __forceinline__ float exp_half_square(float h) { return __builtin_amdgcn_exp2f(h * h * -0.72134752f); }
+template <int OT> constexpr float FAR_TAIL = OT == W3D_DTYPE_F32 ? 16.0f : 13.2f;               // (Phi is 0 there: below 2^-126)
 template <int OT>
-__device__ __forceinline__ float normal_tail_16(float h) {
+__device__ __forceinline__ float normal_tail(float h, float e) {
+    if (OT == W3D_DTYPE_F32) {
+        const float t = __builtin_amdgcn_rcpf(fmaf(h, 0.3f, 1.0f));
+        const float p = fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, 3.5531368e-2f, -1.5657105e-1f), 2.0520240e-1f), -5.2566256e-2f), 1.2794091e-1f), 1.0010950e-1f), 1.2072159e-1f), 1.1963145e-1f);
+        return e * (t * p);
+    }
     const float p = OT == W3D_DTYPE_F16
         ? fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, -1.4817135e-06f, 5.4606211e-05f), -0.000879072f), 0.0083331997f), -0.05368023f), -0.45865902f), -1.1512053f), -0.99999714f)
         : fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, fmaf(h, -1.2373911e-06f, 4.9450155e-05f), -0.00084103353f), 0.0082123438f), -0.053499933f), -0.45878318f), -1.1511714f), -0.99999928f);
@@ -93,14 +96,12 @@ __device__ __forceinline__ void sigmoid_pair(float z, float &s, float &q) {
     s = z < 0.f ? er : r;
     q = z < 0.f ? r : er;
 }
-__device__ __forceinline__ float exp_half_square(float h) { return __builtin_amdgcn_exp2f(h * h * -0.72134752f); }
 // OT: the layer's output type
 template <int ACT, int OT>
 __device__ __forceinline__ float act_fwd(float z) {
     if (ACT == ACT_RELU) return z < 0.f ? 0.f : z;                       // (a NaN stays)
     if (ACT == ACT_GELU) {
-        const bool wide = OT == W3D_DTYPE_F32;
-        const float h = fminf(fabsf(z), wide ? 16.0f : 13.2f), tail = wide ? normal_tail(h, exp_half_square(h)) : normal_tail_16<OT>(h);
+        const float h = fminf(fabsf(z), FAR_TAIL<OT>), tail = normal_tail<OT>(h, exp_half_square(h));
         return fmaf(-h, tail, __builtin_elementwise_maximum(z, 0.f));    // (a NaN stays)
     }
     if (OT == W3D_DTYPE_F32 && (ACT == ACT_SILU || ACT == ACT_SIGMOID)) {
@@ -117,7 +118,7 @@ __device__ __forceinline__ void act_both(float z, float &a, float &d) {
     if (ACT == ACT_NONE) { a = z; d = 1.f; }
     else if (ACT == ACT_RELU) { a = z < 0.f ? 0.f : z; d = z > 0.f ? 1.f : 0.f; }
     else if (ACT == ACT_GELU) {
-        const float h = fminf(fabsf(z), 16.0f), e = exp_half_square(h), tail = normal_tail(h, e);
+        const float h = fminf(fabsf(z), FAR_TAIL<OT>), e = exp_half_square(z), tail = normal_tail<OT>(h, e);
         a = fmaf(-h, tail, z < 0.f ? 0.f : z);
         d = fmaf(z * 0.39894228f, e, z < 0.f ? tail : 1.0f - tail);
     } else {
